@@ -1,10 +1,13 @@
 """Shared plumbing of the op wrappers."""
 from __future__ import annotations
 
+import contextlib
+
 import torch
 
 from .. import _native
 
+_SAME_DEVICE = contextlib.nullcontext()
 
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
@@ -26,6 +29,14 @@ def on_gpu(*tensors) -> bool:
     if any(flags) and not all(flags):
         raise ValueError("op received a mix of host and device tensors")
     return flags[0]
+
+
+def launch_device(device: torch.device):
+    """Context in which ``device`` is the current one (a launch on a stream of another device than the current one
+    fails); free where it already is, or where ``device`` names none."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return _SAME_DEVICE
+    return torch.cuda.device(device)
 
 
 def hip():

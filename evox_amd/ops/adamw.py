@@ -1,0 +1,226 @@
+"""AdamW over many tensors at once, moments in 32 or in 8 bits (kernel: ``csrc/adamw.hip``).
+
+The moments of all leaves live in one flat buffer each: leaf after leaf in the order given, every leaf padded with zeros
+to a multiple of ``ALIGN`` elements.  A state is a dict of tensors:
+
+``count``                  float32 scalar, steps taken
+``mu``, ``nu``             ``(total,)`` float32, or uint8 codes
+``mu_scale``, ``nu_scale`` (8 bits only) ``(total / BLOCK,)`` uint8: ``BLOCK`` neighbours share the unit ``2^(scale - 127)``
+
+Codes: ``mu`` sign, 4 exponent and 3 mantissa bits, ``nu`` 5 exponent and 3 mantissa bits; exponent e > 0 and mantissa m stand
+for ``(8 + m) 2^(e - 1)`` units, e = 0 for ``m`` units, ``0x7f`` / ``0xff`` for NaN (an infinite moment becomes NaN).  A
+block's unit is the smallest that holds its largest magnitude; magnitudes are rounded down or up by a dither that is
+equidistributed over the steps, so slow averages move as they should (rounding to nearest would freeze them)."""
+from __future__ import annotations
+
+import ctypes
+import math
+from typing import List, Sequence
+
+import torch
+
+from .. import _native
+from ._util import DTYPE_CODE, check, hip, launch_device, on_gpu, stream_of
+
+ALIGN = 256
+BLOCK = 32
+_PHASE, _STEP_MU, _STEP_NU = 0x9E3779B9, 0x91E10DA5, 0xC13FA9A9
+
+P, I, I64 = _native.P, _native.I, _native.I64
+_native.register_hip_api({
+    "evox_hip_adamw": (I, [I, I, P, P, P, P, P, P, I, P, P, P, P, P, P, P, P, P, P, I64, P]),
+    "evox_hip_adamw_read": (I, [P, P, P, P, P, P, I64, P]),
+})
+
+
+def padded(n: int) -> int:
+    """Elements that a leaf of ``n`` takes in the flat moments."""
+    return -(-n // ALIGN) * ALIGN
+
+
+def adamw_init(params: Sequence[torch.Tensor], state_bits: int = 32) -> dict:
+    """The state before the first step."""
+    _check_leaves(params, "params")
+    if state_bits not in (8, 32):
+        raise ValueError(f"state_bits must be 8 or 32, got {state_bits}")
+    dev = params[0].device
+    total = sum(padded(p.numel()) for p in params)
+    state = {"count": torch.zeros((), dtype=torch.float32, device=dev)}
+    if state_bits == 32:
+        state["mu"] = torch.zeros(total, dtype=torch.float32, device=dev)
+        state["nu"] = torch.zeros(total, dtype=torch.float32, device=dev)
+    else:
+        for name in ("mu", "nu"):
+            state[name] = torch.zeros(total, dtype=torch.uint8, device=dev)
+            state[name + "_scale"] = torch.ones(total // BLOCK, dtype=torch.uint8, device=dev)
+    return state
+
+
+def _check_leaves(leaves, what):
+    if not leaves:
+        raise ValueError(f"adamw needs at least one tensor in {what}")
+    for t in leaves:
+        if not isinstance(t, torch.Tensor) or t.dtype not in DTYPE_CODE:
+            raise TypeError(f"adamw takes float32 or bfloat16 tensors, got "
+                            f"{t.dtype if isinstance(t, torch.Tensor) else type(t).__name__} in {what}")
+        if t.device != leaves[0].device:
+            raise ValueError(f"adamw: the tensors of {what} are on different devices")
+
+
+def _check_state(state, device, total):
+    bits = 8 if state["mu"].dtype == torch.uint8 else 32
+    want = {"count": (torch.float32, 1), "mu": (torch.float32 if bits == 32 else torch.uint8, total)}
+    want["nu"] = want["mu"]
+    if bits == 8:
+        want["mu_scale"] = want["nu_scale"] = (torch.uint8, total // BLOCK)
+    for name, (dtype, n) in want.items():
+        t = state.get(name)
+        if t is None or t.dtype != dtype or t.numel() != n or t.device != device or not t.is_contiguous():
+            raise ValueError(f"adamw: the state's {name!r} does not belong to these parameters "
+                             f"(expected {n} contiguous {dtype} elements on {device})")
+    return bits
+
+
+def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], state: dict, *, learning_rate: float,
+               b1: float = 0.9, b2: float = 0.999, eps: float = 1e-8, weight_decay: float = 1e-2, decay: Sequence[bool] = None,
+               updates: bool = False):
+    """One step: ``(new parameters, new state)``, or with ``updates`` the amounts to add in the place of the parameters.
+
+    ``params`` and ``grads`` are lists of float32 or bfloat16 tensors of pairwise equal shapes (any strides; types may differ
+    from leaf to leaf and between a parameter and its gradient), ``decay`` says for each leaf whether ``weight_decay`` applies
+    to it (default: to all).  Arithmetic is float32 whatever the types, results have the parameters' types and are contiguous.
+    Nothing is written in place, no autograd graph is built.  On a GPU all leaves take one launch per 72 of them."""
+    _check_leaves(params, "params")
+    _check_leaves(grads, "grads")
+    if len(params) != len(grads):
+        raise ValueError(f"adamw: {len(params)} parameters but {len(grads)} gradients")
+    total = 0
+    for p, g in zip(params, grads):
+        if p.shape != g.shape:
+            raise ValueError(f"adamw: a parameter of shape {tuple(p.shape)} has a gradient of shape {tuple(g.shape)}")
+        total += padded(p.numel())
+    device = params[0].device
+    if grads[0].device != device:
+        raise ValueError("adamw: parameters and gradients are on different devices")
+    if decay is not None and len(decay) != len(params):
+        raise ValueError("adamw: decay needs one entry per parameter")
+    bits = _check_state(state, device, total)
+    hyper = (learning_rate, b1, b2, 1 - b1, 1 - b2, eps, weight_decay, math.log(b1) if b1 else -math.inf,
+             math.log(b2) if b2 else -math.inf)
+    if not on_gpu(params[0]) or total == 0:
+        return adamw_step_reference(params, grads, state, hyper, bits, decay, updates)
+    return _step_hip(params, grads, state, hyper, bits, decay, updates, total, device)
+
+
+def _step_hip(params, grads, state, hyper, bits, decay, updates, total, device):
+    n = len(params)
+    params = [p if p.is_contiguous() else p.contiguous() for p in params]
+    grads = [g if g.is_contiguous() else g.contiguous() for g in grads]
+    out = [torch.empty(p.shape, dtype=p.dtype, device=device) for p in params]
+    new = {k: torch.empty_like(v) for k, v in state.items()}
+    table = (ctypes.c_int64 * (5 * n))(
+        *[p.data_ptr() for p in params], *[g.data_ptr() for g in grads], *[o.data_ptr() for o in out], *[p.numel() for p in params],
+        *[(p.dtype is torch.bfloat16) | (g.dtype is torch.bfloat16) << 1 | (decay is None or bool(decay[k])) << 2
+          for k, (p, g) in enumerate(zip(params, grads))])
+    at = ctypes.addressof(table)
+    h = (ctypes.c_float * 9)(*hyper)
+    scales = [state["mu_scale"].data_ptr(), state["nu_scale"].data_ptr()] if bits == 8 else [None, None]
+    new_scales = [new["mu_scale"].data_ptr(), new["nu_scale"].data_ptr()] if bits == 8 else [None, None]
+    with launch_device(device):
+        check(hip().evox_hip_adamw(bits, n, at, at + 8 * n, at + 16 * n, at + 24 * n, at + 32 * n, ctypes.addressof(h), int(updates),
+                                   state["count"].data_ptr(), new["count"].data_ptr(), state["mu"].data_ptr(),
+                                   state["nu"].data_ptr(), *scales, new["mu"].data_ptr(), new["nu"].data_ptr(), *new_scales,
+                                   total, stream_of(params[0])), "adamw")
+    return out, new
+
+
+def adamw_moments(state: dict):
+    """The flat moments ``(mu, nu)`` that a state holds: float32 as they are, or the bfloat16 values that 8-bit codes stand for
+    (exact: a code has four significant bits and its unit is a power of two)."""
+    if state["mu"].dtype != torch.uint8:
+        return state["mu"], state["nu"]
+    names = ("mu", "nu", "mu_scale", "nu_scale")
+    total = state["mu"].numel()
+    device = state["mu"].device
+    if total % ALIGN:
+        raise ValueError(f"adamw: moments hold a multiple of {ALIGN} elements, got {total}")
+    _check_state(state, device, total)
+    if not on_gpu(state["mu"]):
+        return tuple(decode(state[k], state[k + "_scale"], k == "mu").to(torch.bfloat16) for k in ("mu", "nu"))
+    out = torch.empty((2, total), dtype=torch.bfloat16, device=device)
+    mu, nu = out.unbind(0)
+    with launch_device(device):
+        check(hip().evox_hip_adamw_read(*(state[k].data_ptr() for k in names), mu.data_ptr(), nu.data_ptr(), total,
+                                        stream_of(out)), "adamw_read")
+    return mu, nu
+
+
+# ------------------------------------------------------------------ the same in tensor operations (host tensors, oracle)
+
+def _pow2(e: torch.Tensor) -> torch.Tensor:
+    return torch.ldexp(torch.ones(e.shape, dtype=torch.float32, device=e.device), e)
+
+
+def decode(codes: torch.Tensor, scale: torch.Tensor, signed: bool) -> torch.Tensor:
+    c = codes.to(torch.int64)
+    mag = c & 0x7F if signed else c
+    e, m = mag >> 3, mag & 7
+    v = torch.where(e > 0, (m + 8) << (e - 1).clamp(min=0), m).to(torch.float32)
+    v = v * _pow2(scale.to(torch.int32) - 127).repeat_interleave(BLOCK)
+    v = torch.where(mag == (0x7F if signed else 0xFF), torch.full_like(v, math.nan), v)
+    return torch.where(c > 0x7F, -v, v) if signed else v
+
+
+def dither(step: int, n: int, constant: int, device=None) -> torch.Tensor:
+    phase = torch.arange(n, dtype=torch.int64, device=device) * _PHASE + step * constant
+    return ((phase & 0xFFFFFFFF) >> 16).to(torch.float32) * 2.0 ** -16
+
+
+def encode(v: torch.Tensor, u: torch.Tensor, signed: bool):
+    """``(codes, scales)`` of a flat float32 tensor, rounded by the dither ``u``."""
+    bits = 14 if signed else 30
+    finite = torch.isfinite(v)
+    mag = torch.where(finite, v.abs(), torch.zeros_like(v))
+    big = mag.view(-1, BLOCK).amax(1)
+    unit = ((big.view(torch.int32) >> 23) - 130 - bits).clamp(min=-126)
+    unit = unit + (big > 14.0 * 2.0 ** bits * _pow2(unit)).to(torch.int32)
+    y = torch.ldexp(mag, -unit.repeat_interleave(BLOCK))
+    shift = ((y.view(torch.int32) >> 23) - 127).clamp(min=3) - 3
+    code = torch.floor(torch.ldexp(y, -shift) + u).to(torch.int32) + 8 * shift
+    if signed:
+        code = torch.where(finite, code, torch.full_like(code, 0x7F)) | (torch.signbit(v).to(torch.int32) << 7)
+    else:
+        code = torch.where((code == 0) & (v > 0), torch.ones_like(code), code)
+        code = torch.where(finite, code, torch.full_like(code, 0xFF))
+    return code.to(torch.uint8), (unit + 127).to(torch.uint8)
+
+
+def adamw_step_reference(params, grads, state, hyper, bits, decay=None, updates=False):
+    lr, b1, b2, omb1, omb2, eps, wd, _, _ = hyper
+    count = state["count"] + 1
+    t = float(count)
+    c1, c2 = -math.expm1(t * math.log(b1)) if b1 else 1.0, -math.expm1(t * math.log(b2)) if b2 else 1.0
+    new = {"count": count}
+    if bits == 32:
+        mu, nu = state["mu"].clone(), state["nu"].clone()
+    else:
+        mu, nu = decode(state["mu"], state["mu_scale"], True), decode(state["nu"], state["nu_scale"], False)
+    out: List[torch.Tensor] = []
+    at = 0
+    for k, (p, g) in enumerate(zip(params, grads)):
+        n = p.numel()
+        p32, g32 = p.detach().reshape(-1).float(), g.detach().reshape(-1).float()
+        m, v = mu[at:at + n], nu[at:at + n]
+        m.copy_(b1 * m + omb1 * g32)
+        v.copy_(b2 * v + omb2 * g32 * g32)
+        d = (m / c1) / (torch.sqrt(v / c2) + eps)
+        if wd and (decay is None or decay[k]):
+            d = d + wd * p32
+        out.append((-lr * d if updates else p32 - lr * d).to(p.dtype).reshape(p.shape))
+        at += padded(n)
+    if bits == 32:
+        new["mu"], new["nu"] = mu, nu
+    else:
+        for name, x, c in (("mu", mu, _STEP_MU), ("nu", nu, _STEP_NU)):
+            new[name], new[name + "_scale"] = encode(x, dither(int(t), x.numel(), c, x.device), name == "mu")
+    return out, new

@@ -72,7 +72,80 @@ def rmsprop(learning_rate: float, decay: float = 0.9, eps: float = 1e-8) -> Grad
     return GradientTransformation(init, update)
 
 
-_BY_NAME = {"adam": adam, "sgd": sgd, "rmsprop": rmsprop}
+class AdamW(GradientTransformation):
+    """What :func:`adamw` returns: ``init`` and ``update`` like every optimizer here, and
+
+    ``step(grads, state, params) -> (params, state)``  one whole step (on a GPU one launch per 72 leaves; parameters in
+                                                       bfloat16 are rounded once);
+    ``moments(state, params=None) -> (mu, nu)``        the running averages as trees like ``params``, or flat (leaf after
+                                                       leaf, each padded to a multiple of 256) where none are given."""
+
+    step: Callable
+    moments: Callable
+
+
+def adamw(learning_rate: float, b1: float = 0.9, b2: float = 0.999, eps: float = 1e-8, weight_decay: float = 1e-2,
+          state_bits: int = 32, mask=None) -> AdamW:
+    """Adam with decoupled weight decay, all leaves of a tree in one kernel (``ops.adamw``).
+
+    ``state_bits=8`` keeps both moments in 8 bits (2.06 bytes per parameter instead of 8; see ``ops.adamw`` for the format).
+    ``mask``: a tree of truth values like the parameters, or a function that makes one from them; ``weight_decay`` applies
+    where it is true (default: everywhere).  Leaves are float32 or bfloat16."""
+    if not (learning_rate >= 0 and 0 <= b1 < 1 and 0 <= b2 < 1 and eps >= 0 and weight_decay >= 0):
+        raise ValueError("adamw: learning_rate, eps and weight_decay must not be negative, b1 and b2 lie in [0, 1)")
+    if state_bits not in (8, 32):
+        raise ValueError(f"state_bits must be 8 or 32, got {state_bits}")
+    from ..ops import adamw as _aw
+
+    def init(params):
+        return _aw.adamw_init(_tree.tree_leaves(params), state_bits)
+
+    def run(grads, state, params, updates):
+        if params is None:
+            raise ValueError("adamw needs the parameters next to the gradients")
+        leaves, treedef = _tree.tree_flatten(params)
+        g, gdef = _tree.tree_flatten(grads)
+        if gdef != treedef:
+            raise ValueError(f"adamw: structure mismatch\n  {treedef}\n  {gdef}")
+        decay = None
+        if mask is not None:
+            decay, mdef = _tree.tree_flatten(mask(params) if callable(mask) else mask)
+            if mdef != treedef:
+                raise ValueError(f"adamw: the mask's structure differs from the parameters'\n  {treedef}\n  {mdef}")
+        if (state["mu"].dtype == torch.uint8) != (state_bits == 8):
+            raise ValueError(f"adamw: state_bits={state_bits}, but the state was made for another width")
+        out, state = _aw.adamw_step(leaves, g, state, learning_rate=learning_rate, b1=b1, b2=b2, eps=eps,
+                                    weight_decay=weight_decay, decay=decay, updates=updates)
+        return _tree.tree_unflatten(treedef, out), state
+
+    def update(grads, state, params=None):
+        return run(grads, state, params, True)
+
+    def step(grads, state, params):
+        return run(grads, state, params, False)
+
+    def moments(state, params=None):
+        flat = _aw.adamw_moments(state)
+        if params is None:
+            return flat
+        leaves, treedef = _tree.tree_flatten(params)
+        if sum(_aw.padded(p.numel()) for p in leaves) != flat[0].numel():
+            raise ValueError("adamw: the state does not belong to these parameters")
+        trees = []
+        for x in flat:
+            parts, at = [], 0
+            for p in leaves:
+                parts.append(x[at:at + p.numel()].view(p.shape))
+                at += _aw.padded(p.numel())
+            trees.append(_tree.tree_unflatten(treedef, parts))
+        return tuple(trees)
+
+    opt = AdamW(init, update)
+    opt.step, opt.moments = step, moments
+    return opt
+
+
+_BY_NAME = {"adam": adam, "adamw": adamw, "sgd": sgd, "rmsprop": rmsprop}
 
 
 def by_name(name: str, learning_rate: float) -> GradientTransformation:

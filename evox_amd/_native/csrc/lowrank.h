@@ -1,0 +1,135 @@
+// Low-rank population layer: what its kernels share.
+//
+//   y[t] = act(x[t] W + bias + s (x[t] A_p^T) B_p + s c_p),  p the individual of row t        (linear)
+//   G = s sum_p w_p A_p^T B_p,  g = s sum_p w_p c_p                                           (weighted sum)
+//
+// W (K x N) row-major; A_p (R x K), B_p (R x N, followed by c_p where the layer has own biases), all individuals at one stride.
+#pragma once
+#include "hip_common.h"
+
+namespace evox {
+namespace lr {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ float bf2f(uint32_t b) { return __uint_as_float(b << 16); }
+__device__ __forceinline__ uint32_t f2bf(float v) {
+  const uint32_t u = __float_as_uint(v);
+  if ((u & 0x7fffffffu) > 0x7f800000u) return (u >> 16) | 0x40u;
+  return (u + 0x7fffu + ((u >> 16) & 1u)) >> 16;
+}
+__device__ __forceinline__ float ld(const float* p) { return *p; }
+__device__ __forceinline__ float ld(const uint16_t* p) { return bf2f(*p); }
+__device__ __forceinline__ void st(float* p, float v) { *p = v; }
+__device__ __forceinline__ void st(uint16_t* p, float v) { *p = (uint16_t)f2bf(v); }
+
+// four consecutive elements; `vec`: the address is a multiple of four elements
+__device__ __forceinline__ f32x4 ld4(const float* p) { return *reinterpret_cast<const f32x4*>(p); }
+__device__ __forceinline__ f32x4 ld4(const uint16_t* p) {
+  const uint2 w = *reinterpret_cast<const uint2*>(p);
+  return f32x4{bf2f(w.x & 0xffffu), __uint_as_float(w.x & 0xffff0000u), bf2f(w.y & 0xffffu), __uint_as_float(w.y & 0xffff0000u)};
+}
+__device__ __forceinline__ void st4(float* p, f32x4 v) { *reinterpret_cast<f32x4*>(p) = v; }
+__device__ __forceinline__ void st4(uint16_t* p, f32x4 v) {
+  *reinterpret_cast<uint2*>(p) = make_uint2(f2bf(v[0]) | (f2bf(v[1]) << 16), f2bf(v[2]) | (f2bf(v[3]) << 16));
+}
+
+__device__ __forceinline__ float activate(float v, int act) {
+  switch (act) {
+    case 1: return tanhf(v);
+    case 2: return v > 0.f ? v : (v != v ? v : 0.f);
+    case 3: return 1.f / (1.f + expf(-v));
+    default: return v;
+  }
+}
+
+// One call of the layer.  Row t is x0 = t / per, x1 = t % per of the input; without an index its individual is x0.
+struct Linear {
+  const void* x;
+  const void* w;
+  const void* a;
+  const void* b;
+  const float* bias;        // N, or null
+  const void* index;        // rows individuals (int32 or int64), or null
+  float* t;                 // rows x R: s (x A^T)
+  void* y;                  // rows x N
+  float* slab;              // splits x rows x N partial products, where K is split over workgroups
+  int64_t sx0, sx1;         // strides of x in elements (the last one is 1)
+  int64_t sa, sb;           // stride from one individual's A (B) to the next
+  int64_t rows, pop, per;
+  int K, N, R;
+  int own_bias, act, index64;
+  int vec;                  // bit 0: x and A, bit 1: B, bias and y, bit 2: W may be read four elements at a time
+  float scale;
+  int splits, k_per_split;
+
+  // the individual of a row; -1: the shared part alone
+  __device__ __forceinline__ int64_t individual(int64_t row) const {
+    if (index == nullptr) return row / per;
+    const int64_t p = index64 ? reinterpret_cast<const int64_t*>(index)[row] : (int64_t) reinterpret_cast<const int32_t*>(index)[row];
+    return p >= 0 && p < pop ? p : -1;
+  }
+  template <typename T>
+  __device__ __forceinline__ const T* row_of(int64_t row) const {
+    const int64_t q = row / per;
+    return reinterpret_cast<const T*>(x) + q * sx0 + (row - q * per) * sx1;
+  }
+  // own part, bias and activation of four columns n .. n + 3 of one row, and the store
+  template <typename T>
+  __device__ __forceinline__ void finish(int64_t row, int n, f32x4 v) const {
+    const int64_t p = individual(row);
+    const bool whole = (vec & 2) && n + 4 <= N;
+    if (bias != nullptr) {
+      if (whole) v += *reinterpret_cast<const f32x4*>(bias + n);
+      else
+        for (int l = 0; l < 4; ++l) if (n + l < N) v[l] += bias[n + l];
+    }
+    if (p >= 0) {
+      const T* bp = reinterpret_cast<const T*>(b) + p * sb + n;
+      const float* tr = t + row * R;
+      f32x4 d = {0.f, 0.f, 0.f, 0.f};
+      if (whole) {
+        for (int j = 0; j < R; ++j, bp += N) {
+          const f32x4 q = ld4(bp);
+          const float tj = tr[j];
+          for (int l = 0; l < 4; ++l) d[l] = fmaf(tj, q[l], d[l]);
+        }
+        if (own_bias) {
+          const f32x4 q = ld4(bp);
+          for (int l = 0; l < 4; ++l) d[l] = fmaf(scale, q[l], d[l]);
+        }
+      } else {
+        for (int j = 0; j < R + own_bias; ++j, bp += N) {
+          const float tj = j < R ? tr[j] : scale;
+          for (int l = 0; l < 4; ++l) if (n + l < N) d[l] = fmaf(tj, ld(bp + l), d[l]);
+        }
+      }
+      v += d;
+    }
+    for (int l = 0; l < 4; ++l) v[l] = activate(v[l], act);
+    T* o = reinterpret_cast<T*>(y) + row * N + n;
+    if (whole) st4(o, v);
+    else
+      for (int l = 0; l < 4; ++l) if (n + l < N) st(o + l, v[l]);
+  }
+};
+
+// One weighted sum.  K = pop * R products; k stands for individual k / R and row k % R of its factors.
+struct Sum {
+  const float* w;
+  const void* a;
+  const void* b;
+  float* g;                 // M x N
+  float* gb;                // N, or null
+  float* slab;              // splits x (M + 1) x N partial sums (row M: own biases), where K is split over workgroups
+  int64_t sa, sb;
+  int64_t pop, K;
+  int M, N, R;
+  int vec;                  // bit 0: A, bit 1: B, bit 2: g may be accessed four elements at a time
+  float scale;
+  int splits;
+  int64_t k_per_split;
+};
+
+}  // namespace lr
+}  // namespace evox

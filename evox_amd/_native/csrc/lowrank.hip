@@ -1,0 +1,352 @@
+// Low-rank population layer: the kernels that take every size, type, stride and alignment.
+//
+// Products run on v_mfma_f32_16x16x4_f32 with operands in fp32 (bf16 ones are widened while they are staged), so nothing
+// is rounded before the end; a workgroup of four wavefronts owns 64 x 64 outputs and walks K in steps of 16 through LDS.
+#include "lowrank.h"
+
+using namespace evox;
+using namespace evox::lr;
+
+namespace {
+
+constexpr int BM = 64, BN = 64, BK = 16, NT = 256;
+constexpr int PM = BM + 4;                         // LDS pitch: the four rows of a fragment read start 4 banks apart
+
+// t[row, j] = s * <x[row], A_p[j]>: one wavefront per row, its lanes along K, four factors at a time.
+template <typename T>
+__global__ __launch_bounds__(NT) void shrink_kernel(Linear q) {
+  const int lane = threadIdx.x & 63;
+  for (int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); row < q.rows; row += (int64_t)gridDim.x * 4) {
+    const int64_t p = q.individual(row);
+    float* tr = q.t + row * q.R;
+    if (p < 0) {
+      for (int j = lane; j < q.R; j += 64) tr[j] = 0.f;
+      continue;
+    }
+    const T* x = q.row_of<T>(row);
+    const T* a = reinterpret_cast<const T*>(q.a) + p * q.sa;
+    for (int j0 = 0; j0 < q.R; j0 += 4) {
+      const int nj = min(4, q.R - j0);
+      float acc[4] = {0.f, 0.f, 0.f, 0.f};
+      const T* aj = a + (int64_t)j0 * q.K;
+      if (q.vec & 1) {
+        for (int k = lane * 4; k < q.K; k += 256) {
+          const f32x4 xv = ld4(x + k);
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (j < nj) {
+              const f32x4 av = ld4(aj + (int64_t)j * q.K + k);
+              for (int l = 0; l < 4; ++l) acc[j] = fmaf(xv[l], av[l], acc[j]);
+            }
+        }
+      } else {
+        for (int k = lane; k < q.K; k += 64) {
+          const float xv = ld(x + k);
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (j < nj) acc[j] = fmaf(xv, ld(aj + (int64_t)j * q.K + k), acc[j]);
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[j] = wave_sum(acc[j]);
+      if (lane == 0)
+        for (int j = 0; j < nj; ++j) tr[j0 + j] = q.scale * acc[j];
+    }
+  }
+}
+
+// acc[a][b][i] = C[wm0 + 16 a + (lane & 15)][wn0 + 16 b + 4 (lane >> 4) + i] of the tile, given its operands' stagers:
+// stage_a(k, m), stage_b(k, n) return element (m0 + m, k) and (k, n0 + n) as floats, zero outside.
+template <class SA, class SB>
+__device__ __forceinline__ void tile_product(int64_t k_begin, int64_t k_end, SA stage_a, SB stage_b, f32x4 (&acc)[2][2]) {
+  __shared__ float sa[BK][PM], sb[BK][PM];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int wm0 = (wave >> 1) * 32, wn0 = (wave & 1) * 32;
+  for (int a = 0; a < 2; ++a)
+    for (int b = 0; b < 2; ++b) acc[a][b] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int64_t k0 = k_begin; k0 < k_end; k0 += BK) {
+    stage_a(sa, k0, k_end);
+    stage_b(sb, k0, k_end);
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < BK; k += 4) {
+      float fa[2], fb[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        fa[i] = sa[k + (lane >> 4)][wm0 + 16 * i + (lane & 15)];
+        fb[i] = sb[k + (lane >> 4)][wn0 + 16 * i + (lane & 15)];
+      }
+#pragma unroll
+      for (int a = 0; a < 2; ++a)
+#pragma unroll
+        for (int b = 0; b < 2; ++b) acc[a][b] = __builtin_amdgcn_mfma_f32_16x16x4f32(fb[b], fa[a], acc[a][b], 0, 0, 0);
+    }
+    __syncthreads();
+  }
+}
+
+template <typename T>
+__global__ __launch_bounds__(NT) void linear_kernel(Linear q, int tiles_n) {
+  const int nwg = (int)gridDim.x;
+  const int u = xcd_remap((int)blockIdx.x, nwg);
+  const int tile = u / q.splits, split = u % q.splits;
+  const int64_t m0 = (int64_t)(tile / tiles_n) * BM;
+  const int n0 = (tile % tiles_n) * BN;
+  const T* w = reinterpret_cast<const T*>(q.w);
+  const int tid = threadIdx.x;
+  // x: thread (m = tid / 4, k = 4 (tid % 4)); W: thread (k = tid / 16, n = 4 (tid % 16))
+  const int64_t xrow = m0 + (tid >> 2);
+  const T* xr = q.row_of<T>(xrow < q.rows ? xrow : q.rows - 1);
+  auto stage_x = [&](float (&s)[BK][PM], int64_t k0, int64_t k_end) {
+    const int64_t k = k0 + (tid & 3) * 4;
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    if (xrow < q.rows) {
+      if ((q.vec & 1) && k + 4 <= k_end) v = ld4(xr + k);
+      else
+        for (int l = 0; l < 4; ++l) if (k + l < k_end) v[l] = ld(xr + k + l);
+    }
+    for (int l = 0; l < 4; ++l) s[(tid & 3) * 4 + l][tid >> 2] = v[l];
+  };
+  auto stage_w = [&](float (&s)[BK][PM], int64_t k0, int64_t k_end) {
+    const int64_t k = k0 + (tid >> 4);
+    const int n = n0 + (tid & 15) * 4;
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    if (k < k_end) {
+      const T* wr = w + k * q.N + n;
+      if ((q.vec & 4) && n + 4 <= q.N) v = ld4(wr);
+      else
+        for (int l = 0; l < 4; ++l) if (n + l < q.N) v[l] = ld(wr + l);
+    }
+    *reinterpret_cast<f32x4*>(&s[tid >> 4][(tid & 15) * 4]) = v;
+  };
+  f32x4 acc[2][2];
+  const int64_t kb = (int64_t)split * q.k_per_split;
+  tile_product(kb, min((int64_t)q.K, kb + q.k_per_split), stage_x, stage_w, acc);
+  const int lane = tid & 63, wave = tid >> 6;
+#pragma unroll
+  for (int a = 0; a < 2; ++a)
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      const int64_t row = m0 + (wave >> 1) * 32 + 16 * a + (lane & 15);
+      const int n = n0 + (wave & 1) * 32 + 16 * b + (lane >> 4) * 4;
+      if (row >= q.rows || n >= q.N) continue;
+      if (q.splits == 1) {
+        q.finish<T>(row, n, acc[a][b]);
+      } else {
+        float* o = q.slab + ((int64_t)split * q.rows + row) * q.N + n;
+        for (int l = 0; l < 4; ++l) if (n + l < q.N) o[l] = acc[a][b][l];
+      }
+    }
+}
+
+// y from the partial products of all splits, added in a fixed order
+template <typename T>
+__global__ __launch_bounds__(NT) void linear_join_kernel(Linear q) {
+  const int quads = (q.N + 3) / 4;
+  const int64_t total = q.rows * quads;
+  for (int64_t i = (int64_t)blockIdx.x * NT + threadIdx.x; i < total; i += (int64_t)gridDim.x * NT) {
+    const int64_t row = i / quads;
+    const int n = (int)(i - row * quads) * 4;
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < q.splits; ++s) {
+      const float* p = q.slab + ((int64_t)s * q.rows + row) * q.N + n;
+      for (int l = 0; l < 4; ++l) if (n + l < q.N) v[l] += p[l];
+    }
+    q.finish<T>(row, n, v);
+  }
+}
+
+template <typename T>
+__global__ __launch_bounds__(NT) void sum_kernel(Sum q, int tiles_n, int tiles) {
+  const int tid = threadIdx.x;
+  const int products = tiles * q.splits;
+  if ((int)blockIdx.x >= products) {
+    // own biases: 64 columns of one split of the individuals; four wavefronts take every fourth individual
+    __shared__ float part[4][64];
+    const int u = (int)blockIdx.x - products;
+    const int split = u % q.splits, n = (u / q.splits) * 64 + (tid & 63);
+    const int64_t per = (q.pop + q.splits - 1) / q.splits;
+    const int64_t end = min(q.pop, (split + 1) * per);
+    float s = 0.f;
+    if (n < q.N)
+      for (int64_t p = split * per + (tid >> 6); p < end; p += 4)
+        s = fmaf(q.w[p], ld(reinterpret_cast<const T*>(q.b) + p * q.sb + (int64_t)q.R * q.N + n), s);
+    part[tid >> 6][tid & 63] = s;
+    __syncthreads();
+    if (tid < 64 && n < q.N) {
+      s = part[0][tid] + part[1][tid] + part[2][tid] + part[3][tid];
+      if (q.splits == 1) q.gb[n] = q.scale * s;
+      else q.slab[((int64_t)split * (q.M + 1) + q.M) * q.N + n] = s;
+    }
+    return;
+  }
+  const int u = xcd_remap((int)blockIdx.x, products);
+  const int tile = u / q.splits, split = u % q.splits;
+  const int m0 = (tile / tiles_n) * BM, n0 = (tile % tiles_n) * BN;
+  const int kk = tid >> 4, c = (tid & 15) * 4;
+  auto stage_a = [&](float (&s)[BK][PM], int64_t k0, int64_t k_end) {
+    const int64_t k = k0 + kk;
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    if (k < k_end) {
+      const int64_t p = k / q.R;
+      const T* r = reinterpret_cast<const T*>(q.a) + p * q.sa + (k - p * q.R) * q.M + m0 + c;
+      if ((q.vec & 1) && m0 + c + 4 <= q.M) v = ld4(r);
+      else
+        for (int l = 0; l < 4; ++l) if (m0 + c + l < q.M) v[l] = ld(r + l);
+      v *= q.w[p];
+    }
+    *reinterpret_cast<f32x4*>(&s[kk][c]) = v;
+  };
+  auto stage_b = [&](float (&s)[BK][PM], int64_t k0, int64_t k_end) {
+    const int64_t k = k0 + kk;
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    if (k < k_end) {
+      const int64_t p = k / q.R;
+      const T* r = reinterpret_cast<const T*>(q.b) + p * q.sb + (k - p * q.R) * q.N + n0 + c;
+      if ((q.vec & 2) && n0 + c + 4 <= q.N) v = ld4(r);
+      else
+        for (int l = 0; l < 4; ++l) if (n0 + c + l < q.N) v[l] = ld(r + l);
+    }
+    *reinterpret_cast<f32x4*>(&s[kk][c]) = v;
+  };
+  f32x4 acc[2][2];
+  const int64_t kb = split * q.k_per_split;
+  tile_product(kb, min(q.K, kb + q.k_per_split), stage_a, stage_b, acc);
+  const int lane = tid & 63, wave = tid >> 6;
+#pragma unroll
+  for (int a = 0; a < 2; ++a)
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      const int m = m0 + (wave >> 1) * 32 + 16 * a + (lane & 15);
+      const int n = n0 + (wave & 1) * 32 + 16 * b + (lane >> 4) * 4;
+      if (m >= q.M || n >= q.N) continue;
+      const float f = q.splits == 1 ? q.scale : 1.f;
+      float* o = q.splits == 1 ? q.g + (int64_t)m * q.N + n : q.slab + ((int64_t)split * (q.M + 1) + m) * q.N + n;
+      for (int l = 0; l < 4; ++l) if (n + l < q.N) o[l] = f * acc[a][b][l];
+    }
+}
+
+__global__ __launch_bounds__(NT) void sum_join_kernel(Sum q) {
+  const int64_t mn = (int64_t)q.M * q.N, total = mn + (q.gb != nullptr ? q.N : 0), pitch = mn + q.N;
+  for (int64_t i = (int64_t)blockIdx.x * NT + threadIdx.x; i < total; i += (int64_t)gridDim.x * NT) {
+    float s = 0.f;
+    for (int k = 0; k < q.splits; ++k) s += q.slab[k * pitch + i];
+    s *= q.scale;
+    if (i < mn) q.g[i] = s;
+    else q.gb[i - mn] = s;
+  }
+}
+
+template <typename T>
+int launch_linear(const Linear& q, hipStream_t s) {
+  const int64_t tiles_m = (q.rows + BM - 1) / BM;
+  const int tiles_n = (q.N + BN - 1) / BN;
+  const int64_t wgs = tiles_m * tiles_n * q.splits;
+  if (wgs > 0x7fffffff) return (int)hipErrorInvalidValue;
+  const int64_t sg = (q.rows + 3) / 4;
+  shrink_kernel<T><<<(unsigned)(sg < 65536 ? sg : 65536), NT, 0, s>>>(q);
+  linear_kernel<T><<<(unsigned)wgs, NT, 0, s>>>(q, tiles_n);
+  if (q.splits > 1) linear_join_kernel<T><<<stream_grid(q.rows * ((q.N + 3) / 4), NT), NT, 0, s>>>(q);
+  return last_launch_status();
+}
+
+template <typename T>
+int launch_sum(const Sum& q, hipStream_t s) {
+  const int tiles_n = (q.N + BN - 1) / BN;
+  const int64_t tiles = (int64_t)((q.M + BM - 1) / BM) * tiles_n;
+  const int64_t wgs = (tiles + (q.gb != nullptr ? (q.N + 63) / 64 : 0)) * q.splits;
+  if (wgs > 0x7fffffff) return (int)hipErrorInvalidValue;
+  sum_kernel<T><<<(unsigned)wgs, NT, 0, s>>>(q, tiles_n, (int)tiles);
+  if (q.splits > 1) sum_join_kernel<<<stream_grid((int64_t)(q.M + 1) * q.N, NT), NT, 0, s>>>(q);
+  return last_launch_status();
+}
+
+bool aligned4(const void* p, int elem) { return (reinterpret_cast<uintptr_t>(p) & (uintptr_t)(4 * elem - 1)) == 0; }
+
+// How many workgroups share one tile's K: enough that about two workgroups per compute unit run, but at least 128 products each.
+int64_t splits_for(int64_t tiles, int64_t K) {
+  int64_t s = (2 * kNumCU) / (tiles < 1 ? 1 : tiles);
+  if (s > (K + 127) / 128) s = (K + 127) / 128;
+  return s < 1 ? 1 : s;
+}
+
+void plan_linear(Linear& q) {
+  const int64_t tiles = ((q.rows + BM - 1) / BM) * ((q.N + BN - 1) / BN);
+  q.splits = (int)splits_for(tiles, q.K);
+  const int64_t per = (q.K + q.splits - 1) / q.splits;
+  q.k_per_split = per > 0 ? (int)((per + BK - 1) / BK * BK) : BK;
+  q.splits = (q.K + q.k_per_split - 1) / q.k_per_split;
+  if (q.splits < 1) q.splits = 1;
+}
+
+void plan_sum(Sum& q) {
+  const int64_t tiles = (int64_t)((q.M + BM - 1) / BM) * ((q.N + BN - 1) / BN);
+  int64_t s = splits_for(tiles, q.K);
+  const int64_t per = (q.K + s - 1) / s;
+  q.k_per_split = per > 0 ? (per + BK - 1) / BK * BK : BK;
+  q.splits = (int)((q.K + q.k_per_split - 1) / q.k_per_split);
+  if (q.splits < 1) q.splits = 1;
+}
+
+}  // namespace
+
+// Floats of workspace that a call of evox_hip_lowrank_linear takes: t and the partial products.
+EVOX_API int64_t evox_hip_lowrank_linear_ws(int64_t rows, int K, int N, int R) {
+  Linear q{};
+  q.rows = rows; q.K = K; q.N = N; q.R = R;
+  plan_linear(q);
+  return (rows * R + 3) / 4 * 4 + (q.splits > 1 ? (int64_t)q.splits * rows * N : 0);
+}
+
+// dims: rows, pop, per, sx0, sx1, sa, sb.  ints: K, N, R, own_bias, act, dtype (0 fp32, 1 bf16), index type (0 none, 1 int32, 2 int64)
+EVOX_API int evox_hip_lowrank_linear(const void* x, const void* w, const void* a, const void* b, const float* bias,
+                                     const void* index, void* y, float* ws, int64_t ws_floats, const int64_t* dims,
+                                     const int* ints, float scale, void* stream) {
+  Linear q{};
+  q.x = x; q.w = w; q.a = a; q.b = b; q.bias = bias; q.y = y;
+  q.rows = dims[0]; q.pop = dims[1]; q.per = dims[2];
+  q.sx0 = dims[3]; q.sx1 = dims[4]; q.sa = dims[5]; q.sb = dims[6];
+  q.K = ints[0]; q.N = ints[1]; q.R = ints[2]; q.own_bias = ints[3]; q.act = ints[4];
+  const int dtype = ints[5];
+  q.index = ints[6] ? index : nullptr;
+  q.index64 = ints[6] == 2;
+  q.scale = scale;
+  if (q.rows <= 0 || q.N <= 0) return 0;
+  if (q.K <= 0 || q.R <= 0 || q.per <= 0 || dtype < 0 || dtype > 1) return (int)hipErrorInvalidValue;
+  if (ws_floats < evox_hip_lowrank_linear_ws(q.rows, q.K, q.N, q.R)) return (int)hipErrorInvalidValue;
+  plan_linear(q);
+  q.t = ws;
+  q.slab = ws + (q.rows * q.R + 3) / 4 * 4;
+  const int el = dtype ? 2 : 4;
+  if (q.K % 4 == 0 && q.sx0 % 4 == 0 && q.sx1 % 4 == 0 && q.sa % 4 == 0 && aligned4(x, el) && aligned4(a, el)) q.vec |= 1;
+  if (q.N % 4 == 0 && q.sb % 4 == 0 && aligned4(b, el) && aligned4(y, el) && (!bias || aligned4(bias, 4))) q.vec |= 2;
+  if (q.N % 4 == 0 && aligned4(w, el)) q.vec |= 4;
+  return dtype ? launch_linear<uint16_t>(q, (hipStream_t)stream) : launch_linear<float>(q, (hipStream_t)stream);
+}
+
+EVOX_API int64_t evox_hip_lowrank_sum_ws(int64_t pop, int M, int N, int R) {
+  Sum q{};
+  q.pop = pop; q.K = pop * R; q.M = M; q.N = N; q.R = R;
+  plan_sum(q);
+  return q.splits > 1 ? (int64_t)q.splits * (M + 1) * N : 0;
+}
+
+// dims: pop, sa, sb.  ints: M, N, R, dtype
+EVOX_API int evox_hip_lowrank_sum(const float* w, const void* a, const void* b, float* g, float* gb, float* ws, int64_t ws_floats,
+                                  const int64_t* dims, const int* ints, float scale, void* stream) {
+  Sum q{};
+  q.w = w; q.a = a; q.b = b; q.g = g; q.gb = gb; q.slab = ws;
+  q.pop = dims[0]; q.sa = dims[1]; q.sb = dims[2];
+  q.M = ints[0]; q.N = ints[1]; q.R = ints[2];
+  const int dtype = ints[3];
+  q.K = q.pop * q.R;
+  q.scale = scale;
+  if (q.M <= 0 || q.N <= 0) return 0;
+  if (q.R <= 0 || q.pop < 0 || dtype < 0 || dtype > 1) return (int)hipErrorInvalidValue;
+  if (ws_floats < evox_hip_lowrank_sum_ws(q.pop, q.M, q.N, q.R)) return (int)hipErrorInvalidValue;
+  plan_sum(q);
+  const int el = dtype ? 2 : 4;
+  if (q.M % 4 == 0 && q.sa % 4 == 0 && aligned4(a, el)) q.vec |= 1;
+  if (q.N % 4 == 0 && q.sb % 4 == 0 && aligned4(b, el)) q.vec |= 2;
+  return dtype ? launch_sum<uint16_t>(q, (hipStream_t)stream) : launch_sum<float>(q, (hipStream_t)stream);
+}

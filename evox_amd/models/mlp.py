@@ -221,6 +221,60 @@ class MLP:
 
     __call__ = batched_apply
 
+    # Low-rank populations: an individual is the shared centre plus, per layer, scale (B_p^T A_p)^T on the weights and scale c_p on
+    # the bias.  Its factors are one row: layer after layer A (rank x in), B (rank x out) and, with biases, c (out); every layer
+    # starts at a multiple of eight elements, so that rows of a population can be read sixteen bytes at a time.
+    def lowrank_size(self, rank: int) -> int:
+        """Elements of one individual's factors."""
+        return sum(-(-(rank * i + (rank + bool(self.bias)) * o) // 8) * 8 for i, o in zip(self.sizes[:-1], self.sizes[1:]))
+
+    def lowrank_factors(self, factors: torch.Tensor, rank: int):
+        """``[(a, b), …]`` per layer, views of a ``(P, lowrank_size(rank))`` population: a (P, rank, in), b (P, rank [+ 1], out)."""
+        if rank < 1 or factors.dim() != 2 or factors.shape[1] != self.lowrank_size(rank):
+            raise ValueError(f"factors of rank {rank} for {self.sizes} have shape (P, {self.lowrank_size(rank) if rank > 0 else '?'}), "
+                             f"got {tuple(factors.shape)}")
+        out, off = [], 0
+        rows = rank + bool(self.bias)
+        for i, o in zip(self.sizes[:-1], self.sizes[1:]):
+            a, b = factors[:, off:off + rank * i], factors[:, off + rank * i:off + rank * i + rows * o]
+            out.append((a.unflatten(1, (rank, i)), b.unflatten(1, (rows, o))))
+            off += -(-(rank * i + rows * o) // 8) * 8
+        return out
+
+    def lowrank_apply(self, center: torch.Tensor, factors: torch.Tensor, obs: torch.Tensor, rank: int, scale: float = 1.0,
+                      index=None) -> torch.Tensor:
+        """The networks of a low-rank population on ``obs`` (P, E, in) or (P, in); with ``index`` (T,) on ``obs`` (T, in), row t
+        by individual ``index[t]`` (by the centre itself where that is negative).  Computes in the factors' type."""
+        from ..ops.lowrank import lowrank_linear
+
+        if center.dim() != 1 or center.shape[0] != self.n_params:
+            raise ValueError(f"the centre of {self.sizes} has shape ({self.n_params},), got {tuple(center.shape)}")
+        h, off, last = obs.to(factors.dtype), 0, len(self.sizes) - 2
+        for li, (a, b) in enumerate(self.lowrank_factors(factors, rank)):
+            i, o = self.sizes[li], self.sizes[li + 1]
+            weight = center[off:off + i * o].view(i, o).to(factors.dtype)
+            off += i * o
+            bias = None
+            if self.bias:
+                bias = center[off:off + o]
+                off += o
+            h = lowrank_linear(h, weight, a, b, index=index, bias=bias, scale=scale,
+                               activation=self.final_activation if li == last else self.activation)
+        return h
+
+    def lowrank_gradient(self, w: torch.Tensor, factors: torch.Tensor, rank: int, scale: float = 1.0) -> torch.Tensor:
+        """``scale · Σ_p w_p (individual p − centre)`` as a flat float32 vector like the centre: the evolution-strategy gradient of
+        the fitness weights ``w`` (P,), without any individual's matrix being formed."""
+        from ..ops.lowrank import lowrank_weighted_sum
+
+        parts = []
+        for a, b in self.lowrank_factors(factors, rank):
+            g, gb = lowrank_weighted_sum(w, a, b, scale=scale)
+            parts.append(g.reshape(-1))
+            if gb is not None:
+                parts.append(gb)
+        return torch.cat(parts)
+
     def to_tree(self, params: torch.Tensor):
         """Split a flat vector (or a (P, n) population) into ``[{"w", "b"}, …]`` views."""
         out, off = [], 0

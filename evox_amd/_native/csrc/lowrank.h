@@ -63,15 +63,21 @@ struct Linear {
   float scale;
   int splits, k_per_split;
 
+  // row / per; a division of 64 bits takes a hundred instructions, so rows that fit are divided in 32
+  __device__ __forceinline__ int64_t group(int64_t row) const {
+    if (per == 1) return row;
+    if (rows <= 0xffffffffll) return (uint32_t)row / (uint32_t)per;
+    return row / per;
+  }
   // the individual of a row; -1: the shared part alone
   __device__ __forceinline__ int64_t individual(int64_t row) const {
-    if (index == nullptr) return row / per;
+    if (index == nullptr) return group(row);
     const int64_t p = index64 ? reinterpret_cast<const int64_t*>(index)[row] : (int64_t) reinterpret_cast<const int32_t*>(index)[row];
     return p >= 0 && p < pop ? p : -1;
   }
   template <typename T>
   __device__ __forceinline__ const T* row_of(int64_t row) const {
-    const int64_t q = row / per;
+    const int64_t q = group(row);
     return reinterpret_cast<const T*>(x) + q * sx0 + (row - q * per) * sx1;
   }
   // own part, bias and activation of four columns n .. n + 3 of one row, and the store

@@ -7,6 +7,13 @@
 using namespace evox;
 using namespace evox::lr;
 
+namespace evox {
+namespace lr {
+bool linear_mfma_grouped(const Linear& q);                       // lowrank_mfma.hip
+int linear_mfma(const Linear& q, bool grouped, hipStream_t s);
+}  // namespace lr
+}  // namespace evox
+
 namespace {
 
 constexpr int BM = 64, BN = 64, BK = 16, NT = 256;
@@ -237,8 +244,25 @@ __global__ __launch_bounds__(NT) void sum_join_kernel(Sum q) {
   }
 }
 
+// bf16 on the matrix cores at full rate: sixteen-byte pieces everywhere, and enough rows to fill its tiles
+bool mfma_fits(const Linear& q) {
+  auto al = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; };
+  return q.rows >= 128 && q.K >= 64 && q.K % 8 == 0 && q.N % 8 == 0 && q.sx0 % 8 == 0 && q.sx1 % 8 == 0 && al(q.x) && al(q.w) &&
+         al(q.y) && (q.vec & 2);
+}
+
 template <typename T>
 int launch_linear(const Linear& q, hipStream_t s) {
+  if constexpr (sizeof(T) == 2) {
+    if (mfma_fits(q)) {
+      const bool grouped = linear_mfma_grouped(q);
+      if (!grouped) {
+        const int64_t sg = (q.rows + 3) / 4;
+        shrink_kernel<T><<<(unsigned)(sg < 65536 ? sg : 65536), NT, 0, s>>>(q);
+      }
+      return linear_mfma(q, grouped, s);
+    }
+  }
   const int64_t tiles_m = (q.rows + BM - 1) / BM;
   const int tiles_n = (q.N + BN - 1) / BN;
   const int64_t wgs = tiles_m * tiles_n * q.splits;

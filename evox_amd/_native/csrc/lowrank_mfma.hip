@@ -1,0 +1,480 @@
+// Low-rank population layer in bf16 on v_mfma_f32_16x16x32_bf16: y = act(x W + bias + s (x A_p^T) B_p + s c_p).
+//
+// A workgroup of WM x WN wavefronts owns BM x BN outputs and walks K in steps of 64.  Both operands go from memory to LDS
+// without passing registers (16 bytes a lane, two stages: the next step's loads are in flight while a step is multiplied).
+//   x  (K contiguous): rows of 128 bytes, 16-byte pieces permuted by the row (XOR), read as they are (ds_read_b128);
+//   W  (N contiguous): rows of 2 BN bytes, 32-byte pieces permuted by the row, read transposed (ds_read_b64_tr_b16: 16 lanes
+//      exchange a 4 x 16 block so that a lane holds four consecutive k of its column).  No transposed copy of W is made, which
+//      a step of evolution that changes W every generation would pay for every time.
+// The permutations are applied to the source addresses (the LDS image of a load is linear); they spread the rows that one read
+// touches over all banks.  Pieces behind K come from a zero in memory, so any K that is a multiple of 8 works.
+// The matrix instruction takes W's fragment as its first operand: a lane then holds four consecutive columns of one row.
+//
+// The individuals' part:
+//   GROUPED (an individual has at least 16 rows): the 16-row fragments of a tile each belong to one individual (its last one may
+//     be partly empty).  t = x A_p^T is one more matrix product of the x fragment that is in registers anyway, against A_p read
+//     straight from memory (K contiguous) — 1/16 more instructions per wavefront, no second pass over x and no launch of
+//     its own.  At the end s t is split into two bf16 halves (together 16 bits), [t_hi | t_lo] times [B_p; B_p] is one
+//     instruction per fragment of outputs.  Rank at most 16.
+//   otherwise (single rows, requests): t comes from shrink_kernel, every lane adds its row's R products to its columns.
+#include "lowrank.h"
+
+using namespace evox;
+using namespace evox::lr;
+
+namespace {
+
+using bf16x8 = __attribute__((ext_vector_type(8))) __bf16;
+using s16x8 = __attribute__((ext_vector_type(8))) short;
+typedef __attribute__((address_space(3))) void* lds_vp;
+typedef const __attribute__((address_space(1))) void* glb_vp;
+
+constexpr int BK = 32;
+constexpr int SLOT = 1024;   // bytes of one individual's A_p in a stage: 16 rows of 32 elements
+
+__device__ const uint4 kZero = {0, 0, 0, 0};
+
+struct Tiles {
+  uint32_t frags;      // GROUPED: 16-row fragments of all individuals
+  uint32_t frags_each; // GROUPED: fragments of one individual
+  int tiles_n;
+};
+
+template <int N>
+__device__ __forceinline__ void wait_vmcnt() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+
+// Transposed reads of two adjacent 4-row blocks each for four columns blocks, waited for in place: the compiler would let no
+// such read (through its builtin) pass a load to LDS that is in flight, which is what the stages are for.
+template <int STEP>
+__device__ __forceinline__ void read_tr4(const uint32_t (&at)[4], bf16x8 (&out)[4]) {
+  uint2 r0, r1, r2, r3, r4, r5, r6, r7;
+  asm volatile(
+      "ds_read_b64_tr_b16 %0, %8\n\tds_read_b64_tr_b16 %1, %8 offset:%12\n\t"
+      "ds_read_b64_tr_b16 %2, %9\n\tds_read_b64_tr_b16 %3, %9 offset:%12\n\t"
+      "ds_read_b64_tr_b16 %4, %10\n\tds_read_b64_tr_b16 %5, %10 offset:%12\n\t"
+      "ds_read_b64_tr_b16 %6, %11\n\tds_read_b64_tr_b16 %7, %11 offset:%12\n\t"
+      "s_waitcnt lgkmcnt(0)"
+      : "=&v"(r0), "=&v"(r1), "=&v"(r2), "=&v"(r3), "=&v"(r4), "=&v"(r5), "=&v"(r6), "=&v"(r7)
+      : "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[3]), "n"(STEP)
+      : "memory");
+  out[0] = __builtin_bit_cast(bf16x8, make_uint4(r0.x, r0.y, r1.x, r1.y));
+  out[1] = __builtin_bit_cast(bf16x8, make_uint4(r2.x, r2.y, r3.x, r3.y));
+  out[2] = __builtin_bit_cast(bf16x8, make_uint4(r4.x, r4.y, r5.x, r5.y));
+  out[3] = __builtin_bit_cast(bf16x8, make_uint4(r6.x, r6.y, r7.x, r7.y));
+}
+template <int STEP>
+__device__ __forceinline__ void read_tr2(const uint32_t (&at)[2], bf16x8 (&out)[2]) {
+  uint2 r0, r1, r2, r3;
+  asm volatile(
+      "ds_read_b64_tr_b16 %0, %4\n\tds_read_b64_tr_b16 %1, %4 offset:%6\n\t"
+      "ds_read_b64_tr_b16 %2, %5\n\tds_read_b64_tr_b16 %3, %5 offset:%6\n\t"
+      "s_waitcnt lgkmcnt(0)"
+      : "=&v"(r0), "=&v"(r1), "=&v"(r2), "=&v"(r3)
+      : "v"(at[0]), "v"(at[1]), "n"(STEP)
+      : "memory");
+  out[0] = __builtin_bit_cast(bf16x8, make_uint4(r0.x, r0.y, r1.x, r1.y));
+  out[1] = __builtin_bit_cast(bf16x8, make_uint4(r2.x, r2.y, r3.x, r3.y));
+}
+
+// permutation of the 32-byte pieces of a W row: the 16 rows {r, r + 8, r + 16, r + 24} + 0..3 of one transposed read differ
+template <int BN>
+__device__ __forceinline__ int w_swizzle(int row) {
+  return ((row & 3) | (((row >> 3) & 3) << 2)) & (BN / 16 - 1);
+}
+// permutation of the 16-byte pieces of a 64-byte row (x, A_p): eight neighbouring rows of one read fall on eight bank groups
+__device__ __forceinline__ int x_swizzle(int row) { return (row >> 1) & 3; }
+
+// Activations whose result is rounded to bf16: the exponential of the hardware (2^x) is good to 2^-22, and tanh, which would lose
+// its small values in 1 - 2 / (e^2v + 1), is its series below 1/8 (next term 17/315 v^7: 2^-26 of v).
+__device__ __forceinline__ float tanh_bf16(float v) {
+  const float s = v * v, small = v * fmaf(s, fmaf(s, 2.f / 15.f, -1.f / 3.f), 1.f);
+  const float big = 1.f - 2.f * __builtin_amdgcn_rcpf(__expf(2.f * v) + 1.f);
+  return fabsf(v) < 0.125f ? small : big;
+}
+template <int TN>
+__device__ __forceinline__ void activate_all(f32x4 (&v)[TN], int act) {
+  if (act == 1) {
+#pragma unroll
+    for (int b = 0; b < TN; ++b)
+#pragma unroll
+      for (int l = 0; l < 4; ++l) v[b][l] = tanh_bf16(v[b][l]);
+  } else if (act == 2) {
+#pragma unroll
+    for (int b = 0; b < TN; ++b)
+#pragma unroll
+      for (int l = 0; l < 4; ++l) v[b][l] = v[b][l] > 0.f ? v[b][l] : (v[b][l] != v[b][l] ? v[b][l] : 0.f);
+  } else if (act == 3) {
+#pragma unroll
+    for (int b = 0; b < TN; ++b)
+#pragma unroll
+      for (int l = 0; l < 4; ++l) v[b][l] = __builtin_amdgcn_rcpf(1.f + __expf(-v[b][l]));
+  }
+}
+
+template <int BM, int BN, int WM, int WN, int STAGES, int SLOTS>
+__global__ __launch_bounds__(WM* WN * 64) void linear_mfma_kernel(Linear q, Tiles g) {
+  constexpr bool GROUPED = SLOTS > 0;
+  constexpr int NW = WM * WN;
+  constexpr int TM = BM / WM / 16, TN = BN / WN / 16;
+  constexpr int X_BYTES = BM * BK * 2, W_BYTES = BK * BN * 2, STAGE = X_BYTES + W_BYTES + SLOTS * SLOT;
+  constexpr int XI = X_BYTES / 1024 / NW, WI = W_BYTES / 1024 / NW, AI = SLOTS / NW;   // wave-instructions per stage
+  constexpr int LOADS = XI + WI + AI;
+  constexpr int TT = (TM + WN - 1) / WN;                              // t fragments of a wavefront
+  static_assert(X_BYTES % (1024 * NW) == 0 && W_BYTES % (1024 * NW) == 0 && SLOTS % NW == 0, "whole wave-instructions");
+  static_assert(TN == 4 || TN == 2, "column blocks of a wavefront");
+  static_assert(STAGES >= 3 && LOADS * (STAGES - 2) <= 63 && STAGES * STAGE <= 160 * 1024, "counted waits and LDS");
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const int wm = wave / WN, wn = wave % WN;
+  const int u = xcd_remap((int)blockIdx.x, (int)gridDim.x);
+  const int tm = u / g.tiles_n;
+  const int n0 = (u % g.tiles_n) * BN;
+  const uint16_t* W = reinterpret_cast<const uint16_t*>(q.w);
+  const uint32_t frag0 = (uint32_t)tm * (BM / 16);                    // GROUPED: this tile's first fragment and individual
+  const uint32_t first = GROUPED ? frag0 / g.frags_each : 0;
+
+  // place i of this tile -> individual and row of it (GROUPED), or row of all; false where the place holds none
+  auto place = [&](int i, int64_t& p, int64_t& r) -> bool {
+    if constexpr (GROUPED) {
+      const uint32_t f = frag0 + (i >> 4);
+      const uint32_t pp = f / g.frags_each;
+      p = pp;
+      r = (int64_t)(f - pp * g.frags_each) * 16 + (i & 15);
+      return f < g.frags && r < q.per;
+    } else {
+      p = 0;
+      r = (int64_t)tm * BM + i;
+      return r < q.rows;
+    }
+  };
+  const char* xs[XI];
+  const char* ws[WI];
+  const char* as[AI > 0 ? AI : 1];
+  int xk, wk[WI];
+  // a wave-instruction brings 16 rows of 64 bytes (x, A_p) or 1024 / (2 BN) rows of W
+  xk = ((lane & 3) ^ x_swizzle(lane >> 2)) * 8;                       // first k of this lane's piece (rows repeat mod 16)
+#pragma unroll
+  for (int j = 0; j < XI; ++j) {
+    int64_t p, r;
+    if (!place((j * NW + wave) * 16 + (lane >> 2), p, r)) place(0, p, r);   // (results of such places are not stored)
+    const uint16_t* x = reinterpret_cast<const uint16_t*>(q.x);
+    if constexpr (GROUPED) x += p * q.sx0 + r * q.sx1;
+    else x = q.row_of<uint16_t>(r);
+    xs[j] = reinterpret_cast<const char*>(x + xk);
+  }
+#pragma unroll
+  for (int j = 0; j < WI; ++j) {
+    const int byte = (j * NW + wave) * 1024 + lane * 16;
+    const int row = byte / (BN * 2), c16 = byte % (BN * 2) / 16;
+    int n = n0 + (((c16 >> 1) ^ w_swizzle<BN>(row)) * 16 + (c16 & 1) * 8);
+    if (n >= q.N) n = 0;                                              // columns that are not stored
+    wk[j] = row;
+    ws[j] = reinterpret_cast<const char*>(W + (int64_t)row * q.N + n);
+  }
+#pragma unroll
+  for (int j = 0; j < AI; ++j) {
+    // (a slot behind the individuals of this tile's last fragment holds zeros)
+    const uint32_t p = first + j * NW + wave, end = (min(frag0 + BM / 16, g.frags) - 1) / g.frags_each;
+    const int row = lane >> 2;
+    as[j] = row < q.R && p <= end ? reinterpret_cast<const char*>(reinterpret_cast<const uint16_t*>(q.a) + (int64_t)p * q.sa + (int64_t)row * q.K + xk) : nullptr;
+  }
+  const int64_t wstep = (int64_t)BK * q.N * 2;
+  const char* const zero = reinterpret_cast<const char*>(&kZero);
+  auto stage_x = [&](int buf, int kt) {
+    char* s = smem + buf * STAGE;
+    const int k0 = kt * BK;
+    const bool tail = k0 + BK > q.K;
+#pragma unroll
+    for (int j = 0; j < XI; ++j) {
+      const char* p = xs[j] + (int64_t)kt * (BK * 2);
+      if (tail && k0 + xk >= q.K) p = zero;
+      __builtin_amdgcn_global_load_lds((glb_vp)p, (lds_vp)(s + (j * NW + wave) * 1024), 16, 0, 0);
+    }
+  };
+  auto stage_w = [&](int buf, int kt) {
+    char* s = smem + buf * STAGE;
+    const int k0 = kt * BK;
+    const bool tail = k0 + BK > q.K;
+#pragma unroll
+    for (int j = 0; j < WI; ++j) {
+      const char* p = ws[j] + kt * wstep;
+      if (tail && k0 + wk[j] >= q.K) p = zero;
+      __builtin_amdgcn_global_load_lds((glb_vp)p, (lds_vp)(s + X_BYTES + (j * NW + wave) * 1024), 16, 0, 0);
+    }
+#pragma unroll
+    for (int j = 0; j < AI; ++j) {
+      const char* p = as[j] + (int64_t)kt * (BK * 2);
+      if (as[j] == nullptr || (tail && k0 + xk >= q.K)) p = zero;
+      __builtin_amdgcn_global_load_lds((glb_vp)p, (lds_vp)(s + X_BYTES + W_BYTES + (j * NW + wave) * SLOT), 16, 0, 0);
+    }
+  };
+
+  f32x4 acc[TM][TN], tacc[TT];
+#pragma unroll
+  for (int a = 0; a < TM; ++a)
+#pragma unroll
+    for (int b = 0; b < TN; ++b) acc[a][b] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < TT; ++i) tacc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const int wm0 = wm * TM * 16, wn0 = wn * TN * 16;
+
+  // this lane's offsets in a stage: fragments of x (and A_p) — row lane & 15, eight k from 8 (lane >> 4) — and transposed
+  // reads of W — row 8 (lane >> 4) + (lane & 15) / 4, four columns at 4 (lane & 3) of a 16-column piece
+  const int xo = (lane & 15) * 64 + (((lane >> 4) ^ x_swizzle(lane & 15)) << 4);
+  uint32_t wo[TN];
+  {
+    const int row = (lane >> 4) * 8 + ((lane & 15) >> 2);
+    const uint32_t base = (uint32_t)(uintptr_t)(lds_vp)smem + X_BYTES + row * (BN * 2) + (lane & 3) * 8;
+#pragma unroll
+    for (int b = 0; b < TN; ++b) wo[b] = base + (((wn * TN + b) ^ w_swizzle<BN>(row)) << 5);
+  }
+  int ao[TT];                                                         // offsets of A_p's fragments for this wavefront's t
+  int to[TT];                                                         // and of x's
+  if constexpr (GROUPED) {
+#pragma unroll
+    for (int i = 0; i < TT; ++i) {
+      const int a = min(wn * TT + i, TM - 1);
+      const uint32_t f = min(frag0 + wm * TM + a, g.frags - 1);
+      ao[i] = X_BYTES + W_BYTES + (int)(f / g.frags_each - first) * SLOT + xo;
+      to[i] = (wm0 + a * 16) * 64 + xo;
+    }
+  }
+  bf16x8 fx[TM], fw[TN], fa[TT], ft[TT];
+  auto read = [&](int buf) {
+    const char* s = smem + buf * STAGE;
+#pragma unroll
+    for (int a = 0; a < TM; ++a) fx[a] = *reinterpret_cast<const bf16x8*>(s + (wm0 + a * 16) * 64 + xo);
+    if constexpr (GROUPED) {
+      // (which x fragments t needs depends on the wavefront: they are read again rather than chosen among registers; a branch
+      // around the two instructions for each choice cost more, 408 against 377 us for the multiplying alone)
+#pragma unroll
+      for (int i = 0; i < TT; ++i) {
+        fa[i] = *reinterpret_cast<const bf16x8*>(s + ao[i]);
+        ft[i] = *reinterpret_cast<const bf16x8*>(s + to[i]);
+      }
+    }
+    uint32_t at[TN];
+#pragma unroll
+    for (int b = 0; b < TN; ++b) at[b] = wo[b] + buf * STAGE;
+    if constexpr (TN == 4) read_tr4<4 * BN * 2>(at, fw);
+    else read_tr2<4 * BN * 2>(at, fw);
+  };
+  auto multiply = [&]() {
+#pragma unroll
+    for (int a = 0; a < TM; ++a)
+#pragma unroll
+      for (int b = 0; b < TN; ++b) acc[a][b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fw[b], fx[a], acc[a][b], 0, 0, 0);
+    if constexpr (GROUPED) {
+#pragma unroll
+      for (int i = 0; i < TT; ++i) tacc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fa[i], ft[i], tacc[i], 0, 0, 0);
+    }
+  };
+  auto barrier = [&]() {
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");                                    // (no read of LDS moves up across the barrier)
+  };
+
+  const int nk = (q.K + BK - 1) / BK;
+  int buf = 0;
+  if constexpr (NW == 8) {
+    // Two wavefronts share a SIMD (wave and wave + 4).  They run half a step apart: while one multiplies, the other reads its
+    // fragments from LDS and sends the loads of a step to come, so the matrix pipe does not wait for LDS.  A step's loads have
+    // landed for everybody when each wavefront has waited for its own before the barrier in front of the first half that reads
+    // them: the late group at the end of its reading half, the early one at the end of its multiplying half, which is the same
+    // moment.  The buffer of step kt - 1 is refilled from the early group's reading half of step kt on; the late group has read
+    // it in the half before.
+    auto wait_behind = [&](int later) {                               // at most the loads of the `later` youngest steps outstanding
+      static_assert(STAGES == 4, "the waits of the last steps");
+      if (later >= 2) wait_vmcnt<2 * LOADS>();
+      else if (later == 1) wait_vmcnt<LOADS>();
+      else wait_vmcnt<0>();
+    };
+    const bool late = wave >= 4;
+#pragma unroll
+    for (int i = 0; i < STAGES - 1; ++i)
+      if (i < nk) { stage_x(i, i); stage_w(i, i); }
+    wait_behind(nk - 1);
+    barrier();
+    if (late) barrier();
+    for (int kt = 0; kt < nk; ++kt) {
+      read(buf);
+      if (kt + 3 < nk) {
+        stage_x((buf + 3) & 3, kt + 3);
+        stage_w((buf + 3) & 3, kt + 3);
+      }
+      const int later = min(nk - 1, kt + 3) - (kt + 1);
+      if (late) wait_behind(later);
+      barrier();
+      __builtin_amdgcn_s_setprio(1);
+      multiply();
+      __builtin_amdgcn_s_setprio(0);
+      if (!late) wait_behind(later);
+      barrier();
+      buf = (buf + 1) & 3;
+    }
+    if (!late) barrier();
+  } else {
+    // Per step: wait until this wavefront's loads of the step have landed (those of the following steps stay outstanding), one
+    // barrier (all its loads are in LDS, and every wavefront has read the step before), refill the buffer of the step before,
+    // multiply.
+#pragma unroll
+    for (int i = 0; i < STAGES - 1; ++i)
+      if (i < nk) { stage_x(i, i); stage_w(i, i); }
+    for (int kt = 0; kt < nk; ++kt) {
+      static_assert(STAGES <= 4, "the waits of the last steps");
+      const int later = nk - 1 - kt;
+      if (later >= STAGES - 2) wait_vmcnt<LOADS * (STAGES - 2)>();
+      else if (later == 1) wait_vmcnt<LOADS>();
+      else wait_vmcnt<0>();
+      barrier();
+      if (kt + STAGES - 1 < nk) {
+        const int b = buf == 0 ? STAGES - 1 : buf - 1;
+        stage_x(b, kt + STAGES - 1);
+        stage_w(b, kt + STAGES - 1);
+      }
+      read(buf);
+      multiply();
+      buf = buf == STAGES - 1 ? 0 : buf + 1;
+    }
+  }
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+  __syncthreads();
+
+  if constexpr (GROUPED) {
+    // t in LDS: rows of 32 bf16, s t rounded to bf16, then what that leaves
+    uint16_t* ts = reinterpret_cast<uint16_t*>(smem);
+    constexpr int T_BYTES = BM * 64, W16 = TN * 16, PITCH = W16 + 8;
+    static_assert(T_BYTES + NW * 16 * PITCH * 2 <= STAGES * STAGE, "t and the patches fit the stages");
+    uint16_t* patch = reinterpret_cast<uint16_t*>(smem + T_BYTES) + wave * 16 * PITCH;
+    const int k8 = (lane >> 4) * 8, j16 = lane & 15;
+#pragma unroll
+    for (int i = 0; i < TT; ++i) {
+      const int a = wn * TT + i;
+      if (a < TM) {
+        uint16_t hi[4], lo[4];
+#pragma unroll
+        for (int l = 0; l < 4; ++l) {
+          // (places behind the rank: zero even where the row of x is not finite)
+          const float v = (lane >> 4) * 4 + l < q.R ? q.scale * tacc[i][l] : 0.f;
+          hi[l] = (uint16_t)f2bf(v);
+          const float rest = v - bf2f(hi[l]);
+          lo[l] = rest == rest ? (uint16_t)f2bf(rest) : 0;            // (an infinite v leaves no rest)
+        }
+        uint16_t* o = ts + (wm0 + a * 16 + j16) * 32 + (lane >> 4) * 4;
+        *reinterpret_cast<uint2*>(o) = make_uint2(hi[0] | (uint32_t)hi[1] << 16, hi[2] | (uint32_t)hi[3] << 16);
+        *reinterpret_cast<uint2*>(o + 16) = make_uint2(lo[0] | (uint32_t)lo[1] << 16, lo[2] | (uint32_t)lo[3] << 16);
+      }
+    }
+    __syncthreads();
+    uint32_t last = 0xffffffffu;
+    bf16x8 fb[TN];
+    f32x4 own[TN];                                                    // s c_p + bias of this lane's columns
+#pragma unroll
+    for (int a = 0; a < TM; ++a) {
+      const uint32_t f = frag0 + wm * TM + a;
+      if (f >= g.frags) continue;
+      const uint32_t p = f / g.frags_each;
+      const int64_t r0 = (int64_t)(f - p * g.frags_each) * 16;
+      if (p != last) {
+        last = p;
+        const uint16_t* bp = reinterpret_cast<const uint16_t*>(q.b) + (int64_t)p * q.sb;
+#pragma unroll
+        for (int b = 0; b < TN; ++b) {
+          const int n = n0 + wn0 + b * 16;
+          s16x8 v;
+#pragma unroll
+          for (int l = 0; l < 8; ++l) {
+            const int j = (k8 & 15) + l;
+            v[l] = j < q.R && n + j16 < q.N ? (short)bp[(int64_t)j * q.N + n + j16] : (short)0;
+          }
+          fb[b] = __builtin_bit_cast(bf16x8, v);
+          const int nc = n + (lane >> 4) * 4;
+          own[b] = f32x4{0.f, 0.f, 0.f, 0.f};
+          if (nc < q.N) {
+            if (q.bias != nullptr) own[b] = *reinterpret_cast<const f32x4*>(q.bias + nc);
+            if (q.own_bias) own[b] += q.scale * ld4(bp + (int64_t)q.R * q.N + nc);
+          }
+        }
+      }
+      const bf16x8 ft = *reinterpret_cast<const bf16x8*>(ts + (wm0 + a * 16 + j16) * 32 + k8);
+#pragma unroll
+      for (int b = 0; b < TN; ++b) acc[a][b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb[b], ft, acc[a][b], 0, 0, 0) + own[b];
+      activate_all(acc[a], q.act);
+#pragma unroll
+      for (int b = 0; b < TN; ++b) st4(patch + j16 * PITCH + b * 16 + (lane >> 4) * 4, acc[a][b]);
+      // whole rows of the wavefront's columns: 16 bytes a lane
+      constexpr int LPR = W16 / 8, RPS = 64 / LPR;
+#pragma unroll
+      for (int i = 0; i < 16 / RPS; ++i) {
+        const int r = i * RPS + lane / LPR, n = n0 + wn0 + (lane % LPR) * 8;
+        const uint4 v = *reinterpret_cast<const uint4*>(patch + r * PITCH + (lane % LPR) * 8);
+        if (r0 + r < q.per && n < q.N)
+          *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(q.y) + ((int64_t)p * q.per + r0 + r) * q.N + n) = v;
+      }
+    }
+  } else {
+    // sixteen rows at a time through a patch of LDS of the wavefront's own, so that a row's columns lie in neighbouring lanes
+    // (whole lines of B and y) and the long code of a row's end is there once
+    constexpr int W16 = TN * 16, PITCH = W16 + 4, LPR = W16 / 4, RPS = 64 / LPR;      // lanes per row, rows per step
+    static_assert(NW * 16 * PITCH * 4 <= STAGES * STAGE, "the patches fit the stages");
+    float* patch = reinterpret_cast<float*>(smem) + wave * 16 * PITCH;
+#pragma unroll
+    for (int a = 0; a < TM; ++a) {
+#pragma unroll
+      for (int b = 0; b < TN; ++b)
+        *reinterpret_cast<f32x4*>(patch + (lane & 15) * PITCH + b * 16 + (lane >> 4) * 4) = acc[a][b];
+#pragma unroll 1
+      for (int r = lane / LPR; r < 16; r += RPS) {
+        const int n = n0 + wn0 + (lane % LPR) * 4;
+        const int64_t row = (int64_t)tm * BM + wm0 + a * 16 + r;
+        const f32x4 v = *reinterpret_cast<const f32x4*>(patch + r * PITCH + (lane % LPR) * 4);
+        if (row < q.rows && n < q.N) q.finish<uint16_t>(row, n, v);
+      }
+    }
+  }
+}
+
+template <int BM, int BN, int WM, int WN, int STAGES, int SLOTS>
+int launch(const Linear& q, hipStream_t s) {
+  constexpr int LDS = STAGES * (BM * BK * 2 + BK * BN * 2 + SLOTS * SLOT);
+  Tiles g{};
+  g.tiles_n = (q.N + BN - 1) / BN;
+  g.frags_each = (uint32_t)((q.per + 15) / 16);
+  g.frags = SLOTS ? (uint32_t)(q.pop * g.frags_each) : 0;
+  const int64_t tiles_m = SLOTS ? ((int64_t)g.frags * 16 + BM - 1) / BM : (q.rows + BM - 1) / BM;
+  if (tiles_m * g.tiles_n > 0x7fffffff) return (int)hipErrorInvalidValue;
+  auto* k = &linear_mfma_kernel<BM, BN, WM, WN, STAGES, SLOTS>;
+  static const hipError_t attr =
+      hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
+  if (attr != hipSuccess) return (int)attr;
+  k<<<(unsigned)(tiles_m * g.tiles_n), WM * WN * 64, LDS, s>>>(q, g);
+  return last_launch_status();
+}
+
+}  // namespace
+
+namespace evox {
+namespace lr {
+
+bool linear_mfma_grouped(const Linear& q) {
+  // fragments at least 70 % full: the empty rows cost more than the separate pass over x otherwise
+  const int64_t each = (q.per + 15) / 16;
+  return q.index == nullptr && q.R <= 16 && q.per >= 16 && 10 * q.per >= 7 * 16 * each && q.pop * each < 0x7fffffff / 16 &&
+         q.sa % 8 == 0 && (reinterpret_cast<uintptr_t>(q.a) & 15) == 0;
+}
+
+int linear_mfma(const Linear& q, bool grouped, hipStream_t s) {
+  const int64_t big = ((q.rows + 255) / 256) * ((q.N + 255) / 256);
+  if (grouped) {
+    // a tile of 256 rows holds A_p of eight individuals: at most 16 / each + 1 of them meet in it, 16 / each where they start together
+    const int64_t each = (q.per + 15) / 16, meet = 16 % each == 0 ? 16 / each : 16 / each + 2;
+    return big >= kNumCU && meet <= 8 ? launch<256, 256, 2, 4, 4, 8>(q, s) : launch<128, 128, 2, 2, 3, 8>(q, s);
+  }
+  return big >= kNumCU ? launch<256, 256, 2, 4, 4, 0>(q, s) : launch<128, 64, 2, 2, 4, 0>(q, s);
+}
+
+}  // namespace lr
+}  // namespace evox

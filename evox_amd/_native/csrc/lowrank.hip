@@ -11,6 +11,8 @@ namespace evox {
 namespace lr {
 bool linear_mfma_grouped(const Linear& q);                       // lowrank_mfma.hip
 int linear_mfma(const Linear& q, bool grouped, hipStream_t s);
+void sum_mfma_plan(Sum& q);                                      // lowrank_sum_mfma.hip
+int sum_mfma(const Sum& q, hipStream_t s);
 }  // namespace lr
 }  // namespace evox
 
@@ -348,29 +350,60 @@ EVOX_API int evox_hip_lowrank_linear(const void* x, const void* w, const void* a
   return dtype ? launch_linear<uint16_t>(q, (hipStream_t)stream) : launch_linear<float>(q, (hipStream_t)stream);
 }
 
-EVOX_API int64_t evox_hip_lowrank_sum_ws(int64_t pop, int M, int N, int R) {
-  Sum q{};
-  q.pop = pop; q.K = pop * R; q.M = M; q.N = N; q.R = R;
-  plan_sum(q);
-  return q.splits > 1 ? (int64_t)q.splits * (M + 1) * N : 0;
+// Whether a sum takes the bf16 matrix instructions: pieces of sixteen bytes, sizes that fill a good part of a tile, and
+// enough terms that a step of 32 is not mostly empty.
+static bool sum_takes_mfma(int64_t pop, int M, int N, int R, int dtype, int64_t sa, int64_t sb, const void* a, const void* b,
+                           const void* g) {
+  auto al = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; };
+  return dtype == 1 && M % 8 == 0 && N % 8 == 0 && M >= 64 && N >= 64 && pop * R >= 64 && sa % 8 == 0 && sb % 8 == 0 && al(a) &&
+         al(b) && al(g);
+}
+
+static int64_t sum_workspace(Sum& q, bool mfma) {
+  if (mfma) sum_mfma_plan(q);
+  else plan_sum(q);
+  return q.splits > 1 ? (int64_t)q.splits * (q.M + 1) * q.N : 0;
 }
 
 // dims: pop, sa, sb.  ints: M, N, R, dtype
-EVOX_API int evox_hip_lowrank_sum(const float* w, const void* a, const void* b, float* g, float* gb, float* ws, int64_t ws_floats,
-                                  const int64_t* dims, const int* ints, float scale, void* stream) {
-  Sum q{};
-  q.w = w; q.a = a; q.b = b; q.g = g; q.gb = gb; q.slab = ws;
+static int sum_call(const float* w, const void* a, const void* b, float* g, float* gb, const int64_t* dims, const int* ints, float scale,
+                    Sum& q, bool& mfma) {
+  q = Sum{};
+  q.w = w; q.a = a; q.b = b; q.g = g; q.gb = gb;
   q.pop = dims[0]; q.sa = dims[1]; q.sb = dims[2];
   q.M = ints[0]; q.N = ints[1]; q.R = ints[2];
   const int dtype = ints[3];
+  if (q.M <= 0 || q.N <= 0 || q.R <= 0 || q.pop <= 0 || dtype < 0 || dtype > 1) return (int)hipErrorInvalidValue;
   q.K = q.pop * q.R;
   q.scale = scale;
-  if (q.M <= 0 || q.N <= 0) return 0;
-  if (q.R <= 0 || q.pop < 0 || dtype < 0 || dtype > 1) return (int)hipErrorInvalidValue;
-  if (ws_floats < evox_hip_lowrank_sum_ws(q.pop, q.M, q.N, q.R)) return (int)hipErrorInvalidValue;
-  plan_sum(q);
   const int el = dtype ? 2 : 4;
   if (q.M % 4 == 0 && q.sa % 4 == 0 && aligned4(a, el)) q.vec |= 1;
   if (q.N % 4 == 0 && q.sb % 4 == 0 && aligned4(b, el)) q.vec |= 2;
-  return dtype ? launch_sum<uint16_t>(q, (hipStream_t)stream) : launch_sum<float>(q, (hipStream_t)stream);
+  mfma = sum_takes_mfma(q.pop, q.M, q.N, q.R, dtype, q.sa, q.sb, a, b, g);
+  return 0;
+}
+
+// Floats of workspace that the same call of evox_hip_lowrank_sum takes (negative: the call is refused).
+EVOX_API int64_t evox_hip_lowrank_sum_ws(const float* w, const void* a, const void* b, float* g, float* gb, const int64_t* dims,
+                                         const int* ints) {
+  Sum q;
+  bool mfma;
+  if (sum_call(w, a, b, g, gb, dims, ints, 1.f, q, mfma)) return -1;
+  return sum_workspace(q, mfma);
+}
+
+EVOX_API int evox_hip_lowrank_sum(const float* w, const void* a, const void* b, float* g, float* gb, const int64_t* dims,
+                                  const int* ints, float* ws, int64_t ws_floats, float scale, void* stream) {
+  Sum q;
+  bool mfma;
+  if (const int st = sum_call(w, a, b, g, gb, dims, ints, scale, q, mfma)) return st;
+  if (ws_floats < sum_workspace(q, mfma)) return (int)hipErrorInvalidValue;
+  q.slab = ws;
+  hipStream_t s = (hipStream_t)stream;
+  if (mfma) {
+    if (const int st = sum_mfma(q, s)) return st;
+    if (q.splits > 1) sum_join_kernel<<<stream_grid((int64_t)(q.M + 1) * q.N, NT), NT, 0, s>>>(q);
+    return last_launch_status();
+  }
+  return ints[3] ? launch_sum<uint16_t>(q, s) : launch_sum<float>(q, s);
 }

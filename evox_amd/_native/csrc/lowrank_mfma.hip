@@ -18,16 +18,12 @@
 //     instruction per fragment of outputs.  Rank at most 16.
 //   otherwise (single rows, requests): t comes from shrink_kernel, every lane adds its row's R products to its columns.
 #include "lowrank.h"
+#include "lowrank_tile.h"
 
 using namespace evox;
 using namespace evox::lr;
 
 namespace {
-
-using bf16x8 = __attribute__((ext_vector_type(8))) __bf16;
-using s16x8 = __attribute__((ext_vector_type(8))) short;
-typedef __attribute__((address_space(3))) void* lds_vp;
-typedef const __attribute__((address_space(1))) void* glb_vp;
 
 constexpr int BK = 32;
 constexpr int SLOT = 1024;   // bytes of one individual's A_p in a stage: 16 rows of 32 elements
@@ -40,49 +36,6 @@ struct Tiles {
   int tiles_n;
 };
 
-template <int N>
-__device__ __forceinline__ void wait_vmcnt() {
-  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
-}
-
-// Transposed reads of two adjacent 4-row blocks each for four columns blocks, waited for in place: the compiler would let no
-// such read (through its builtin) pass a load to LDS that is in flight, which is what the stages are for.
-template <int STEP>
-__device__ __forceinline__ void read_tr4(const uint32_t (&at)[4], bf16x8 (&out)[4]) {
-  uint2 r0, r1, r2, r3, r4, r5, r6, r7;
-  asm volatile(
-      "ds_read_b64_tr_b16 %0, %8\n\tds_read_b64_tr_b16 %1, %8 offset:%12\n\t"
-      "ds_read_b64_tr_b16 %2, %9\n\tds_read_b64_tr_b16 %3, %9 offset:%12\n\t"
-      "ds_read_b64_tr_b16 %4, %10\n\tds_read_b64_tr_b16 %5, %10 offset:%12\n\t"
-      "ds_read_b64_tr_b16 %6, %11\n\tds_read_b64_tr_b16 %7, %11 offset:%12\n\t"
-      "s_waitcnt lgkmcnt(0)"
-      : "=&v"(r0), "=&v"(r1), "=&v"(r2), "=&v"(r3), "=&v"(r4), "=&v"(r5), "=&v"(r6), "=&v"(r7)
-      : "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[3]), "n"(STEP)
-      : "memory");
-  out[0] = __builtin_bit_cast(bf16x8, make_uint4(r0.x, r0.y, r1.x, r1.y));
-  out[1] = __builtin_bit_cast(bf16x8, make_uint4(r2.x, r2.y, r3.x, r3.y));
-  out[2] = __builtin_bit_cast(bf16x8, make_uint4(r4.x, r4.y, r5.x, r5.y));
-  out[3] = __builtin_bit_cast(bf16x8, make_uint4(r6.x, r6.y, r7.x, r7.y));
-}
-template <int STEP>
-__device__ __forceinline__ void read_tr2(const uint32_t (&at)[2], bf16x8 (&out)[2]) {
-  uint2 r0, r1, r2, r3;
-  asm volatile(
-      "ds_read_b64_tr_b16 %0, %4\n\tds_read_b64_tr_b16 %1, %4 offset:%6\n\t"
-      "ds_read_b64_tr_b16 %2, %5\n\tds_read_b64_tr_b16 %3, %5 offset:%6\n\t"
-      "s_waitcnt lgkmcnt(0)"
-      : "=&v"(r0), "=&v"(r1), "=&v"(r2), "=&v"(r3)
-      : "v"(at[0]), "v"(at[1]), "n"(STEP)
-      : "memory");
-  out[0] = __builtin_bit_cast(bf16x8, make_uint4(r0.x, r0.y, r1.x, r1.y));
-  out[1] = __builtin_bit_cast(bf16x8, make_uint4(r2.x, r2.y, r3.x, r3.y));
-}
-
-// permutation of the 32-byte pieces of a W row: the 16 rows {r, r + 8, r + 16, r + 24} + 0..3 of one transposed read differ
-template <int BN>
-__device__ __forceinline__ int w_swizzle(int row) {
-  return ((row & 3) | (((row >> 3) & 3) << 2)) & (BN / 16 - 1);
-}
 // permutation of the 16-byte pieces of a 64-byte row (x, A_p): eight neighbouring rows of one read fall on eight bank groups
 __device__ __forceinline__ int x_swizzle(int row) { return (row >> 1) & 3; }
 
@@ -169,7 +122,7 @@ __global__ __launch_bounds__(WM* WN * 64) void linear_mfma_kernel(Linear q, Tile
   for (int j = 0; j < WI; ++j) {
     const int byte = (j * NW + wave) * 1024 + lane * 16;
     const int row = byte / (BN * 2), c16 = byte % (BN * 2) / 16;
-    int n = n0 + (((c16 >> 1) ^ w_swizzle<BN>(row)) * 16 + (c16 & 1) * 8);
+    int n = n0 + (((c16 >> 1) ^ tr_swizzle<BN>(row)) * 16 + (c16 & 1) * 8);
     if (n >= q.N) n = 0;                                              // columns that are not stored
     wk[j] = row;
     ws[j] = reinterpret_cast<const char*>(W + (int64_t)row * q.N + n);
@@ -229,7 +182,7 @@ __global__ __launch_bounds__(WM* WN * 64) void linear_mfma_kernel(Linear q, Tile
     const int row = (lane >> 4) * 8 + ((lane & 15) >> 2);
     const uint32_t base = (uint32_t)(uintptr_t)(lds_vp)smem + X_BYTES + row * (BN * 2) + (lane & 3) * 8;
 #pragma unroll
-    for (int b = 0; b < TN; ++b) wo[b] = base + (((wn * TN + b) ^ w_swizzle<BN>(row)) << 5);
+    for (int b = 0; b < TN; ++b) wo[b] = base + (((wn * TN + b) ^ tr_swizzle<BN>(row)) << 5);
   }
   int ao[TT];                                                         // offsets of A_p's fragments for this wavefront's t
   int to[TT];                                                         // and of x's
@@ -272,10 +225,6 @@ __global__ __launch_bounds__(WM* WN * 64) void linear_mfma_kernel(Linear q, Tile
       for (int i = 0; i < TT; ++i) tacc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fa[i], ft[i], tacc[i], 0, 0, 0);
     }
   };
-  auto barrier = [&]() {
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");                                    // (no read of LDS moves up across the barrier)
-  };
 
   const int nk = (q.K + BK - 1) / BK;
   int buf = 0;
@@ -297,8 +246,8 @@ __global__ __launch_bounds__(WM* WN * 64) void linear_mfma_kernel(Linear q, Tile
     for (int i = 0; i < STAGES - 1; ++i)
       if (i < nk) { stage_x(i, i); stage_w(i, i); }
     wait_behind(nk - 1);
-    barrier();
-    if (late) barrier();
+    barrier_no_fence();
+    if (late) barrier_no_fence();
     for (int kt = 0; kt < nk; ++kt) {
       read(buf);
       if (kt + 3 < nk) {
@@ -307,15 +256,15 @@ __global__ __launch_bounds__(WM* WN * 64) void linear_mfma_kernel(Linear q, Tile
       }
       const int later = min(nk - 1, kt + 3) - (kt + 1);
       if (late) wait_behind(later);
-      barrier();
+      barrier_no_fence();
       __builtin_amdgcn_s_setprio(1);
       multiply();
       __builtin_amdgcn_s_setprio(0);
       if (!late) wait_behind(later);
-      barrier();
+      barrier_no_fence();
       buf = (buf + 1) & 3;
     }
-    if (!late) barrier();
+    if (!late) barrier_no_fence();
   } else {
     // Per step: wait until this wavefront's loads of the step have landed (those of the following steps stay outstanding), one
     // barrier (all its loads are in LDS, and every wavefront has read the step before), refill the buffer of the step before,
@@ -329,7 +278,7 @@ __global__ __launch_bounds__(WM* WN * 64) void linear_mfma_kernel(Linear q, Tile
       if (later >= STAGES - 2) wait_vmcnt<LOADS * (STAGES - 2)>();
       else if (later == 1) wait_vmcnt<LOADS>();
       else wait_vmcnt<0>();
-      barrier();
+      barrier_no_fence();
       if (kt + STAGES - 1 < nk) {
         const int b = buf == 0 ? STAGES - 1 : buf - 1;
         stage_x(b, kt + STAGES - 1);

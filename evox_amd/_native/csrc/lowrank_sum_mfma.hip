@@ -1,0 +1,317 @@
+// Weighted sum of low-rank products in bf16 on v_mfma_f32_16x16x32_bf16: G = s sum_k (w_k a_k)^T b_k over k = (individual, rank row).
+//
+// Both operands have k as their slow axis: tiles of 32 k go from memory to LDS as they lie (16 bytes a lane, 32-byte pieces
+// permuted by the row) and are read transposed (ds_read_b64_tr_b16), so no transposed copy of the factors is made.
+// The weights are float32 and so is the result, so w a must not be rounded to the factors' 8 bits: it is formed in float32
+// after the fragment is in registers and split into bf16 planes by rounding, hi + mid (+ lo), each multiplied by b with one
+// matrix instruction.  Two planes hold w a to 2^-18 (deviation 1.5e-6 of it at random mantissas), three to 2^-26.  Sums of
+// 16384 terms or more take two: the float32 accumulation of such sums leaves more than that by itself (1.6e-6 of the result at
+// 16384 random terms, 4.6e-6 at 65536), and a third plane costs half as much time again.
+// The wavefronts of a workgroup are laid out so that each splits few fragments of A and uses each split for many of B.
+// K is divided over as many workgroups as fill the chip; the partial sums are added by sum_join_kernel in a fixed order.
+#include "lowrank.h"
+#include "lowrank_tile.h"
+
+using namespace evox;
+using namespace evox::lr;
+
+namespace {
+
+constexpr int BK = 32;
+
+__device__ const uint4 kZero = {0, 0, 0, 0};
+
+// Sums of the individuals' biases, 64 columns of one split of the individuals: eight lanes of eight columns each, the other
+// threads along the individuals.  These workgroups ride along behind the ones that multiply.
+template <int THREADS>
+__device__ __forceinline__ void sum_biases(const Sum& q, int u, char* smem) {
+  constexpr int ROWS = THREADS / 8;
+  float(*part)[64] = reinterpret_cast<float(*)[64]>(smem);             // ROWS x 64
+  const int tid = threadIdx.x;
+  const int split = u % q.splits, c = (tid & 7) * 8, n = (u / q.splits) * 64 + c;
+  const int64_t per = (q.pop + q.splits - 1) / q.splits, end = min(q.pop, (split + 1) * per);
+  const uint16_t* b = reinterpret_cast<const uint16_t*>(q.b) + (int64_t)q.R * q.N + n;
+  float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  if (n < q.N) {
+#pragma unroll 4
+    for (int64_t p = split * per + tid / 8; p < end; p += ROWS) {
+      const uint4 v = *reinterpret_cast<const uint4*>(b + p * q.sb);
+      const uint32_t x[4] = {v.x, v.y, v.z, v.w};
+      const float w = q.w[p];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        s[2 * i] = fmaf(w, __uint_as_float(x[i] << 16), s[2 * i]);
+        s[2 * i + 1] = fmaf(w, __uint_as_float(x[i] & 0xffff0000u), s[2 * i + 1]);
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) part[tid / 8][c + i] = s[i];
+  __syncthreads();
+  const int col = (u / q.splits) * 64 + tid;
+  if (tid < 64 && col < q.N) {
+    float v = 0.f;
+    for (int r = 0; r < ROWS; ++r) v += part[r][tid];
+    if (q.splits == 1) q.gb[col] = q.scale * v;
+    else q.slab[((int64_t)split * (q.M + 1) + q.M) * q.N + col] = v;
+  }
+}
+
+// two floats rounded to bf16, in one register
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  using f32x2 = __attribute__((ext_vector_type(2))) float;
+  using bf16x2 = __attribute__((ext_vector_type(2))) __bf16;
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a, b}, bf16x2));
+}
+
+// fragment of A times its eight weights, as planes
+template <int PLANES>
+__device__ __forceinline__ void split_planes(const bf16x8 f, const float (&w)[8], bf16x8 (&out)[PLANES]) {
+  const uint4 u = __builtin_bit_cast(uint4, f);
+  const uint32_t in[4] = {u.x, u.y, u.z, u.w};
+  uint32_t o[PLANES][4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float x = __uint_as_float(in[i] << 16) * w[2 * i], y = __uint_as_float(in[i] & 0xffff0000u) * w[2 * i + 1];
+#pragma unroll
+    for (int p = 0; p < PLANES; ++p) {
+      o[p][i] = pack2(x, y);
+      if (p + 1 < PLANES) {
+        x -= __uint_as_float(o[p][i] << 16);
+        y -= __uint_as_float(o[p][i] & 0xffff0000u);
+      }
+    }
+  }
+#pragma unroll
+  for (int p = 0; p < PLANES; ++p) out[p] = __builtin_bit_cast(bf16x8, make_uint4(o[p][0], o[p][1], o[p][2], o[p][3]));
+}
+
+template <int BM, int BN, int WM, int WN, int STAGES, int PLANES>
+__global__ __launch_bounds__(WM* WN * 64) void sum_mfma_kernel(Sum q, int tiles, int tiles_n) {
+  constexpr int NW = WM * WN;
+  constexpr int TM = BM / WM / 16, TN = BN / WN / 16;
+  constexpr int A_BYTES = BK * BM * 2, B_BYTES = BK * BN * 2, STAGE = A_BYTES + B_BYTES + NW * 256;
+  constexpr int AI = A_BYTES / 1024 / NW, BI = B_BYTES / 1024 / NW, LOADS = AI + BI + 1;
+  static_assert(BM == BN, "the rows of a load are those of both operands");
+  static_assert(TM == 4 && TN % 4 == 0, "fragments are read four at a time");
+  static_assert(STAGES >= 3 && STAGES <= 4 && LOADS * (STAGES - 2) <= 63 && STAGES * STAGE <= 160 * 1024, "counted waits and LDS");
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const int wm = wave / WN, wn = wave % WN;
+  // tiles of one split lie together: they read the same factors
+  const int products = tiles * q.splits;
+  if ((int)blockIdx.x >= products) {
+    sum_biases<NW * 64>(q, (int)blockIdx.x - products, smem);
+    return;
+  }
+  const int u = xcd_remap((int)blockIdx.x, products);
+  const int split = u / tiles, tile = u % tiles;
+  const int m0 = (tile / tiles_n) * BM, n0 = (tile % tiles_n) * BN;
+  const int64_t kb = split * q.k_per_split, ke = min(q.K, kb + q.k_per_split);
+  const int nk = (int)((ke - kb + BK - 1) / BK);
+
+  // This lane's rows.  The factors of an individual lie apart from the next one's: a row's address moves on by a fixed amount per
+  // step and by what lies between two individuals whenever its rank row wraps.
+  constexpr int RPI = 1024 / (BM * 2);
+  static_assert(RPI >= 1 && AI == BI, "");
+  const uint16_t* A = reinterpret_cast<const uint16_t*>(q.a);
+  const uint16_t* B = reinterpret_cast<const uint16_t*>(q.b);
+  const int pstep = BK / q.R, jstep = BK % q.R;
+  const int64_t da = (pstep * q.sa + (int64_t)jstep * q.M) * 2, wrap_a = (q.sa - (int64_t)q.R * q.M) * 2;
+  const int64_t db = (pstep * q.sb + (int64_t)jstep * q.N) * 2, wrap_b = (q.sb - (int64_t)q.R * q.N) * 2;
+  const int left = (int)min(ke - kb, (int64_t)0x7fffffff);            // k of this split
+  const char *pa[AI], *pb[AI];
+  int kr[AI], jr[AI];
+#pragma unroll
+  for (int j = 0; j < AI; ++j) {
+    const int byte = (j * NW + wave) * 1024 + lane * 16;
+    const int row = byte / (BM * 2), c16 = byte % (BM * 2) / 16;
+    const int col = ((c16 >> 1) ^ tr_swizzle<BM>(row)) * 16 + (c16 & 1) * 8;
+    const int64_t p = (kb + row) / q.R;
+    kr[j] = row;
+    jr[j] = (int)(kb + row - p * q.R);
+    pa[j] = reinterpret_cast<const char*>(A + p * q.sa + (int64_t)jr[j] * q.M + (m0 + col < q.M ? m0 + col : 0));
+    pb[j] = reinterpret_cast<const char*>(B + p * q.sb + (int64_t)jr[j] * q.N + (n0 + col < q.N ? n0 + col : 0));
+  }
+  // and its weight: k of lane & 31 (both halves of the wavefront bring the same)
+  int kw = lane & 31, jw = (int)((kb + kw) % q.R);
+  const float* pw = q.w + (kb + kw) / q.R;
+  const char* const zero = reinterpret_cast<const char*>(&kZero);
+  // the loads of the next step in order: every call moves the rows on by 32
+  auto stage = [&](int buf) {
+    char* s = smem + buf * STAGE;
+#pragma unroll
+    for (int j = 0; j < AI; ++j) {
+      const bool in = kr[j] < left;
+      __builtin_amdgcn_global_load_lds((glb_vp)(in ? pa[j] : zero), (lds_vp)(s + (j * NW + wave) * 1024), 16, 0, 0);
+      __builtin_amdgcn_global_load_lds((glb_vp)(in ? pb[j] : zero), (lds_vp)(s + A_BYTES + (j * NW + wave) * 1024), 16, 0, 0);
+      kr[j] += BK;
+      pa[j] += da;
+      pb[j] += db;
+    }
+    // in a place of the wavefront's own
+    __builtin_amdgcn_global_load_lds((glb_vp)(kw < left ? reinterpret_cast<const char*>(pw) : zero),
+                                     (lds_vp)(s + A_BYTES + B_BYTES + wave * 256), 4, 0, 0);
+    kw += BK;
+    pw += pstep;
+    if (jstep != 0) {
+#pragma unroll
+      for (int j = 0; j < AI; ++j) {
+        jr[j] += jstep;
+        if (jr[j] >= q.R) {
+          jr[j] -= q.R;
+          pa[j] += wrap_a;
+          pb[j] += wrap_b;
+        }
+      }
+      jw += jstep;
+      if (jw >= q.R) {
+        jw -= q.R;
+        ++pw;
+      }
+    }
+  };
+
+  f32x4 acc[TM][TN];
+#pragma unroll
+  for (int a = 0; a < TM; ++a)
+#pragma unroll
+    for (int b = 0; b < TN; ++b) acc[a][b] = f32x4{0.f, 0.f, 0.f, 0.f};
+  uint32_t ao[TM], bo[TN];
+  {
+    const int row = (lane >> 4) * 8 + ((lane & 15) >> 2);
+    const uint32_t base = (uint32_t)(uintptr_t)(lds_vp)smem + (lane & 3) * 8;
+#pragma unroll
+    for (int a = 0; a < TM; ++a) ao[a] = base + row * (BM * 2) + (((wm * TM + a) ^ tr_swizzle<BM>(row)) << 5);
+#pragma unroll
+    for (int b = 0; b < TN; ++b) bo[b] = base + A_BYTES + row * (BN * 2) + (((wn * TN + b) ^ tr_swizzle<BN>(row)) << 5);
+  }
+  bf16x8 fa[TM][PLANES], fb[TN];
+  auto read = [&](int buf) {
+    const uint32_t off = buf * STAGE;
+    const float* ws = reinterpret_cast<const float*>(smem + off + A_BYTES + B_BYTES + wave * 256) + (lane >> 4) * 8;
+    const f32x4 w0 = *reinterpret_cast<const f32x4*>(ws), w1 = *reinterpret_cast<const f32x4*>(ws + 4);
+    const float w[8] = {w0[0], w0[1], w0[2], w0[3], w1[0], w1[1], w1[2], w1[3]};
+    bf16x8 raw[4];
+    uint32_t at[4];
+#pragma unroll
+    for (int a = 0; a < 4; ++a) at[a] = ao[a] + off;
+    read_tr4<4 * BM * 2>(at, raw);
+#pragma unroll
+    for (int c = 0; c < TN / 4; ++c) {
+      bf16x8 part[4];
+#pragma unroll
+      for (int b = 0; b < 4; ++b) at[b] = bo[c * 4 + b] + off;
+      read_tr4<4 * BN * 2>(at, part);
+#pragma unroll
+      for (int b = 0; b < 4; ++b) fb[c * 4 + b] = part[b];
+    }
+#pragma unroll
+    for (int a = 0; a < TM; ++a) split_planes<PLANES>(raw[a], w, fa[a]);
+  };
+  auto multiply = [&]() {
+#pragma unroll
+    for (int p = PLANES - 1; p >= 0; --p)
+#pragma unroll
+      for (int a = 0; a < TM; ++a)
+#pragma unroll
+        for (int b = 0; b < TN; ++b) acc[a][b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb[b], fa[a][p], acc[a][b], 0, 0, 0);
+  };
+
+  auto wait_behind = [&](int later) {                                 // at most the loads of the `later` youngest steps outstanding
+    if (later >= STAGES - 2) wait_vmcnt<LOADS * (STAGES - 2)>();
+    else if (later == 1) wait_vmcnt<LOADS>();
+    else wait_vmcnt<0>();
+  };
+#pragma unroll
+  for (int i = 0; i < STAGES - 1; ++i)
+    if (i < nk) stage(i);
+  int buf = 0;
+  auto next = [](int b) { return b == STAGES - 1 ? 0 : b + 1; };
+  auto before = [](int b) { return b == 0 ? STAGES - 1 : b - 1; };
+  if constexpr (NW == 8) {
+    // two wavefronts a SIMD, half a step apart: one multiplies while the other reads and splits (as in lowrank_mfma.hip)
+    const bool late = wave >= 4;
+    wait_behind(nk - 1);
+    barrier_no_fence();
+    if (late) barrier_no_fence();
+    for (int kt = 0; kt < nk; ++kt) {
+      read(buf);
+      if (kt + STAGES - 1 < nk) stage(before(buf));
+      const int later = min(nk - 1, kt + STAGES - 1) - (kt + 1);
+      if (late) wait_behind(later);
+      barrier_no_fence();
+      __builtin_amdgcn_s_setprio(1);
+      multiply();
+      __builtin_amdgcn_s_setprio(0);
+      if (!late) wait_behind(later);
+      barrier_no_fence();
+      buf = next(buf);
+    }
+    if (!late) barrier_no_fence();
+  } else {
+    for (int kt = 0; kt < nk; ++kt) {
+      wait_behind(nk - 1 - kt);
+      barrier_no_fence();
+      if (kt + STAGES - 1 < nk) stage(before(buf));
+      read(buf);
+      multiply();
+      buf = next(buf);
+    }
+  }
+
+  const float f = q.splits == 1 ? q.scale : 1.f;
+  float* out = q.splits == 1 ? q.g : q.slab + (int64_t)split * (q.M + 1) * q.N;
+#pragma unroll
+  for (int a = 0; a < TM; ++a)
+#pragma unroll
+    for (int b = 0; b < TN; ++b) {
+      const int m = m0 + (wm * TM + a) * 16 + (lane & 15), n = n0 + (wn * TN + b) * 16 + (lane >> 4) * 4;
+      if (m < q.M && n < q.N) *reinterpret_cast<f32x4*>(out + (int64_t)m * q.N + n) = f * acc[a][b];
+    }
+}
+
+template <int BM, int WM, int WN, int STAGES, int PLANES>
+int launch(const Sum& q, hipStream_t s) {
+  constexpr int LDS = STAGES * (2 * BK * BM * 2 + WM * WN * 256);
+  const int tiles_n = (q.N + BM - 1) / BM;
+  const int64_t tiles = (int64_t)((q.M + BM - 1) / BM) * tiles_n;
+  const int64_t wgs = (tiles + (q.gb != nullptr ? (q.N + 63) / 64 : 0)) * q.splits;
+  if (wgs > 0x7fffffff) return (int)hipErrorInvalidValue;
+  auto* k = &sum_mfma_kernel<BM, BM, WM, WN, STAGES, PLANES>;
+  static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
+  if (attr != hipSuccess) return (int)attr;
+  k<<<(unsigned)wgs, WM * WN * 64, LDS, s>>>(q, (int)tiles, tiles_n);
+  return last_launch_status();
+}
+
+bool big_tiles(int M, int N) { return (int64_t)((M + 255) / 256) * ((N + 255) / 256) >= 32; }
+
+}  // namespace
+
+namespace evox {
+namespace lr {
+
+// Tiles of 256 x 256 where there are at least 32 of them (2048 x 2048: 64), else of 128 x 128, two workgroups a compute unit.
+// K is split so that the chip is filled once; a split has at least four steps.
+void sum_mfma_plan(Sum& q) {
+  const bool big = big_tiles(q.M, q.N);
+  const int64_t side = big ? 256 : 128, tiles = ((q.M + side - 1) / side) * ((q.N + side - 1) / side);
+  int64_t s = (big ? kNumCU : 2 * kNumCU) / tiles;
+  const int64_t most = (q.K + 127) / 128;
+  if (s > most) s = most;
+  if (s < 1) s = 1;
+  const int64_t per = (q.K + s - 1) / s;
+  q.k_per_split = (per + BK - 1) / BK * BK;
+  q.splits = (int)((q.K + q.k_per_split - 1) / q.k_per_split);
+}
+
+int sum_mfma(const Sum& q, hipStream_t s) {
+  const bool two = q.K >= 16384;
+  if (big_tiles(q.M, q.N)) return two ? launch<256, 4, 2, 4, 2>(q, s) : launch<256, 4, 2, 4, 3>(q, s);
+  return two ? launch<128, 2, 2, 4, 2>(q, s) : launch<128, 2, 2, 4, 3>(q, s);
+}
+
+}  // namespace lr
+}  // namespace evox

@@ -1,0 +1,63 @@
+// Tiles in LDS for the bf16 matrix instructions: counted waits, transposed reads, permuted rows.
+#pragma once
+#include "hip_common.h"
+
+namespace evox {
+namespace lr {
+
+using bf16x8 = __attribute__((ext_vector_type(8))) __bf16;
+using s16x8 = __attribute__((ext_vector_type(8))) short;
+typedef __attribute__((address_space(3))) void* lds_vp;
+typedef const __attribute__((address_space(1))) void* glb_vp;
+
+template <int N>
+__device__ __forceinline__ void wait_vmcnt() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+
+// Transposed reads of two adjacent 4-row blocks each for four columns blocks, waited for in place: the compiler would let no
+// such read (through its builtin) pass a load to LDS that is in flight, which is what the stages are for.
+template <int STEP>
+__device__ __forceinline__ void read_tr4(const uint32_t (&at)[4], bf16x8 (&out)[4]) {
+  uint2 r0, r1, r2, r3, r4, r5, r6, r7;
+  asm volatile(
+      "ds_read_b64_tr_b16 %0, %8\n\tds_read_b64_tr_b16 %1, %8 offset:%12\n\t"
+      "ds_read_b64_tr_b16 %2, %9\n\tds_read_b64_tr_b16 %3, %9 offset:%12\n\t"
+      "ds_read_b64_tr_b16 %4, %10\n\tds_read_b64_tr_b16 %5, %10 offset:%12\n\t"
+      "ds_read_b64_tr_b16 %6, %11\n\tds_read_b64_tr_b16 %7, %11 offset:%12\n\t"
+      "s_waitcnt lgkmcnt(0)"
+      : "=&v"(r0), "=&v"(r1), "=&v"(r2), "=&v"(r3), "=&v"(r4), "=&v"(r5), "=&v"(r6), "=&v"(r7)
+      : "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[3]), "n"(STEP)
+      : "memory");
+  out[0] = __builtin_bit_cast(bf16x8, make_uint4(r0.x, r0.y, r1.x, r1.y));
+  out[1] = __builtin_bit_cast(bf16x8, make_uint4(r2.x, r2.y, r3.x, r3.y));
+  out[2] = __builtin_bit_cast(bf16x8, make_uint4(r4.x, r4.y, r5.x, r5.y));
+  out[3] = __builtin_bit_cast(bf16x8, make_uint4(r6.x, r6.y, r7.x, r7.y));
+}
+template <int STEP>
+__device__ __forceinline__ void read_tr2(const uint32_t (&at)[2], bf16x8 (&out)[2]) {
+  uint2 r0, r1, r2, r3;
+  asm volatile(
+      "ds_read_b64_tr_b16 %0, %4\n\tds_read_b64_tr_b16 %1, %4 offset:%6\n\t"
+      "ds_read_b64_tr_b16 %2, %5\n\tds_read_b64_tr_b16 %3, %5 offset:%6\n\t"
+      "s_waitcnt lgkmcnt(0)"
+      : "=&v"(r0), "=&v"(r1), "=&v"(r2), "=&v"(r3)
+      : "v"(at[0]), "v"(at[1]), "n"(STEP)
+      : "memory");
+  out[0] = __builtin_bit_cast(bf16x8, make_uint4(r0.x, r0.y, r1.x, r1.y));
+  out[1] = __builtin_bit_cast(bf16x8, make_uint4(r2.x, r2.y, r3.x, r3.y));
+}
+
+// permutation of the 32-byte pieces of a row of COLS elements that is read transposed: the 16 rows {r, r + 8, r + 16, r + 24} + 0..3 of one transposed read differ
+template <int COLS>
+__device__ __forceinline__ int tr_swizzle(int row) {
+  return ((row & 3) | (((row >> 3) & 3) << 2)) & (COLS / 16 - 1);
+}
+// a barrier that leaves this wavefront's loads to LDS in flight; no read of LDS moves up across it
+__device__ __forceinline__ void barrier_no_fence() {
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+}  // namespace lr
+}  // namespace evox

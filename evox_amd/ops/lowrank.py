@@ -22,8 +22,8 @@ P, I, I64, F = _native.P, _native.I, _native.I64, _native.F
 _native.register_hip_api({
     "evox_hip_lowrank_linear_ws": (I64, [I64, I, I, I]),
     "evox_hip_lowrank_linear": (I, [P, P, P, P, P, P, P, P, I64, P, P, F, P]),
-    "evox_hip_lowrank_sum_ws": (I64, [I64, I, I, I]),
-    "evox_hip_lowrank_sum": (I, [P, P, P, P, P, P, I64, P, P, F, P]),
+    "evox_hip_lowrank_sum_ws": (I64, [P, P, P, P, P, P, P]),
+    "evox_hip_lowrank_sum": (I, [P, P, P, P, P, P, P, P, I64, F, P]),
 })
 
 _ACT = {"identity": 0, "tanh": 1, "relu": 2, "sigmoid": 3}
@@ -185,14 +185,14 @@ def lowrank_weighted_sum(w: torch.Tensor, a: torch.Tensor, b: torch.Tensor, scal
         return g.zero_(), gb if gb is None else gb.zero_()
     w, a, b = w.contiguous(), _packed(a), _packed(b)
     lib = hip()
-    floats = lib.evox_hip_lowrank_sum_ws(pop, n_in, n_out, r)
-    ws = torch.empty(floats, dtype=torch.float32, device=dev)
     dims = (ctypes.c_int64 * 3)(pop, a.stride(0), b.stride(0))
     ints = (ctypes.c_int * 4)(n_in, n_out, r, DTYPE_CODE[a.dtype])
+    call = (w.data_ptr(), a.data_ptr(), b.data_ptr(), g.data_ptr(), None if gb is None else gb.data_ptr(), ctypes.addressof(dims),
+            ctypes.addressof(ints))
+    floats = lib.evox_hip_lowrank_sum_ws(*call)
+    ws = torch.empty(max(floats, 0), dtype=torch.float32, device=dev)
     with launch_device(dev):
-        check(lib.evox_hip_lowrank_sum(w.data_ptr(), a.data_ptr(), b.data_ptr(), g.data_ptr(),
-                                       None if gb is None else gb.data_ptr(), ws.data_ptr(), floats, ctypes.addressof(dims),
-                                       ctypes.addressof(ints), float(scale), stream_of(g)), "lowrank_weighted_sum")
+        check(lib.evox_hip_lowrank_sum(*call, ws.data_ptr(), floats, float(scale), stream_of(g)), "lowrank_weighted_sum")
     return g, gb
 
 

@@ -95,7 +95,14 @@ struct Linear {
       const float* tr = t + row * R;
       f32x4 d = {0.f, 0.f, 0.f, 0.f};
       if (whole) {
-        for (int j = 0; j < R; ++j, bp += N) {
+        // four rows of B in flight at a time
+        int j = 0;
+        for (; j + 4 <= R; j += 4, bp += 4 * (int64_t)N) {
+          const f32x4 q0 = ld4(bp), q1 = ld4(bp + N), q2 = ld4(bp + 2 * (int64_t)N), q3 = ld4(bp + 3 * (int64_t)N);
+          const float t0 = tr[j], t1 = tr[j + 1], t2 = tr[j + 2], t3 = tr[j + 3];
+          for (int l = 0; l < 4; ++l) d[l] = fmaf(t3, q3[l], fmaf(t2, q2[l], fmaf(t1, q1[l], fmaf(t0, q0[l], d[l]))));
+        }
+        for (; j < R; ++j, bp += N) {
           const f32x4 q = ld4(bp);
           const float tj = tr[j];
           for (int l = 0; l < 4; ++l) d[l] = fmaf(tj, q[l], d[l]);

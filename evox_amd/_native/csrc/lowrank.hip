@@ -10,6 +10,7 @@ using namespace evox::lr;
 namespace evox {
 namespace lr {
 bool linear_mfma_grouped(const Linear& q);                       // lowrank_mfma.hip
+void linear_mfma_plan(Linear& q);
 int linear_mfma(const Linear& q, bool grouped, hipStream_t s);
 void sum_mfma_plan(Sum& q);                                      // lowrank_sum_mfma.hip
 int sum_mfma(const Sum& q, hipStream_t s);
@@ -153,15 +154,122 @@ template <typename T>
 __global__ __launch_bounds__(NT) void linear_join_kernel(Linear q) {
   const int quads = (q.N + 3) / 4;
   const int64_t total = q.rows * quads;
-  for (int64_t i = (int64_t)blockIdx.x * NT + threadIdx.x; i < total; i += (int64_t)gridDim.x * NT) {
+  const int64_t pitch = q.rows * q.N;
+  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
     const int64_t row = i / quads;
     const int n = (int)(i - row * quads) * 4;
     f32x4 v = {0.f, 0.f, 0.f, 0.f};
-    for (int s = 0; s < q.splits; ++s) {
-      const float* p = q.slab + ((int64_t)s * q.rows + row) * q.N + n;
-      for (int l = 0; l < 4; ++l) if (n + l < q.N) v[l] += p[l];
+    const float* p = q.slab + row * q.N + n;
+    if ((q.N & 3) == 0) {
+#pragma unroll 8
+      for (int s = 0; s < q.splits; ++s) v += *reinterpret_cast<const f32x4*>(p + s * pitch);
+    } else {
+      for (int s = 0; s < q.splits; ++s)
+        for (int l = 0; l < 4; ++l) if (n + l < q.N) v[l] += p[s * pitch + l];
     }
     q.finish<T>(row, n, v);
+  }
+}
+
+// Few rows (requests, single tokens): W is read once and that is what the call takes.  A lane owns 16 bytes of a row of W (CPL
+// columns) for all TR rows of x, a workgroup of eight wavefronts FEW_K rows of W (each wavefront every eighth), whose partial
+// sums meet in LDS and then, over the workgroups that share the columns, in linear_join_kernel.  Workgroups behind the ones that
+// multiply compute t, one wavefront for each of its entries, so that it costs no launch of its own.
+constexpr int FEW_K = 128, FEW_NT = 512;
+
+template <typename T, int TR>
+__global__ __launch_bounds__(FEW_NT) void linear_few_kernel(Linear q, int products) {
+  constexpr int CPL = 16 / sizeof(T), COLS = 64 * CPL, PAIR = TR > 1 ? 2 : 1;
+  __shared__ float xs[FEW_K][TR];
+  __shared__ __attribute__((aligned(16))) float red[PAIR][8][COLS];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  if ((int)blockIdx.x >= products) {
+    const int64_t e = (int64_t)((int)blockIdx.x - products) * 8 + wave;
+    if (e >= q.rows * q.R) return;
+    const int64_t row = e / q.R;
+    const int j = (int)(e - row * q.R);
+    const int64_t p = q.individual(row);
+    float s = 0.f;
+    if (p >= 0) {
+      const T* x = q.row_of<T>(row);
+      const T* a = reinterpret_cast<const T*>(q.a) + p * q.sa + (int64_t)j * q.K;
+      if (q.vec & 1) {
+#pragma unroll 4
+        for (int k = lane * 4; k < q.K; k += 256) {
+          const f32x4 xv = ld4(x + k), av = ld4(a + k);
+          for (int l = 0; l < 4; ++l) s = fmaf(xv[l], av[l], s);
+        }
+      } else {
+        for (int k = lane; k < q.K; k += 64) s = fmaf(ld(x + k), ld(a + k), s);
+      }
+    }
+    s = wave_sum(s);
+    if (lane == 0) q.t[e] = q.scale * s;
+    return;
+  }
+  const int split = (int)blockIdx.x % q.splits, n0 = ((int)blockIdx.x / q.splits) * COLS, n = n0 + lane * CPL;
+  const int k0 = split * FEW_K, kn = min(FEW_K, q.K - k0);
+  float acc[TR][CPL];
+#pragma unroll
+  for (int r = 0; r < TR; ++r)
+#pragma unroll
+    for (int c = 0; c < CPL; ++c) acc[r][c] = 0.f;
+  // this wavefront's 16 rows of W, all in flight before x is there
+  constexpr int MINE = FEW_K / 8;
+  uint4 w[MINE];
+  const T* wp = reinterpret_cast<const T*>(q.w) + (int64_t)k0 * q.N + n;
+#pragma unroll
+  for (int i = 0; i < MINE; ++i) {
+    w[i] = make_uint4(0, 0, 0, 0);
+    const int k = i * 8 + wave;
+    if (k < kn && n < q.N) w[i] = *reinterpret_cast<const uint4*>(wp + (int64_t)k * q.N);
+  }
+  for (int i = tid; i < TR * FEW_K; i += FEW_NT) {
+    const int r = i / FEW_K, k = i % FEW_K;
+    xs[k][r] = r < q.rows && k < kn ? ld(q.row_of<T>(r) + k0 + k) : 0.f;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < MINE; ++i) {
+    float c[CPL];
+    const uint32_t u[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+#pragma unroll
+    for (int l = 0; l < 4; ++l) {
+      if constexpr (sizeof(T) == 2) {
+        c[2 * l] = __uint_as_float(u[l] << 16);
+        c[2 * l + 1] = __uint_as_float(u[l] & 0xffff0000u);
+      } else {
+        c[l] = __uint_as_float(u[l]);
+      }
+    }
+    // (rows of W behind K: x is zero there, and so is what stands in w)
+    const float* xr = xs[i * 8 + wave];
+#pragma unroll
+    for (int r = 0; r < TR; ++r) {
+      const float xv = xr[r];
+#pragma unroll
+      for (int l = 0; l < CPL; ++l) acc[r][l] = fmaf(xv, c[l], acc[r][l]);
+    }
+  }
+#pragma unroll
+  for (int r0 = 0; r0 < TR; r0 += PAIR) {
+    if (r0 >= q.rows) break;
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < PAIR; ++r)
+#pragma unroll
+      for (int c = 0; c < CPL; c += 4)
+        *reinterpret_cast<f32x4*>(&red[r][wave][lane * CPL + c]) = f32x4{acc[r0 + r][c], acc[r0 + r][c + 1], acc[r0 + r][c + 2], acc[r0 + r][c + 3]};
+    __syncthreads();
+    for (int i = tid; i < PAIR * COLS; i += FEW_NT) {
+      const int r = i / COLS, c = i % COLS;
+      if (r0 + r < q.rows && n0 + c < q.N) {
+        float s = 0.f;
+#pragma unroll
+        for (int v = 0; v < 8; ++v) s += red[r][v][c];
+        q.slab[((int64_t)split * q.rows + r0 + r) * q.N + n0 + c] = s;
+      }
+    }
   }
 }
 
@@ -246,33 +354,39 @@ __global__ __launch_bounds__(NT) void sum_join_kernel(Sum q) {
   }
 }
 
-// bf16 on the matrix cores at full rate: sixteen-byte pieces everywhere, and enough rows to fill its tiles
-bool mfma_fits(const Linear& q) {
-  auto al = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; };
-  return q.rows >= 128 && q.K >= 64 && q.K % 8 == 0 && q.N % 8 == 0 && q.sx0 % 8 == 0 && q.sx1 % 8 == 0 && al(q.x) && al(q.w) &&
-         al(q.y) && (q.vec & 2);
-}
+enum class Path { kTile, kMfma, kGrouped, kFew };
 
 template <typename T>
-int launch_linear(const Linear& q, hipStream_t s) {
-  if constexpr (sizeof(T) == 2) {
-    if (mfma_fits(q)) {
-      const bool grouped = linear_mfma_grouped(q);
-      if (!grouped) {
-        const int64_t sg = (q.rows + 3) / 4;
-        shrink_kernel<T><<<(unsigned)(sg < 65536 ? sg : 65536), NT, 0, s>>>(q);
-      }
-      return linear_mfma(q, grouped, s);
-    }
+int launch_linear(const Linear& q, Path path, hipStream_t s) {
+  auto join = [&]() {
+    const int64_t quads = q.rows * ((q.N + 3) / 4);
+    // (few outputs: small workgroups, so that they spread over the chip)
+    if (quads < 64 * kNumCU) linear_join_kernel<T><<<(unsigned)((quads + 63) / 64), 64, 0, s>>>(q);
+    else linear_join_kernel<T><<<stream_grid(quads, NT), NT, 0, s>>>(q);
+  };
+  if (path == Path::kFew) {
+    constexpr int COLS = 64 * 16 / (int)sizeof(T);
+    const int products = (q.N + COLS - 1) / COLS * q.splits;
+    const unsigned wgs = (unsigned)(products + (q.rows * q.R + 7) / 8);
+    if (q.rows == 1) linear_few_kernel<T, 1><<<wgs, FEW_NT, 0, s>>>(q, products);
+    else if (q.rows <= 4) linear_few_kernel<T, 4><<<wgs, FEW_NT, 0, s>>>(q, products);
+    else if (q.rows <= 8) linear_few_kernel<T, 8><<<wgs, FEW_NT, 0, s>>>(q, products);
+    else linear_few_kernel<T, 16><<<wgs, FEW_NT, 0, s>>>(q, products);
+    join();
+    return last_launch_status();
   }
-  const int64_t tiles_m = (q.rows + BM - 1) / BM;
-  const int tiles_n = (q.N + BN - 1) / BN;
-  const int64_t wgs = tiles_m * tiles_n * q.splits;
-  if (wgs > 0x7fffffff) return (int)hipErrorInvalidValue;
+  if (path == Path::kGrouped) return linear_mfma(q, true, s);
   const int64_t sg = (q.rows + 3) / 4;
   shrink_kernel<T><<<(unsigned)(sg < 65536 ? sg : 65536), NT, 0, s>>>(q);
-  linear_kernel<T><<<(unsigned)wgs, NT, 0, s>>>(q, tiles_n);
-  if (q.splits > 1) linear_join_kernel<T><<<stream_grid(q.rows * ((q.N + 3) / 4), NT), NT, 0, s>>>(q);
+  if (path == Path::kMfma) {
+    if (const int st = linear_mfma(q, false, s)) return st;
+  } else {
+    const int tiles_n = (q.N + BN - 1) / BN;
+    const int64_t wgs = (q.rows + BM - 1) / BM * tiles_n * q.splits;
+    if (wgs > 0x7fffffff) return (int)hipErrorInvalidValue;
+    linear_kernel<T><<<(unsigned)wgs, NT, 0, s>>>(q, tiles_n);
+  }
+  if (q.splits > 1) join();
   return last_launch_status();
 }
 
@@ -316,19 +430,10 @@ void plan_sum(Sum& q) {
 
 }  // namespace
 
-// Floats of workspace that a call of evox_hip_lowrank_linear takes: t and the partial products.
-EVOX_API int64_t evox_hip_lowrank_linear_ws(int64_t rows, int K, int N, int R) {
-  Linear q{};
-  q.rows = rows; q.K = K; q.N = N; q.R = R;
-  plan_linear(q);
-  return (rows * R + 3) / 4 * 4 + (q.splits > 1 ? (int64_t)q.splits * rows * N : 0);
-}
-
-// dims: rows, pop, per, sx0, sx1, sa, sb.  ints: K, N, R, own_bias, act, dtype (0 fp32, 1 bf16), index type (0 none, 1 int32, 2 int64)
-EVOX_API int evox_hip_lowrank_linear(const void* x, const void* w, const void* a, const void* b, const float* bias,
-                                     const void* index, void* y, float* ws, int64_t ws_floats, const int64_t* dims,
-                                     const int* ints, float scale, void* stream) {
-  Linear q{};
+// Fills in a call and chooses its kernels.
+static int linear_call(const void* x, const void* w, const void* a, const void* b, const float* bias, const void* index, void* y,
+                       const int64_t* dims, const int* ints, float scale, Linear& q, Path& path) {
+  q = Linear{};
   q.x = x; q.w = w; q.a = a; q.b = b; q.bias = bias; q.y = y;
   q.rows = dims[0]; q.pop = dims[1]; q.per = dims[2];
   q.sx0 = dims[3]; q.sx1 = dims[4]; q.sa = dims[5]; q.sb = dims[6];
@@ -337,17 +442,58 @@ EVOX_API int evox_hip_lowrank_linear(const void* x, const void* w, const void* a
   q.index = ints[6] ? index : nullptr;
   q.index64 = ints[6] == 2;
   q.scale = scale;
-  if (q.rows <= 0 || q.N <= 0) return 0;
-  if (q.K <= 0 || q.R <= 0 || q.per <= 0 || dtype < 0 || dtype > 1) return (int)hipErrorInvalidValue;
-  if (ws_floats < evox_hip_lowrank_linear_ws(q.rows, q.K, q.N, q.R)) return (int)hipErrorInvalidValue;
-  plan_linear(q);
-  q.t = ws;
-  q.slab = ws + (q.rows * q.R + 3) / 4 * 4;
+  if (q.rows <= 0 || q.N <= 0 || q.K <= 0 || q.R <= 0 || q.per <= 0 || dtype < 0 || dtype > 1) return (int)hipErrorInvalidValue;
   const int el = dtype ? 2 : 4;
+  auto al = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; };
   if (q.K % 4 == 0 && q.sx0 % 4 == 0 && q.sx1 % 4 == 0 && q.sa % 4 == 0 && aligned4(x, el) && aligned4(a, el)) q.vec |= 1;
   if (q.N % 4 == 0 && q.sb % 4 == 0 && aligned4(b, el) && aligned4(y, el) && (!bias || aligned4(bias, 4))) q.vec |= 2;
   if (q.N % 4 == 0 && aligned4(w, el)) q.vec |= 4;
-  return dtype ? launch_linear<uint16_t>(q, (hipStream_t)stream) : launch_linear<float>(q, (hipStream_t)stream);
+  path = Path::kTile;
+  // few rows: bound by W, where W is more than a few tiles
+  if (q.rows <= 16 && q.N * el % 16 == 0 && al(w) && (int64_t)q.K * q.N >= 1 << 16) {
+    path = Path::kFew;
+    q.splits = (q.K + FEW_K - 1) / FEW_K;
+    q.k_per_split = FEW_K;
+    return 0;
+  }
+  // bf16 on the matrix cores at full rate: sixteen-byte pieces everywhere, and enough rows to fill a good part of a tile
+  if (dtype == 1 && q.rows >= 48 && q.K >= 64 && q.K % 8 == 0 && q.N % 8 == 0 && q.sx0 % 8 == 0 && q.sx1 % 8 == 0 && al(x) && al(w) &&
+      al(y) && (q.vec & 2)) {
+    path = linear_mfma_grouped(q) ? Path::kGrouped : Path::kMfma;
+    if (path == Path::kMfma) linear_mfma_plan(q);
+    else q.splits = 1;
+    return 0;
+  }
+  plan_linear(q);
+  return 0;
+}
+
+static int64_t linear_workspace(const Linear& q, Path path) {
+  if (path == Path::kGrouped) return 0;
+  return (q.rows * q.R + 3) / 4 * 4 + (q.splits > 1 || path == Path::kFew ? (int64_t)q.splits * q.rows * q.N : 0);
+}
+
+// Floats of workspace that the same call of evox_hip_lowrank_linear takes (negative: the call is refused): t and the partial
+// products.  dims: rows, pop, per, sx0, sx1, sa, sb.  ints: K, N, R, own_bias, act, dtype (0 fp32, 1 bf16), index type (0 none,
+// 1 int32, 2 int64)
+EVOX_API int64_t evox_hip_lowrank_linear_ws(const void* x, const void* w, const void* a, const void* b, const float* bias,
+                                            const void* index, void* y, const int64_t* dims, const int* ints) {
+  Linear q;
+  Path path;
+  if (linear_call(x, w, a, b, bias, index, y, dims, ints, 1.f, q, path)) return -1;
+  return linear_workspace(q, path);
+}
+
+EVOX_API int evox_hip_lowrank_linear(const void* x, const void* w, const void* a, const void* b, const float* bias,
+                                     const void* index, void* y, const int64_t* dims, const int* ints, float* ws, int64_t ws_floats,
+                                     float scale, void* stream) {
+  Linear q;
+  Path path;
+  if (const int st = linear_call(x, w, a, b, bias, index, y, dims, ints, scale, q, path)) return st;
+  if (ws_floats < linear_workspace(q, path)) return (int)hipErrorInvalidValue;
+  q.t = ws;
+  q.slab = ws + (q.rows * q.R + 3) / 4 * 4;
+  return ints[5] ? launch_linear<uint16_t>(q, path, (hipStream_t)stream) : launch_linear<float>(q, path, (hipStream_t)stream);
 }
 
 // Whether a sum takes the bf16 matrix instructions: pieces of sixteen bytes, sizes that fill a good part of a tile, and

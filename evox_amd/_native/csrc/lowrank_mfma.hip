@@ -83,8 +83,9 @@ __global__ __launch_bounds__(WM* WN * 64) void linear_mfma_kernel(Linear q, Tile
   const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const int wm = wave / WN, wn = wave % WN;
   const int u = xcd_remap((int)blockIdx.x, (int)gridDim.x);
-  const int tm = u / g.tiles_n;
-  const int n0 = (u % g.tiles_n) * BN;
+  const int split = GROUPED ? 0 : u % q.splits, tile = GROUPED ? u : u / q.splits;
+  const int tm = tile / g.tiles_n;
+  const int n0 = (tile % g.tiles_n) * BN;
   const uint16_t* W = reinterpret_cast<const uint16_t*>(q.w);
   const uint32_t frag0 = (uint32_t)tm * (BM / 16);                    // GROUPED: this tile's first fragment and individual
   const uint32_t first = GROUPED ? frag0 / g.frags_each : 0;
@@ -226,7 +227,9 @@ __global__ __launch_bounds__(WM* WN * 64) void linear_mfma_kernel(Linear q, Tile
     }
   };
 
-  const int nk = (q.K + BK - 1) / BK;
+  // steps of this workgroup (ungrouped: K may be divided, k_per_split a multiple of BK)
+  const int k_first = GROUPED ? 0 : split * (q.k_per_split / BK);
+  const int nk = GROUPED ? (q.K + BK - 1) / BK : (min(q.K, (split + 1) * q.k_per_split) - split * q.k_per_split + BK - 1) / BK;
   int buf = 0;
   if constexpr (NW == 8) {
     // Two wavefronts share a SIMD (wave and wave + 4).  They run half a step apart: while one multiplies, the other reads its
@@ -244,15 +247,15 @@ __global__ __launch_bounds__(WM* WN * 64) void linear_mfma_kernel(Linear q, Tile
     const bool late = wave >= 4;
 #pragma unroll
     for (int i = 0; i < STAGES - 1; ++i)
-      if (i < nk) { stage_x(i, i); stage_w(i, i); }
+      if (i < nk) { stage_x(i, k_first + i); stage_w(i, k_first + i); }
     wait_behind(nk - 1);
     barrier_no_fence();
     if (late) barrier_no_fence();
     for (int kt = 0; kt < nk; ++kt) {
       read(buf);
       if (kt + 3 < nk) {
-        stage_x((buf + 3) & 3, kt + 3);
-        stage_w((buf + 3) & 3, kt + 3);
+        stage_x((buf + 3) & 3, k_first + kt + 3);
+        stage_w((buf + 3) & 3, k_first + kt + 3);
       }
       const int later = min(nk - 1, kt + 3) - (kt + 1);
       if (late) wait_behind(later);
@@ -271,7 +274,7 @@ __global__ __launch_bounds__(WM* WN * 64) void linear_mfma_kernel(Linear q, Tile
     // multiply.
 #pragma unroll
     for (int i = 0; i < STAGES - 1; ++i)
-      if (i < nk) { stage_x(i, i); stage_w(i, i); }
+      if (i < nk) { stage_x(i, k_first + i); stage_w(i, k_first + i); }
     for (int kt = 0; kt < nk; ++kt) {
       static_assert(STAGES <= 4, "the waits of the last steps");
       const int later = nk - 1 - kt;
@@ -281,8 +284,8 @@ __global__ __launch_bounds__(WM* WN * 64) void linear_mfma_kernel(Linear q, Tile
       barrier_no_fence();
       if (kt + STAGES - 1 < nk) {
         const int b = buf == 0 ? STAGES - 1 : buf - 1;
-        stage_x(b, kt + STAGES - 1);
-        stage_w(b, kt + STAGES - 1);
+        stage_x(b, k_first + kt + STAGES - 1);
+        stage_w(b, k_first + kt + STAGES - 1);
       }
       read(buf);
       multiply();
@@ -380,7 +383,10 @@ __global__ __launch_bounds__(WM* WN * 64) void linear_mfma_kernel(Linear q, Tile
         const int n = n0 + wn0 + (lane % LPR) * 4;
         const int64_t row = (int64_t)tm * BM + wm0 + a * 16 + r;
         const f32x4 v = *reinterpret_cast<const f32x4*>(patch + r * PITCH + (lane % LPR) * 4);
-        if (row < q.rows && n < q.N) q.finish<uint16_t>(row, n, v);
+        if (row < q.rows && n < q.N) {
+          if (q.splits == 1) q.finish<uint16_t>(row, n, v);
+          else *reinterpret_cast<f32x4*>(q.slab + ((int64_t)split * q.rows + row) * q.N + n) = v;
+        }
       }
     }
   }
@@ -394,12 +400,13 @@ int launch(const Linear& q, hipStream_t s) {
   g.frags_each = (uint32_t)((q.per + 15) / 16);
   g.frags = SLOTS ? (uint32_t)(q.pop * g.frags_each) : 0;
   const int64_t tiles_m = SLOTS ? ((int64_t)g.frags * 16 + BM - 1) / BM : (q.rows + BM - 1) / BM;
-  if (tiles_m * g.tiles_n > 0x7fffffff) return (int)hipErrorInvalidValue;
+  const int64_t wgs = tiles_m * g.tiles_n * (SLOTS ? 1 : q.splits);
+  if (wgs > 0x7fffffff) return (int)hipErrorInvalidValue;
   auto* k = &linear_mfma_kernel<BM, BN, WM, WN, STAGES, SLOTS>;
   static const hipError_t attr =
       hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
   if (attr != hipSuccess) return (int)attr;
-  k<<<(unsigned)(tiles_m * g.tiles_n), WM * WN * 64, LDS, s>>>(q, g);
+  k<<<(unsigned)wgs, WM * WN * 64, LDS, s>>>(q, g);
   return last_launch_status();
 }
 
@@ -415,10 +422,24 @@ bool linear_mfma_grouped(const Linear& q) {
          q.sa % 8 == 0 && (reinterpret_cast<uintptr_t>(q.a) & 15) == 0;
 }
 
+// Ungrouped: tiles of 256 x 256 where they fill the chip, else of 128 x 64 with K divided over as many workgroups as make about two
+// for each compute unit (eight steps each at least).
+void linear_mfma_plan(Linear& q) {
+  q.splits = 1;
+  q.k_per_split = (q.K + BK - 1) / BK * BK;
+  if (((q.rows + 255) / 256) * ((q.N + 255) / 256) >= kNumCU) return;
+  const int64_t tiles = ((q.rows + 127) / 128) * ((q.N + 63) / 64);
+  int64_t s = 2 * kNumCU / tiles;
+  if (s > q.K / (8 * BK)) s = q.K / (8 * BK);
+  if (s <= 1) return;
+  q.k_per_split = (int)(((q.K + s - 1) / s + BK - 1) / BK * BK);
+  q.splits = (q.K + q.k_per_split - 1) / q.k_per_split;
+}
+
 int linear_mfma(const Linear& q, bool grouped, hipStream_t s) {
   const int64_t big = ((q.rows + 255) / 256) * ((q.N + 255) / 256);
   if (grouped) {
-    // a tile of 256 rows holds A_p of eight individuals: at most 16 / each + 1 of them meet in it, 16 / each where they start together
+    // a tile of 256 rows holds A_p of eight individuals: 16 / each meet in it where they start together, else up to two more
     const int64_t each = (q.per + 15) / 16, meet = 16 % each == 0 ? 16 / each : 16 / each + 2;
     return big >= kNumCU && meet <= 8 ? launch<256, 256, 2, 4, 4, 8>(q, s) : launch<128, 128, 2, 2, 3, 8>(q, s);
   }

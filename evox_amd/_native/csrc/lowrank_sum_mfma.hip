@@ -286,7 +286,7 @@ int launch(const Sum& q, hipStream_t s) {
   return last_launch_status();
 }
 
-bool big_tiles(int M, int N) { return (int64_t)((M + 255) / 256) * ((N + 255) / 256) >= 32; }
+bool big_tiles(int M, int N) { return (int64_t)((M + 255) / 256) * ((N + 255) / 256) >= 12; }
 
 }  // namespace
 

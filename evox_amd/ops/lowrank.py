@@ -20,8 +20,8 @@ from ._util import DTYPE_CODE, check, hip, launch_device, on_gpu, stream_of
 
 P, I, I64, F = _native.P, _native.I, _native.I64, _native.F
 _native.register_hip_api({
-    "evox_hip_lowrank_linear_ws": (I64, [I64, I, I, I]),
-    "evox_hip_lowrank_linear": (I, [P, P, P, P, P, P, P, P, I64, P, P, F, P]),
+    "evox_hip_lowrank_linear_ws": (I64, [P, P, P, P, P, P, P, P, P]),
+    "evox_hip_lowrank_linear": (I, [P, P, P, P, P, P, P, P, P, P, I64, F, P]),
     "evox_hip_lowrank_sum_ws": (I64, [P, P, P, P, P, P, P]),
     "evox_hip_lowrank_sum": (I, [P, P, P, P, P, P, P, P, I64, F, P]),
 })
@@ -119,16 +119,15 @@ def lowrank_linear(x: torch.Tensor, weight: torch.Tensor, a: torch.Tensor, b: to
     bias = bias if bias is None else bias.to(torch.float32).contiguous()
     index = index if index is None else index.contiguous()
     lib = hip()
-    floats = lib.evox_hip_lowrank_linear_ws(rows, n_in, n_out, r)
-    ws = torch.empty(floats, dtype=torch.float32, device=dev)
     dims = (ctypes.c_int64 * 7)(rows, pop, per, x.stride(0), x.stride(1) if x.dim() == 3 else 0, a.stride(0), b.stride(0))
     ints = (ctypes.c_int * 7)(n_in, n_out, r, own_bias, _ACT[activation], DTYPE_CODE[x.dtype],
                               0 if index is None else _INDEX[index.dtype])
+    call = (x.data_ptr(), weight.data_ptr(), a.data_ptr(), b.data_ptr(), None if bias is None else bias.data_ptr(),
+            None if index is None else index.data_ptr(), y.data_ptr(), ctypes.addressof(dims), ctypes.addressof(ints))
+    floats = lib.evox_hip_lowrank_linear_ws(*call)
+    ws = torch.empty(max(floats, 0), dtype=torch.float32, device=dev)
     with launch_device(dev):
-        check(lib.evox_hip_lowrank_linear(
-            x.data_ptr(), weight.data_ptr(), a.data_ptr(), b.data_ptr(), None if bias is None else bias.data_ptr(),
-            None if index is None else index.data_ptr(), y.data_ptr(), ws.data_ptr(), floats, ctypes.addressof(dims),
-            ctypes.addressof(ints), float(scale), stream_of(y)), "lowrank_linear")
+        check(lib.evox_hip_lowrank_linear(*call, ws.data_ptr(), floats, float(scale), stream_of(y)), "lowrank_linear")
     return y
 
 

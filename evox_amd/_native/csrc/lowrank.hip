@@ -9,8 +9,9 @@ using namespace evox::lr;
 
 namespace evox {
 namespace lr {
-bool linear_mfma_grouped(const Linear& q);                       // lowrank_mfma.hip
-void linear_mfma_plan(Linear& q);
+bool linear_mfma_grouped(const Linear& q, int elem);             // lowrank_mfma.hip
+void linear_mfma_plan(Linear& q, int elem);
+template <typename T>
 int linear_mfma(const Linear& q, bool grouped, hipStream_t s);
 void sum_mfma_plan(Sum& q);                                      // lowrank_sum_mfma.hip
 int sum_mfma(const Sum& q, hipStream_t s);
@@ -375,11 +376,11 @@ int launch_linear(const Linear& q, Path path, hipStream_t s) {
     join();
     return last_launch_status();
   }
-  if (path == Path::kGrouped) return linear_mfma(q, true, s);
+  if (path == Path::kGrouped) return linear_mfma<T>(q, true, s);
   const int64_t sg = (q.rows + 3) / 4;
   shrink_kernel<T><<<(unsigned)(sg < 65536 ? sg : 65536), NT, 0, s>>>(q);
   if (path == Path::kMfma) {
-    if (const int st = linear_mfma(q, false, s)) return st;
+    if (const int st = linear_mfma<T>(q, false, s)) return st;
   } else {
     const int tiles_n = (q.N + BN - 1) / BN;
     const int64_t wgs = (q.rows + BM - 1) / BM * tiles_n * q.splits;
@@ -456,11 +457,12 @@ static int linear_call(const void* x, const void* w, const void* a, const void* 
     q.k_per_split = FEW_K;
     return 0;
   }
-  // bf16 on the matrix cores at full rate: sixteen-byte pieces everywhere, and enough rows to fill a good part of a tile
-  if (dtype == 1 && q.rows >= 48 && q.K >= 64 && q.K % 8 == 0 && q.N % 8 == 0 && q.sx0 % 8 == 0 && q.sx1 % 8 == 0 && al(x) && al(w) &&
-      al(y) && (q.vec & 2)) {
-    path = linear_mfma_grouped(q) ? Path::kGrouped : Path::kMfma;
-    if (path == Path::kMfma) linear_mfma_plan(q);
+  // the tiles of lowrank_mfma.hip: sixteen-byte pieces everywhere, and enough rows to fill a good part of a tile
+  const int piece = 16 / el;
+  if (q.rows >= 48 && q.K * el >= 128 && q.K % piece == 0 && q.N % piece == 0 && q.sx0 % piece == 0 && q.sx1 % piece == 0 && al(x) &&
+      al(w) && al(y) && (q.vec & 2)) {
+    path = linear_mfma_grouped(q, el) ? Path::kGrouped : Path::kMfma;
+    if (path == Path::kMfma) linear_mfma_plan(q, el);
     else q.splits = 1;
     return 0;
   }

@@ -1,4 +1,4 @@
-// Low-rank population layer in bf16 on v_mfma_f32_16x16x32_bf16: y = act(x W + bias + s (x A_p^T) B_p + s c_p).
+// Low-rank population layer on v_mfma_f32_16x16x32_bf16 and v_mfma_f32_16x16x4_f32: y = act(x W + bias + s (x A_p^T) B_p + s c_p).
 //
 // A workgroup of WM x WN wavefronts owns BM x BN outputs and walks K in steps of 64.  Both operands go from memory to LDS
 // without passing registers (16 bytes a lane, two stages: the next step's loads are in flight while a step is multiplied).
@@ -25,8 +25,20 @@ using namespace evox::lr;
 
 namespace {
 
-constexpr int BK = 32;
-constexpr int SLOT = 1024;   // bytes of one individual's A_p in a stage: 16 rows of 32 elements
+// A fragment is 16 bytes a lane: 16 rows of 32 bf16, one instruction, or of 16 floats, four.  The order in which the four
+// instructions take k is free as long as both operands agree: a lane gives four consecutive ones.
+template <typename T>
+struct Frag { using type = bf16x8; };
+template <>
+struct Frag<float> { using type = f32x4; };
+__device__ __forceinline__ f32x4 mfma64(bf16x8 a, bf16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f32x4 mfma64(f32x4 a, f32x4 b, f32x4 c) {
+#pragma unroll
+  for (int l = 0; l < 4; ++l) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[l], b[l], c, 0, 0, 0);
+  return c;
+}
+
+constexpr int SLOT = 1024;   // bytes of one individual's A_p in a stage: 16 rows of 64 bytes
 
 __device__ const uint4 kZero = {0, 0, 0, 0};
 
@@ -36,16 +48,11 @@ struct Tiles {
   int tiles_n;
 };
 
+// float32: permutation of the 16-byte pieces of a W row: rows 4 g of the four lane groups of one read fall 16 banks apart
+__device__ __forceinline__ int w32_swizzle(int row) { return ((row >> 2) & 3) << 2; }
 // permutation of the 16-byte pieces of a 64-byte row (x, A_p): eight neighbouring rows of one read fall on eight bank groups
 __device__ __forceinline__ int x_swizzle(int row) { return (row >> 1) & 3; }
 
-// Activations whose result is rounded to bf16: the exponential of the hardware (2^x) is good to 2^-22, and tanh, which would lose
-// its small values in 1 - 2 / (e^2v + 1), is its series below 1/8 (next term 17/315 v^7: 2^-26 of v).
-__device__ __forceinline__ float tanh_bf16(float v) {
-  const float s = v * v, small = v * fmaf(s, fmaf(s, 2.f / 15.f, -1.f / 3.f), 1.f);
-  const float big = 1.f - 2.f * __builtin_amdgcn_rcpf(__expf(2.f * v) + 1.f);
-  return fabsf(v) < 0.125f ? small : big;
-}
 template <int TN>
 __device__ __forceinline__ void activate_all(f32x4 (&v)[TN], int act) {
   if (act == 1) {
@@ -66,17 +73,18 @@ __device__ __forceinline__ void activate_all(f32x4 (&v)[TN], int act) {
   }
 }
 
-template <int BM, int BN, int WM, int WN, int STAGES, int SLOTS>
+template <typename T, int BM, int BN, int WM, int WN, int STAGES, int SLOTS>
 __global__ __launch_bounds__(WM* WN * 64) void linear_mfma_kernel(Linear q, Tiles g) {
-  constexpr bool GROUPED = SLOTS > 0;
+  constexpr bool GROUPED = SLOTS > 0, BF = sizeof(T) == 2;
+  constexpr int BK = 64 / sizeof(T), E16 = 16 / sizeof(T);             // k of a step, elements of a 16-byte piece
   constexpr int NW = WM * WN;
   constexpr int TM = BM / WM / 16, TN = BN / WN / 16;
-  constexpr int X_BYTES = BM * BK * 2, W_BYTES = BK * BN * 2, STAGE = X_BYTES + W_BYTES + SLOTS * SLOT;
+  constexpr int X_BYTES = BM * 64, W_BYTES = BN * 64, W_ROW = BN * (int)sizeof(T), STAGE = X_BYTES + W_BYTES + SLOTS * SLOT;
   constexpr int XI = X_BYTES / 1024 / NW, WI = W_BYTES / 1024 / NW, AI = SLOTS / NW;   // wave-instructions per stage
   constexpr int LOADS = XI + WI + AI;
   constexpr int TT = (TM + WN - 1) / WN;                              // t fragments of a wavefront
   static_assert(X_BYTES % (1024 * NW) == 0 && W_BYTES % (1024 * NW) == 0 && SLOTS % NW == 0, "whole wave-instructions");
-  static_assert(TN == 4 || TN == 2, "column blocks of a wavefront");
+  static_assert(!BF || TN == 4 || TN == 2, "column blocks of a wavefront");
   static_assert(STAGES >= 3 && LOADS * (STAGES - 2) <= 63 && STAGES * STAGE <= 160 * 1024, "counted waits and LDS");
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int lane = threadIdx.x & 63;
@@ -86,7 +94,7 @@ __global__ __launch_bounds__(WM* WN * 64) void linear_mfma_kernel(Linear q, Tile
   const int split = GROUPED ? 0 : u % q.splits, tile = GROUPED ? u : u / q.splits;
   const int tm = tile / g.tiles_n;
   const int n0 = (tile % g.tiles_n) * BN;
-  const uint16_t* W = reinterpret_cast<const uint16_t*>(q.w);
+  const T* W = reinterpret_cast<const T*>(q.w);
   const uint32_t frag0 = (uint32_t)tm * (BM / 16);                    // GROUPED: this tile's first fragment and individual
   const uint32_t first = GROUPED ? frag0 / g.frags_each : 0;
 
@@ -109,21 +117,21 @@ __global__ __launch_bounds__(WM* WN * 64) void linear_mfma_kernel(Linear q, Tile
   const char* as[AI > 0 ? AI : 1];
   int xk, wk[WI];
   // a wave-instruction brings 16 rows of 64 bytes (x, A_p) or 1024 / (2 BN) rows of W
-  xk = ((lane & 3) ^ x_swizzle(lane >> 2)) * 8;                       // first k of this lane's piece (rows repeat mod 16)
+  xk = ((lane & 3) ^ x_swizzle(lane >> 2)) * E16;                     // first k of this lane's piece (rows repeat mod 16)
 #pragma unroll
   for (int j = 0; j < XI; ++j) {
     int64_t p, r;
     if (!place((j * NW + wave) * 16 + (lane >> 2), p, r)) place(0, p, r);   // (results of such places are not stored)
-    const uint16_t* x = reinterpret_cast<const uint16_t*>(q.x);
+    const T* x = reinterpret_cast<const T*>(q.x);
     if constexpr (GROUPED) x += p * q.sx0 + r * q.sx1;
-    else x = q.row_of<uint16_t>(r);
+    else x = q.row_of<T>(r);
     xs[j] = reinterpret_cast<const char*>(x + xk);
   }
 #pragma unroll
   for (int j = 0; j < WI; ++j) {
     const int byte = (j * NW + wave) * 1024 + lane * 16;
-    const int row = byte / (BN * 2), c16 = byte % (BN * 2) / 16;
-    int n = n0 + (((c16 >> 1) ^ tr_swizzle<BN>(row)) * 16 + (c16 & 1) * 8);
+    const int row = byte / W_ROW, c16 = byte % W_ROW / 16;
+    int n = n0 + (BF ? ((c16 >> 1) ^ tr_swizzle<BN>(row)) * 16 + (c16 & 1) * 8 : (c16 ^ w32_swizzle(row)) * 4);
     if (n >= q.N) n = 0;                                              // columns that are not stored
     wk[j] = row;
     ws[j] = reinterpret_cast<const char*>(W + (int64_t)row * q.N + n);
@@ -133,9 +141,9 @@ __global__ __launch_bounds__(WM* WN * 64) void linear_mfma_kernel(Linear q, Tile
     // (a slot behind the individuals of this tile's last fragment holds zeros)
     const uint32_t p = first + j * NW + wave, end = (min(frag0 + BM / 16, g.frags) - 1) / g.frags_each;
     const int row = lane >> 2;
-    as[j] = row < q.R && p <= end ? reinterpret_cast<const char*>(reinterpret_cast<const uint16_t*>(q.a) + (int64_t)p * q.sa + (int64_t)row * q.K + xk) : nullptr;
+    as[j] = row < q.R && p <= end ? reinterpret_cast<const char*>(reinterpret_cast<const T*>(q.a) + (int64_t)p * q.sa + (int64_t)row * q.K + xk) : nullptr;
   }
-  const int64_t wstep = (int64_t)BK * q.N * 2;
+  const int64_t wstep = (int64_t)BK * q.N * sizeof(T);
   const char* const zero = reinterpret_cast<const char*>(&kZero);
   auto stage_x = [&](int buf, int kt) {
     char* s = smem + buf * STAGE;
@@ -143,7 +151,7 @@ __global__ __launch_bounds__(WM* WN * 64) void linear_mfma_kernel(Linear q, Tile
     const bool tail = k0 + BK > q.K;
 #pragma unroll
     for (int j = 0; j < XI; ++j) {
-      const char* p = xs[j] + (int64_t)kt * (BK * 2);
+      const char* p = xs[j] + (int64_t)kt * 64;
       if (tail && k0 + xk >= q.K) p = zero;
       __builtin_amdgcn_global_load_lds((glb_vp)p, (lds_vp)(s + (j * NW + wave) * 1024), 16, 0, 0);
     }
@@ -160,7 +168,7 @@ __global__ __launch_bounds__(WM* WN * 64) void linear_mfma_kernel(Linear q, Tile
     }
 #pragma unroll
     for (int j = 0; j < AI; ++j) {
-      const char* p = as[j] + (int64_t)kt * (BK * 2);
+      const char* p = as[j] + (int64_t)kt * 64;
       if (as[j] == nullptr || (tail && k0 + xk >= q.K)) p = zero;
       __builtin_amdgcn_global_load_lds((glb_vp)p, (lds_vp)(s + X_BYTES + W_BYTES + (j * NW + wave) * SLOT), 16, 0, 0);
     }
@@ -179,11 +187,17 @@ __global__ __launch_bounds__(WM* WN * 64) void linear_mfma_kernel(Linear q, Tile
   // reads of W — row 8 (lane >> 4) + (lane & 15) / 4, four columns at 4 (lane & 3) of a 16-column piece
   const int xo = (lane & 15) * 64 + (((lane >> 4) ^ x_swizzle(lane & 15)) << 4);
   uint32_t wo[TN];
-  {
+  if constexpr (BF) {
     const int row = (lane >> 4) * 8 + ((lane & 15) >> 2);
-    const uint32_t base = (uint32_t)(uintptr_t)(lds_vp)smem + X_BYTES + row * (BN * 2) + (lane & 3) * 8;
+    const uint32_t base = (uint32_t)(uintptr_t)(lds_vp)smem + X_BYTES + row * W_ROW + (lane & 3) * 8;
 #pragma unroll
     for (int b = 0; b < TN; ++b) wo[b] = base + (((wn * TN + b) ^ tr_swizzle<BN>(row)) << 5);
+  } else {
+    // column lane & 15 of a 16-column block in rows 4 (lane >> 4) + 0..3, which share a permutation
+    const int row = (lane >> 4) * 4;
+#pragma unroll
+    for (int b = 0; b < TN; ++b)
+      wo[b] = X_BYTES + row * W_ROW + ((((wn * TN + b) * 4 + ((lane & 15) >> 2)) ^ w32_swizzle(row)) << 4) + (lane & 3) * 4;
   }
   int ao[TT];                                                         // offsets of A_p's fragments for this wavefront's t
   int to[TT];                                                         // and of x's
@@ -196,34 +210,42 @@ __global__ __launch_bounds__(WM* WN * 64) void linear_mfma_kernel(Linear q, Tile
       to[i] = (wm0 + a * 16) * 64 + xo;
     }
   }
-  bf16x8 fx[TM], fw[TN], fa[TT], ft[TT];
+  typename Frag<T>::type fx[TM], fw[TN], fa[TT], ft[TT];
+  using F = typename Frag<T>::type;
   auto read = [&](int buf) {
     const char* s = smem + buf * STAGE;
 #pragma unroll
-    for (int a = 0; a < TM; ++a) fx[a] = *reinterpret_cast<const bf16x8*>(s + (wm0 + a * 16) * 64 + xo);
+    for (int a = 0; a < TM; ++a) fx[a] = *reinterpret_cast<const F*>(s + (wm0 + a * 16) * 64 + xo);
     if constexpr (GROUPED) {
       // (which x fragments t needs depends on the wavefront: they are read again rather than chosen among registers; a branch
       // around the two instructions for each choice cost more, 408 against 377 us for the multiplying alone)
 #pragma unroll
       for (int i = 0; i < TT; ++i) {
-        fa[i] = *reinterpret_cast<const bf16x8*>(s + ao[i]);
-        ft[i] = *reinterpret_cast<const bf16x8*>(s + to[i]);
+        fa[i] = *reinterpret_cast<const F*>(s + ao[i]);
+        ft[i] = *reinterpret_cast<const F*>(s + to[i]);
       }
     }
-    uint32_t at[TN];
+    if constexpr (BF) {
+      uint32_t at[TN];
 #pragma unroll
-    for (int b = 0; b < TN; ++b) at[b] = wo[b] + buf * STAGE;
-    if constexpr (TN == 4) read_tr4<4 * BN * 2>(at, fw);
-    else read_tr2<4 * BN * 2>(at, fw);
+      for (int b = 0; b < TN; ++b) at[b] = wo[b] + buf * STAGE;
+      if constexpr (TN == 4) read_tr4<4 * W_ROW>(at, fw);
+      else read_tr2<4 * W_ROW>(at, fw);
+    } else {
+#pragma unroll
+      for (int b = 0; b < TN; ++b)
+#pragma unroll
+        for (int l = 0; l < 4; ++l) fw[b][l] = *reinterpret_cast<const float*>(s + wo[b] + l * W_ROW);
+    }
   };
   auto multiply = [&]() {
 #pragma unroll
     for (int a = 0; a < TM; ++a)
 #pragma unroll
-      for (int b = 0; b < TN; ++b) acc[a][b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fw[b], fx[a], acc[a][b], 0, 0, 0);
+      for (int b = 0; b < TN; ++b) acc[a][b] = mfma64(fw[b], fx[a], acc[a][b]);
     if constexpr (GROUPED) {
 #pragma unroll
-      for (int i = 0; i < TT; ++i) tacc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fa[i], ft[i], tacc[i], 0, 0, 0);
+      for (int i = 0; i < TT; ++i) tacc[i] = mfma64(fa[i], ft[i], tacc[i]);
     }
   };
 
@@ -296,33 +318,37 @@ __global__ __launch_bounds__(WM* WN * 64) void linear_mfma_kernel(Linear q, Tile
   __syncthreads();
 
   if constexpr (GROUPED) {
-    // t in LDS: rows of 32 bf16, s t rounded to bf16, then what that leaves
-    uint16_t* ts = reinterpret_cast<uint16_t*>(smem);
-    constexpr int T_BYTES = BM * 64, W16 = TN * 16, PITCH = W16 + 8;
-    static_assert(T_BYTES + NW * 16 * PITCH * 2 <= STAGES * STAGE, "t and the patches fit the stages");
-    uint16_t* patch = reinterpret_cast<uint16_t*>(smem + T_BYTES) + wave * 16 * PITCH;
-    const int k8 = (lane >> 4) * 8, j16 = lane & 15;
+    // t in LDS, 64 bytes a row: 16 floats, or s t rounded to bf16 and then what that leaves
+    constexpr int T_BYTES = BM * 64, W16 = TN * 16, PITCH = W16 + E16;
+    static_assert(T_BYTES + NW * 16 * PITCH * (int)sizeof(T) <= STAGES * STAGE, "t and the patches fit the stages");
+    T* patch = reinterpret_cast<T*>(smem + T_BYTES) + wave * 16 * PITCH;
+    const int j16 = lane & 15, g4 = (lane >> 4) * 4;
 #pragma unroll
     for (int i = 0; i < TT; ++i) {
       const int a = wn * TT + i;
       if (a < TM) {
-        uint16_t hi[4], lo[4];
+        char* o = smem + (wm0 + a * 16 + j16) * 64;
+        f32x4 v;
+        // (places behind the rank: zero even where the row of x is not finite)
 #pragma unroll
-        for (int l = 0; l < 4; ++l) {
-          // (places behind the rank: zero even where the row of x is not finite)
-          const float v = (lane >> 4) * 4 + l < q.R ? q.scale * tacc[i][l] : 0.f;
-          hi[l] = (uint16_t)f2bf(v);
-          const float rest = v - bf2f(hi[l]);
-          lo[l] = rest == rest ? (uint16_t)f2bf(rest) : 0;            // (an infinite v leaves no rest)
+        for (int l = 0; l < 4; ++l) v[l] = g4 + l < q.R ? q.scale * tacc[i][l] : 0.f;
+        if constexpr (BF) {
+          f32x4 rest;
+#pragma unroll
+          for (int l = 0; l < 4; ++l) {
+            rest[l] = v[l] - bf2f(f2bf(v[l]));
+            if (rest[l] != rest[l]) rest[l] = 0.f;                    // (an infinite v leaves no rest)
+          }
+          st4(reinterpret_cast<uint16_t*>(o) + g4, v);
+          st4(reinterpret_cast<uint16_t*>(o) + 16 + g4, rest);
+        } else {
+          *reinterpret_cast<f32x4*>(reinterpret_cast<float*>(o) + g4) = v;
         }
-        uint16_t* o = ts + (wm0 + a * 16 + j16) * 32 + (lane >> 4) * 4;
-        *reinterpret_cast<uint2*>(o) = make_uint2(hi[0] | (uint32_t)hi[1] << 16, hi[2] | (uint32_t)hi[3] << 16);
-        *reinterpret_cast<uint2*>(o + 16) = make_uint2(lo[0] | (uint32_t)lo[1] << 16, lo[2] | (uint32_t)lo[3] << 16);
       }
     }
     __syncthreads();
     uint32_t last = 0xffffffffu;
-    bf16x8 fb[TN];
+    F fb[TN];
     f32x4 own[TN];                                                    // s c_p + bias of this lane's columns
 #pragma unroll
     for (int a = 0; a < TM; ++a) {
@@ -332,18 +358,24 @@ __global__ __launch_bounds__(WM* WN * 64) void linear_mfma_kernel(Linear q, Tile
       const int64_t r0 = (int64_t)(f - p * g.frags_each) * 16;
       if (p != last) {
         last = p;
-        const uint16_t* bp = reinterpret_cast<const uint16_t*>(q.b) + (int64_t)p * q.sb;
+        const T* bp = reinterpret_cast<const T*>(q.b) + (int64_t)p * q.sb;
 #pragma unroll
         for (int b = 0; b < TN; ++b) {
           const int n = n0 + wn0 + b * 16;
-          s16x8 v;
+          // (bf16: both halves of t meet the same rows of B_p)
+          if constexpr (BF) {
+            s16x8 v;
 #pragma unroll
-          for (int l = 0; l < 8; ++l) {
-            const int j = (k8 & 15) + l;
-            v[l] = j < q.R && n + j16 < q.N ? (short)bp[(int64_t)j * q.N + n + j16] : (short)0;
+            for (int l = 0; l < 8; ++l) {
+              const int j = ((lane >> 4) * 8 & 15) + l;
+              v[l] = j < q.R && n + j16 < q.N ? (short)bp[(int64_t)j * q.N + n + j16] : (short)0;
+            }
+            fb[b] = __builtin_bit_cast(F, v);
+          } else {
+#pragma unroll
+            for (int l = 0; l < 4; ++l) fb[b][l] = g4 + l < q.R && n + j16 < q.N ? bp[(int64_t)(g4 + l) * q.N + n + j16] : 0.f;
           }
-          fb[b] = __builtin_bit_cast(bf16x8, v);
-          const int nc = n + (lane >> 4) * 4;
+          const int nc = n + g4;
           own[b] = f32x4{0.f, 0.f, 0.f, 0.f};
           if (nc < q.N) {
             if (q.bias != nullptr) own[b] = *reinterpret_cast<const f32x4*>(q.bias + nc);
@@ -351,25 +383,33 @@ __global__ __launch_bounds__(WM* WN * 64) void linear_mfma_kernel(Linear q, Tile
           }
         }
       }
-      const bf16x8 ft = *reinterpret_cast<const bf16x8*>(ts + (wm0 + a * 16 + j16) * 32 + k8);
+      const F ft = *reinterpret_cast<const F*>(smem + (wm0 + a * 16 + j16) * 64 + (lane >> 4) * 16);
 #pragma unroll
-      for (int b = 0; b < TN; ++b) acc[a][b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb[b], ft, acc[a][b], 0, 0, 0) + own[b];
-      activate_all(acc[a], q.act);
+      for (int b = 0; b < TN; ++b) acc[a][b] = mfma64(fb[b], ft, acc[a][b]) + own[b];
+      if constexpr (BF) activate_all(acc[a], q.act);
 #pragma unroll
-      for (int b = 0; b < TN; ++b) st4(patch + j16 * PITCH + b * 16 + (lane >> 4) * 4, acc[a][b]);
-      // whole rows of the wavefront's columns: 16 bytes a lane
-      constexpr int LPR = W16 / 8, RPS = 64 / LPR;
-#pragma unroll
+      for (int b = 0; b < TN; ++b) st4(patch + j16 * PITCH + b * 16 + g4, acc[a][b]);
+      // whole rows of the wavefront's columns: 16 bytes a lane (float32: activated here, where the code stands once per fragment)
+      constexpr int LPR = W16 / E16, RPS = 64 / LPR;
+#pragma unroll(BF ? 16 / RPS : 1)
       for (int i = 0; i < 16 / RPS; ++i) {
-        const int r = i * RPS + lane / LPR, n = n0 + wn0 + (lane % LPR) * 8;
-        const uint4 v = *reinterpret_cast<const uint4*>(patch + r * PITCH + (lane % LPR) * 8);
+        const int r = i * RPS + lane / LPR, n = n0 + wn0 + (lane % LPR) * E16;
+        uint4 v = *reinterpret_cast<const uint4*>(patch + r * PITCH + (lane % LPR) * E16);
+        if constexpr (!BF) {
+          if (q.act != 0) {
+            f32x4 w = __builtin_bit_cast(f32x4, v);
+#pragma unroll
+            for (int l = 0; l < 4; ++l) w[l] = activate(w[l], q.act);
+            v = __builtin_bit_cast(uint4, w);
+          }
+        }
         if (r0 + r < q.per && n < q.N)
-          *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(q.y) + ((int64_t)p * q.per + r0 + r) * q.N + n) = v;
+          *reinterpret_cast<uint4*>(reinterpret_cast<T*>(q.y) + ((int64_t)p * q.per + r0 + r) * q.N + n) = v;
       }
     }
   } else {
     // sixteen rows at a time through a patch of LDS of the wavefront's own, so that a row's columns lie in neighbouring lanes
-    // (whole lines of B and y) and the long code of a row's end is there once
+    // (whole lines of B and y)
     constexpr int W16 = TN * 16, PITCH = W16 + 4, LPR = W16 / 4, RPS = 64 / LPR;      // lanes per row, rows per step
     static_assert(NW * 16 * PITCH * 4 <= STAGES * STAGE, "the patches fit the stages");
     float* patch = reinterpret_cast<float*>(smem) + wave * 16 * PITCH;
@@ -378,13 +418,15 @@ __global__ __launch_bounds__(WM* WN * 64) void linear_mfma_kernel(Linear q, Tile
 #pragma unroll
       for (int b = 0; b < TN; ++b)
         *reinterpret_cast<f32x4*>(patch + (lane & 15) * PITCH + b * 16 + (lane >> 4) * 4) = acc[a][b];
-#pragma unroll 1
-      for (int r = lane / LPR; r < 16; r += RPS) {
+      // (both steps' loads in flight where the tile is small; the code of the large one would not unroll)
+#pragma unroll(TM <= 4 ? 16 / RPS : 1)
+      for (int i = 0; i < 16 / RPS; ++i) {
+        const int r = i * RPS + lane / LPR;
         const int n = n0 + wn0 + (lane % LPR) * 4;
         const int64_t row = (int64_t)tm * BM + wm0 + a * 16 + r;
         const f32x4 v = *reinterpret_cast<const f32x4*>(patch + r * PITCH + (lane % LPR) * 4);
         if (row < q.rows && n < q.N) {
-          if (q.splits == 1) q.finish<uint16_t>(row, n, v);
+          if (q.splits == 1) q.finish<T>(row, n, v);
           else *reinterpret_cast<f32x4*>(q.slab + ((int64_t)split * q.rows + row) * q.N + n) = v;
         }
       }
@@ -392,9 +434,9 @@ __global__ __launch_bounds__(WM* WN * 64) void linear_mfma_kernel(Linear q, Tile
   }
 }
 
-template <int BM, int BN, int WM, int WN, int STAGES, int SLOTS>
+template <typename T, int BM, int BN, int WM, int WN, int STAGES, int SLOTS>
 int launch(const Linear& q, hipStream_t s) {
-  constexpr int LDS = STAGES * (BM * BK * 2 + BK * BN * 2 + SLOTS * SLOT);
+  constexpr int LDS = STAGES * ((BM + BN) * 64 + SLOTS * SLOT);
   Tiles g{};
   g.tiles_n = (q.N + BN - 1) / BN;
   g.frags_each = (uint32_t)((q.per + 15) / 16);
@@ -402,7 +444,7 @@ int launch(const Linear& q, hipStream_t s) {
   const int64_t tiles_m = SLOTS ? ((int64_t)g.frags * 16 + BM - 1) / BM : (q.rows + BM - 1) / BM;
   const int64_t wgs = tiles_m * g.tiles_n * (SLOTS ? 1 : q.splits);
   if (wgs > 0x7fffffff) return (int)hipErrorInvalidValue;
-  auto* k = &linear_mfma_kernel<BM, BN, WM, WN, STAGES, SLOTS>;
+  auto* k = &linear_mfma_kernel<T, BM, BN, WM, WN, STAGES, SLOTS>;
   static const hipError_t attr =
       hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
   if (attr != hipSuccess) return (int)attr;
@@ -415,36 +457,46 @@ int launch(const Linear& q, hipStream_t s) {
 namespace evox {
 namespace lr {
 
-bool linear_mfma_grouped(const Linear& q) {
+bool linear_mfma_grouped(const Linear& q, int elem) {
   // fragments at least 70 % full: the empty rows cost more than the separate pass over x otherwise
   const int64_t each = (q.per + 15) / 16;
   return q.index == nullptr && q.R <= 16 && q.per >= 16 && 10 * q.per >= 7 * 16 * each && q.pop * each < 0x7fffffff / 16 &&
-         q.sa % 8 == 0 && (reinterpret_cast<uintptr_t>(q.a) & 15) == 0;
+         q.sa * elem % 16 == 0 && (reinterpret_cast<uintptr_t>(q.a) & 15) == 0;
 }
 
-// Ungrouped: tiles of 256 x 256 where they fill the chip, else of 128 x 64 with K divided over as many workgroups as make about two
-// for each compute unit (eight steps each at least).
-void linear_mfma_plan(Linear& q) {
+static int64_t tiles_of(const Linear& q, int side) { return ((q.rows + side - 1) / side) * ((q.N + side - 1) / side); }
+
+// Ungrouped: the largest tiles that fill the chip, else the smallest with K divided over as many workgroups as make about two for
+// each compute unit (256 k each at least).
+void linear_mfma_plan(Linear& q, int elem) {
+  const int bk = 64 / elem;
   q.splits = 1;
-  q.k_per_split = (q.K + BK - 1) / BK * BK;
-  if (((q.rows + 255) / 256) * ((q.N + 255) / 256) >= kNumCU) return;
-  const int64_t tiles = ((q.rows + 127) / 128) * ((q.N + 63) / 64);
-  int64_t s = 2 * kNumCU / tiles;
-  if (s > q.K / (8 * BK)) s = q.K / (8 * BK);
+  q.k_per_split = (q.K + bk - 1) / bk * bk;
+  if (tiles_of(q, 128) >= kNumCU) return;
+  int64_t s = 2 * kNumCU / tiles_of(q, 64);
+  if (s > q.K / 256) s = q.K / 256;
   if (s <= 1) return;
-  q.k_per_split = (int)(((q.K + s - 1) / s + BK - 1) / BK * BK);
+  q.k_per_split = (int)(((q.K + s - 1) / s + bk - 1) / bk * bk);
   q.splits = (q.K + q.k_per_split - 1) / q.k_per_split;
 }
 
+template <typename T>
 int linear_mfma(const Linear& q, bool grouped, hipStream_t s) {
-  const int64_t big = ((q.rows + 255) / 256) * ((q.N + 255) / 256);
+  // (float32 products last sixteen times as long as the reads that feed them: nothing is gained by the largest tiles)
+  const bool big = sizeof(T) == 2 && tiles_of(q, 256) >= kNumCU, medium = tiles_of(q, 128) >= kNumCU;
   if (grouped) {
     // a tile of 256 rows holds A_p of eight individuals: 16 / each meet in it where they start together, else up to two more
     const int64_t each = (q.per + 15) / 16, meet = 16 % each == 0 ? 16 / each : 16 / each + 2;
-    return big >= kNumCU && meet <= 8 ? launch<256, 256, 2, 4, 4, 8>(q, s) : launch<128, 128, 2, 2, 3, 8>(q, s);
+    if constexpr (sizeof(T) == 2)
+      if (big && meet <= 8) return launch<T, 256, 256, 2, 4, 4, 8>(q, s);
+    return medium ? launch<T, 128, 128, 2, 2, 3, 8>(q, s) : launch<T, 64, 64, 2, 2, 4, 4>(q, s);
   }
-  return big >= kNumCU ? launch<256, 256, 2, 4, 4, 0>(q, s) : launch<128, 64, 2, 2, 4, 0>(q, s);
+  if constexpr (sizeof(T) == 2)
+    if (big) return launch<T, 256, 256, 2, 4, 4, 0>(q, s);
+  return medium ? launch<T, 128, 128, 2, 2, 3, 0>(q, s) : launch<T, 64, 64, 2, 2, 4, 0>(q, s);
 }
+template int linear_mfma<uint16_t>(const Linear&, bool, hipStream_t);
+template int linear_mfma<float>(const Linear&, bool, hipStream_t);
 
 }  // namespace lr
 }  // namespace evox

@@ -13,8 +13,8 @@ bool linear_mfma_grouped(const Linear& q, int elem);             // lowrank_mfma
 void linear_mfma_plan(Linear& q, int elem);
 template <typename T>
 int linear_mfma(const Linear& q, bool grouped, hipStream_t s);
-void sum_mfma_plan(Sum& q);                                      // lowrank_sum_mfma.hip
-int sum_mfma(const Sum& q, hipStream_t s);
+void sum_mfma_plan(Sum& q, int elem);                            // lowrank_sum_mfma.hip
+int sum_mfma(const Sum& q, int elem, hipStream_t s);
 }  // namespace lr
 }  // namespace evox
 
@@ -498,17 +498,18 @@ EVOX_API int evox_hip_lowrank_linear(const void* x, const void* w, const void* a
   return ints[5] ? launch_linear<uint16_t>(q, path, (hipStream_t)stream) : launch_linear<float>(q, path, (hipStream_t)stream);
 }
 
-// Whether a sum takes the bf16 matrix instructions: pieces of sixteen bytes, sizes that fill a good part of a tile, and
+// Whether a sum takes the tiles of lowrank_sum_mfma.hip: pieces of sixteen bytes, sizes that fill a good part of a tile, and
 // enough terms that a step of 32 is not mostly empty.
 static bool sum_takes_mfma(int64_t pop, int M, int N, int R, int dtype, int64_t sa, int64_t sb, const void* a, const void* b,
                            const void* g) {
   auto al = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; };
-  return dtype == 1 && M % 8 == 0 && N % 8 == 0 && M >= 64 && N >= 64 && pop * R >= 64 && sa % 8 == 0 && sb % 8 == 0 && al(a) &&
+  const int piece = dtype ? 8 : 4;
+  return M % piece == 0 && N % piece == 0 && M >= 48 && N >= 48 && pop * R >= 64 && sa % piece == 0 && sb % piece == 0 && al(a) &&
          al(b) && al(g);
 }
 
-static int64_t sum_workspace(Sum& q, bool mfma) {
-  if (mfma) sum_mfma_plan(q);
+static int64_t sum_workspace(Sum& q, bool mfma, int dtype) {
+  if (mfma) sum_mfma_plan(q, dtype ? 2 : 4);
   else plan_sum(q);
   return q.splits > 1 ? (int64_t)q.splits * (q.M + 1) * q.N : 0;
 }
@@ -537,7 +538,7 @@ EVOX_API int64_t evox_hip_lowrank_sum_ws(const float* w, const void* a, const vo
   Sum q;
   bool mfma;
   if (sum_call(w, a, b, g, gb, dims, ints, 1.f, q, mfma)) return -1;
-  return sum_workspace(q, mfma);
+  return sum_workspace(q, mfma, ints[3]);
 }
 
 EVOX_API int evox_hip_lowrank_sum(const float* w, const void* a, const void* b, float* g, float* gb, const int64_t* dims,
@@ -545,11 +546,11 @@ EVOX_API int evox_hip_lowrank_sum(const float* w, const void* a, const void* b, 
   Sum q;
   bool mfma;
   if (const int st = sum_call(w, a, b, g, gb, dims, ints, scale, q, mfma)) return st;
-  if (ws_floats < sum_workspace(q, mfma)) return (int)hipErrorInvalidValue;
+  if (ws_floats < sum_workspace(q, mfma, ints[3])) return (int)hipErrorInvalidValue;
   q.slab = ws;
   hipStream_t s = (hipStream_t)stream;
   if (mfma) {
-    if (const int st = sum_mfma(q, s)) return st;
+    if (const int st = sum_mfma(q, ints[3] ? 2 : 4, s)) return st;
     if (q.splits > 1) sum_join_kernel<<<stream_grid((int64_t)(q.M + 1) * q.N, NT), NT, 0, s>>>(q);
     return last_launch_status();
   }

@@ -25,19 +25,6 @@ using namespace evox::lr;
 
 namespace {
 
-// A fragment is 16 bytes a lane: 16 rows of 32 bf16, one instruction, or of 16 floats, four.  The order in which the four
-// instructions take k is free as long as both operands agree: a lane gives four consecutive ones.
-template <typename T>
-struct Frag { using type = bf16x8; };
-template <>
-struct Frag<float> { using type = f32x4; };
-__device__ __forceinline__ f32x4 mfma64(bf16x8 a, bf16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
-__device__ __forceinline__ f32x4 mfma64(f32x4 a, f32x4 b, f32x4 c) {
-#pragma unroll
-  for (int l = 0; l < 4; ++l) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[l], b[l], c, 0, 0, 0);
-  return c;
-}
-
 constexpr int SLOT = 1024;   // bytes of one individual's A_p in a stage: 16 rows of 64 bytes
 
 __device__ const uint4 kZero = {0, 0, 0, 0};
@@ -48,8 +35,6 @@ struct Tiles {
   int tiles_n;
 };
 
-// float32: permutation of the 16-byte pieces of a W row: rows 4 g of the four lane groups of one read fall 16 banks apart
-__device__ __forceinline__ int w32_swizzle(int row) { return ((row >> 2) & 3) << 2; }
 // permutation of the 16-byte pieces of a 64-byte row (x, A_p): eight neighbouring rows of one read fall on eight bank groups
 __device__ __forceinline__ int x_swizzle(int row) { return (row >> 1) & 3; }
 

@@ -1,8 +1,9 @@
-// Weighted sum of low-rank products in bf16 on v_mfma_f32_16x16x32_bf16: G = s sum_k (w_k a_k)^T b_k over k = (individual, rank row).
+// Weighted sum of low-rank products on v_mfma_f32_16x16x32_bf16 and v_mfma_f32_16x16x4_f32: G = s sum_k (w_k a_k)^T b_k over k = (individual, rank row).
 //
-// Both operands have k as their slow axis: tiles of 32 k go from memory to LDS as they lie (16 bytes a lane, 32-byte pieces
-// permuted by the row) and are read transposed (ds_read_b64_tr_b16), so no transposed copy of the factors is made.
-// The weights are float32 and so is the result, so w a must not be rounded to the factors' 8 bits: it is formed in float32
+// Both operands have k as their slow axis: tiles of 32 k (float32: 16) go from memory to LDS as they lie (16 bytes a lane, 32-byte pieces
+// permuted by the row) and are read transposed (bf16: ds_read_b64_tr_b16; float32: four words), so no transposed copy of the
+// factors is made.  Float32 factors are multiplied by their weight as they are read.
+// bf16: the weights are float32 and so is the result, so w a must not be rounded to the factors' 8 bits: it is formed in float32
 // after the fragment is in registers and split into bf16 planes by rounding, hi + mid (+ lo), each multiplied by b with one
 // matrix instruction.  Two planes hold w a to 2^-18 (deviation 1.5e-6 of it at random mantissas), three to 2^-26.  Sums of
 // 16384 terms or more take two: the float32 accumulation of such sums leaves more than that by itself (1.6e-6 of the result at
@@ -17,36 +18,40 @@ using namespace evox::lr;
 
 namespace {
 
-constexpr int BK = 32;
-
 __device__ const uint4 kZero = {0, 0, 0, 0};
 
-// Sums of the individuals' biases, 64 columns of one split of the individuals: eight lanes of eight columns each, the other
+// Sums of the individuals' biases, 64 columns of one split of the individuals: lanes of 16 bytes of columns each, the other
 // threads along the individuals.  These workgroups ride along behind the ones that multiply.
-template <int THREADS>
+template <typename T, int THREADS>
 __device__ __forceinline__ void sum_biases(const Sum& q, int u, char* smem) {
-  constexpr int ROWS = THREADS / 8;
+  constexpr int E16 = 16 / sizeof(T), LANES = 64 / E16, ROWS = THREADS / LANES;
   float(*part)[64] = reinterpret_cast<float(*)[64]>(smem);             // ROWS x 64
   const int tid = threadIdx.x;
-  const int split = u % q.splits, c = (tid & 7) * 8, n = (u / q.splits) * 64 + c;
+  const int split = u % q.splits, c = (tid % LANES) * E16, n = (u / q.splits) * 64 + c;
   const int64_t per = (q.pop + q.splits - 1) / q.splits, end = min(q.pop, (split + 1) * per);
-  const uint16_t* b = reinterpret_cast<const uint16_t*>(q.b) + (int64_t)q.R * q.N + n;
-  float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  const T* b = reinterpret_cast<const T*>(q.b) + (int64_t)q.R * q.N + n;
+  float s[E16];
+#pragma unroll
+  for (int i = 0; i < E16; ++i) s[i] = 0.f;
   if (n < q.N) {
 #pragma unroll 4
-    for (int64_t p = split * per + tid / 8; p < end; p += ROWS) {
+    for (int64_t p = split * per + tid / LANES; p < end; p += ROWS) {
       const uint4 v = *reinterpret_cast<const uint4*>(b + p * q.sb);
       const uint32_t x[4] = {v.x, v.y, v.z, v.w};
       const float w = q.w[p];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        s[2 * i] = fmaf(w, __uint_as_float(x[i] << 16), s[2 * i]);
-        s[2 * i + 1] = fmaf(w, __uint_as_float(x[i] & 0xffff0000u), s[2 * i + 1]);
+        if constexpr (sizeof(T) == 2) {
+          s[2 * i] = fmaf(w, __uint_as_float(x[i] << 16), s[2 * i]);
+          s[2 * i + 1] = fmaf(w, __uint_as_float(x[i] & 0xffff0000u), s[2 * i + 1]);
+        } else {
+          s[i] = fmaf(w, __uint_as_float(x[i]), s[i]);
+        }
       }
     }
   }
 #pragma unroll
-  for (int i = 0; i < 8; ++i) part[tid / 8][c + i] = s[i];
+  for (int i = 0; i < E16; ++i) part[tid / LANES][c + i] = s[i];
   __syncthreads();
   const int col = (u / q.splits) * 64 + tid;
   if (tid < 64 && col < q.N) {
@@ -86,14 +91,16 @@ __device__ __forceinline__ void split_planes(const bf16x8 f, const float (&w)[8]
   for (int p = 0; p < PLANES; ++p) out[p] = __builtin_bit_cast(bf16x8, make_uint4(o[p][0], o[p][1], o[p][2], o[p][3]));
 }
 
-template <int BM, int BN, int WM, int WN, int STAGES, int PLANES>
+template <typename T, int BM, int BN, int WM, int WN, int STAGES, int PLANES>
 __global__ __launch_bounds__(WM* WN * 64) void sum_mfma_kernel(Sum q, int tiles, int tiles_n) {
   constexpr int NW = WM * WN;
   constexpr int TM = BM / WM / 16, TN = BN / WN / 16;
-  constexpr int A_BYTES = BK * BM * 2, B_BYTES = BK * BN * 2, STAGE = A_BYTES + B_BYTES + NW * 256;
+  constexpr bool BF = sizeof(T) == 2;
+  constexpr int BK = 64 / sizeof(T), ROW = BM * (int)sizeof(T);        // k of a step, bytes of a row of a tile
+  constexpr int A_BYTES = BM * 64, B_BYTES = BN * 64, STAGE = A_BYTES + B_BYTES + NW * 256;
   constexpr int AI = A_BYTES / 1024 / NW, BI = B_BYTES / 1024 / NW, LOADS = AI + BI + 1;
   static_assert(BM == BN, "the rows of a load are those of both operands");
-  static_assert(TM == 4 && TN % 4 == 0, "fragments are read four at a time");
+  static_assert(!BF || (TM == 4 && TN % 4 == 0), "fragments are read four at a time");
   static_assert(STAGES >= 3 && STAGES <= 4 && LOADS * (STAGES - 2) <= 63 && STAGES * STAGE <= 160 * 1024, "counted waits and LDS");
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int lane = threadIdx.x & 63;
@@ -102,7 +109,7 @@ __global__ __launch_bounds__(WM* WN * 64) void sum_mfma_kernel(Sum q, int tiles,
   // tiles of one split lie together: they read the same factors
   const int products = tiles * q.splits;
   if ((int)blockIdx.x >= products) {
-    sum_biases<NW * 64>(q, (int)blockIdx.x - products, smem);
+    sum_biases<T, NW * 64>(q, (int)blockIdx.x - products, smem);
     return;
   }
   const int u = xcd_remap((int)blockIdx.x, products);
@@ -113,32 +120,31 @@ __global__ __launch_bounds__(WM* WN * 64) void sum_mfma_kernel(Sum q, int tiles,
 
   // This lane's rows.  The factors of an individual lie apart from the next one's: a row's address moves on by a fixed amount per
   // step and by what lies between two individuals whenever its rank row wraps.
-  constexpr int RPI = 1024 / (BM * 2);
-  static_assert(RPI >= 1 && AI == BI, "");
-  const uint16_t* A = reinterpret_cast<const uint16_t*>(q.a);
-  const uint16_t* B = reinterpret_cast<const uint16_t*>(q.b);
+  static_assert(1024 % ROW == 0 && AI == BI && (BF || PLANES == 1), "whole rows per wave-instruction");
+  const T* A = reinterpret_cast<const T*>(q.a);
+  const T* B = reinterpret_cast<const T*>(q.b);
   const int pstep = BK / q.R, jstep = BK % q.R;
-  const int64_t da = (pstep * q.sa + (int64_t)jstep * q.M) * 2, wrap_a = (q.sa - (int64_t)q.R * q.M) * 2;
-  const int64_t db = (pstep * q.sb + (int64_t)jstep * q.N) * 2, wrap_b = (q.sb - (int64_t)q.R * q.N) * 2;
+  const int64_t da = (pstep * q.sa + (int64_t)jstep * q.M) * sizeof(T), wrap_a = (q.sa - (int64_t)q.R * q.M) * sizeof(T);
+  const int64_t db = (pstep * q.sb + (int64_t)jstep * q.N) * sizeof(T), wrap_b = (q.sb - (int64_t)q.R * q.N) * sizeof(T);
   const int left = (int)min(ke - kb, (int64_t)0x7fffffff);            // k of this split
   const char *pa[AI], *pb[AI];
   int kr[AI], jr[AI];
 #pragma unroll
   for (int j = 0; j < AI; ++j) {
     const int byte = (j * NW + wave) * 1024 + lane * 16;
-    const int row = byte / (BM * 2), c16 = byte % (BM * 2) / 16;
-    const int col = ((c16 >> 1) ^ tr_swizzle<BM>(row)) * 16 + (c16 & 1) * 8;
+    const int row = byte / ROW, c16 = byte % ROW / 16;
+    const int col = BF ? ((c16 >> 1) ^ tr_swizzle<BM>(row)) * 16 + (c16 & 1) * 8 : (c16 ^ w32_swizzle(row)) * 4;
     const int64_t p = (kb + row) / q.R;
     kr[j] = row;
     jr[j] = (int)(kb + row - p * q.R);
     pa[j] = reinterpret_cast<const char*>(A + p * q.sa + (int64_t)jr[j] * q.M + (m0 + col < q.M ? m0 + col : 0));
     pb[j] = reinterpret_cast<const char*>(B + p * q.sb + (int64_t)jr[j] * q.N + (n0 + col < q.N ? n0 + col : 0));
   }
-  // and its weight: k of lane & 31 (both halves of the wavefront bring the same)
-  int kw = lane & 31, jw = (int)((kb + kw) % q.R);
+  // and its weight: k of lane mod 32 (16) (all parts of the wavefront bring the same)
+  int kw = lane & (BK - 1), jw = (int)((kb + kw) % q.R);
   const float* pw = q.w + (kb + kw) / q.R;
   const char* const zero = reinterpret_cast<const char*>(&kZero);
-  // the loads of the next step in order: every call moves the rows on by 32
+  // the loads of the next step in order: every call moves the rows on by BK
   auto stage = [&](int buf) {
     char* s = smem + buf * STAGE;
 #pragma unroll
@@ -179,36 +185,55 @@ __global__ __launch_bounds__(WM* WN * 64) void sum_mfma_kernel(Sum q, int tiles,
 #pragma unroll
     for (int b = 0; b < TN; ++b) acc[a][b] = f32x4{0.f, 0.f, 0.f, 0.f};
   uint32_t ao[TM], bo[TN];
-  {
+  if constexpr (BF) {
     const int row = (lane >> 4) * 8 + ((lane & 15) >> 2);
-    const uint32_t base = (uint32_t)(uintptr_t)(lds_vp)smem + (lane & 3) * 8;
+    const uint32_t base = (uint32_t)(uintptr_t)(lds_vp)smem + row * ROW + (lane & 3) * 8;
 #pragma unroll
-    for (int a = 0; a < TM; ++a) ao[a] = base + row * (BM * 2) + (((wm * TM + a) ^ tr_swizzle<BM>(row)) << 5);
+    for (int a = 0; a < TM; ++a) ao[a] = base + (((wm * TM + a) ^ tr_swizzle<BM>(row)) << 5);
 #pragma unroll
-    for (int b = 0; b < TN; ++b) bo[b] = base + A_BYTES + row * (BN * 2) + (((wn * TN + b) ^ tr_swizzle<BN>(row)) << 5);
+    for (int b = 0; b < TN; ++b) bo[b] = base + A_BYTES + (((wn * TN + b) ^ tr_swizzle<BN>(row)) << 5);
+  } else {
+    const int row = (lane >> 4) * 4, base = row * ROW + (lane & 3) * 4, piece = (lane & 15) >> 2;
+#pragma unroll
+    for (int a = 0; a < TM; ++a) ao[a] = base + ((((wm * TM + a) * 4 + piece) ^ w32_swizzle(row)) << 4);
+#pragma unroll
+    for (int b = 0; b < TN; ++b) bo[b] = base + A_BYTES + ((((wn * TN + b) * 4 + piece) ^ w32_swizzle(row)) << 4);
   }
-  bf16x8 fa[TM][PLANES], fb[TN];
+  using F = typename Frag<T>::type;
+  F fa[TM][PLANES], fb[TN];
   auto read = [&](int buf) {
     const uint32_t off = buf * STAGE;
-    const float* ws = reinterpret_cast<const float*>(smem + off + A_BYTES + B_BYTES + wave * 256) + (lane >> 4) * 8;
-    const f32x4 w0 = *reinterpret_cast<const f32x4*>(ws), w1 = *reinterpret_cast<const f32x4*>(ws + 4);
-    const float w[8] = {w0[0], w0[1], w0[2], w0[3], w1[0], w1[1], w1[2], w1[3]};
-    bf16x8 raw[4];
-    uint32_t at[4];
+    const float* ws = reinterpret_cast<const float*>(smem + off + A_BYTES + B_BYTES + wave * 256);
+    if constexpr (BF) {
+      const f32x4 w0 = *reinterpret_cast<const f32x4*>(ws + (lane >> 4) * 8), w1 = *reinterpret_cast<const f32x4*>(ws + (lane >> 4) * 8 + 4);
+      const float w[8] = {w0[0], w0[1], w0[2], w0[3], w1[0], w1[1], w1[2], w1[3]};
+      bf16x8 raw[4];
+      uint32_t at[4];
 #pragma unroll
-    for (int a = 0; a < 4; ++a) at[a] = ao[a] + off;
-    read_tr4<4 * BM * 2>(at, raw);
+      for (int a = 0; a < 4; ++a) at[a] = ao[a] + off;
+      read_tr4<4 * ROW>(at, raw);
 #pragma unroll
-    for (int c = 0; c < TN / 4; ++c) {
-      bf16x8 part[4];
+      for (int c = 0; c < TN / 4; ++c) {
+        bf16x8 part[4];
 #pragma unroll
-      for (int b = 0; b < 4; ++b) at[b] = bo[c * 4 + b] + off;
-      read_tr4<4 * BN * 2>(at, part);
+        for (int b = 0; b < 4; ++b) at[b] = bo[c * 4 + b] + off;
+        read_tr4<4 * ROW>(at, part);
 #pragma unroll
-      for (int b = 0; b < 4; ++b) fb[c * 4 + b] = part[b];
+        for (int b = 0; b < 4; ++b) fb[c * 4 + b] = part[b];
+      }
+#pragma unroll
+      for (int a = 0; a < TM; ++a) split_planes<PLANES>(raw[a], w, fa[a]);
+    } else {
+      const f32x4 w = *reinterpret_cast<const f32x4*>(ws + (lane >> 4) * 4);
+#pragma unroll
+      for (int a = 0; a < TM; ++a)
+#pragma unroll
+        for (int l = 0; l < 4; ++l) fa[a][0][l] = w[l] * *reinterpret_cast<const float*>(smem + off + ao[a] + l * ROW);
+#pragma unroll
+      for (int b = 0; b < TN; ++b)
+#pragma unroll
+        for (int l = 0; l < 4; ++l) fb[b][l] = *reinterpret_cast<const float*>(smem + off + bo[b] + l * ROW);
     }
-#pragma unroll
-    for (int a = 0; a < TM; ++a) split_planes<PLANES>(raw[a], w, fa[a]);
   };
   auto multiply = [&]() {
 #pragma unroll
@@ -216,7 +241,7 @@ __global__ __launch_bounds__(WM* WN * 64) void sum_mfma_kernel(Sum q, int tiles,
 #pragma unroll
       for (int a = 0; a < TM; ++a)
 #pragma unroll
-        for (int b = 0; b < TN; ++b) acc[a][b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb[b], fa[a][p], acc[a][b], 0, 0, 0);
+        for (int b = 0; b < TN; ++b) acc[a][b] = mfma64(fb[b], fa[a][p], acc[a][b]);
   };
 
   auto wait_behind = [&](int later) {                                 // at most the loads of the `later` youngest steps outstanding
@@ -272,45 +297,48 @@ __global__ __launch_bounds__(WM* WN * 64) void sum_mfma_kernel(Sum q, int tiles,
     }
 }
 
-template <int BM, int WM, int WN, int STAGES, int PLANES>
+template <typename T, int BM, int WM, int WN, int STAGES, int PLANES>
 int launch(const Sum& q, hipStream_t s) {
-  constexpr int LDS = STAGES * (2 * BK * BM * 2 + WM * WN * 256);
+  constexpr int LDS = STAGES * (2 * BM * 64 + WM * WN * 256);
   const int tiles_n = (q.N + BM - 1) / BM;
   const int64_t tiles = (int64_t)((q.M + BM - 1) / BM) * tiles_n;
   const int64_t wgs = (tiles + (q.gb != nullptr ? (q.N + 63) / 64 : 0)) * q.splits;
   if (wgs > 0x7fffffff) return (int)hipErrorInvalidValue;
-  auto* k = &sum_mfma_kernel<BM, BM, WM, WN, STAGES, PLANES>;
+  auto* k = &sum_mfma_kernel<T, BM, BM, WM, WN, STAGES, PLANES>;
   static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
   if (attr != hipSuccess) return (int)attr;
   k<<<(unsigned)wgs, WM * WN * 64, LDS, s>>>(q, (int)tiles, tiles_n);
   return last_launch_status();
 }
 
-bool big_tiles(int M, int N) { return (int64_t)((M + 255) / 256) * ((N + 255) / 256) >= 12; }
+// Tiles of 256 x 256 for bf16 where there are at least 12 of them (1024 x 720: 73 us against 76 with 128 x 128); float32 products
+// last sixteen times as long as the reads that feed them and gain nothing from them.
+bool big_tiles(const Sum& q, int elem) { return elem == 2 && (int64_t)((q.M + 255) / 256) * ((q.N + 255) / 256) >= 12; }
 
 }  // namespace
 
 namespace evox {
 namespace lr {
 
-// Tiles of 256 x 256 where there are at least 32 of them (2048 x 2048: 64), else of 128 x 128, two workgroups a compute unit.
-// K is split so that the chip is filled once; a split has at least four steps.
-void sum_mfma_plan(Sum& q) {
-  const bool big = big_tiles(q.M, q.N);
+// K is split so that the chip is filled once (256 x 256: one workgroup a compute unit, else two); a split has 128 k at least.
+void sum_mfma_plan(Sum& q, int elem) {
+  const bool big = big_tiles(q, elem);
+  const int bk = 64 / elem;
   const int64_t side = big ? 256 : 128, tiles = ((q.M + side - 1) / side) * ((q.N + side - 1) / side);
   int64_t s = (big ? kNumCU : 2 * kNumCU) / tiles;
   const int64_t most = (q.K + 127) / 128;
   if (s > most) s = most;
   if (s < 1) s = 1;
   const int64_t per = (q.K + s - 1) / s;
-  q.k_per_split = (per + BK - 1) / BK * BK;
+  q.k_per_split = (per + bk - 1) / bk * bk;
   q.splits = (int)((q.K + q.k_per_split - 1) / q.k_per_split);
 }
 
-int sum_mfma(const Sum& q, hipStream_t s) {
+int sum_mfma(const Sum& q, int elem, hipStream_t s) {
+  if (elem == 4) return launch<float, 128, 2, 2, 4, 1>(q, s);
   const bool two = q.K >= 16384;
-  if (big_tiles(q.M, q.N)) return two ? launch<256, 4, 2, 4, 2>(q, s) : launch<256, 4, 2, 4, 3>(q, s);
-  return two ? launch<128, 2, 2, 4, 2>(q, s) : launch<128, 2, 2, 4, 3>(q, s);
+  if (big_tiles(q, elem)) return two ? launch<uint16_t, 256, 4, 2, 4, 2>(q, s) : launch<uint16_t, 256, 4, 2, 4, 3>(q, s);
+  return two ? launch<uint16_t, 128, 2, 2, 4, 2>(q, s) : launch<uint16_t, 128, 2, 2, 4, 3>(q, s);
 }
 
 }  // namespace lr

@@ -1,6 +1,6 @@
 // Tiles in LDS for the bf16 matrix instructions: counted waits, transposed reads, permuted rows.
 #pragma once
-#include "hip_common.h"
+#include "lowrank.h"
 
 namespace evox {
 namespace lr {
@@ -53,6 +53,21 @@ template <int COLS>
 __device__ __forceinline__ int tr_swizzle(int row) {
   return ((row & 3) | (((row >> 3) & 3) << 2)) & (COLS / 16 - 1);
 }
+// A fragment is 16 bytes a lane: 16 rows of 32 bf16, one instruction, or of 16 floats, four.  The order in which the four
+// instructions take k is free as long as both operands agree: a lane gives four consecutive ones.
+template <typename T>
+struct Frag { using type = bf16x8; };
+template <>
+struct Frag<float> { using type = f32x4; };
+__device__ __forceinline__ f32x4 mfma64(bf16x8 a, bf16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f32x4 mfma64(f32x4 a, f32x4 b, f32x4 c) {
+#pragma unroll
+  for (int l = 0; l < 4; ++l) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[l], b[l], c, 0, 0, 0);
+  return c;
+}
+
+// float32: permutation of the 16-byte pieces of a row that is read by words down its columns: rows 4 g of the four lane groups of one read fall 16 banks apart
+__device__ __forceinline__ int w32_swizzle(int row) { return ((row >> 2) & 3) << 2; }
 // a barrier that leaves this wavefront's loads to LDS in flight; no read of LDS moves up across it
 __device__ __forceinline__ void barrier_no_fence() {
   __builtin_amdgcn_s_barrier();

@@ -344,15 +344,40 @@ __global__ __launch_bounds__(NT) void sum_kernel(Sum q, int tiles_n, int tiles) 
     }
 }
 
+// G and g from the partial sums of all splits, in a fixed order.  Few outputs of many splits (352 of 128: 28 us with a thread for each
+// output): LANES threads share an output, each takes every LANES-th split, and their sums are added in order.
+template <int LANES>
 __global__ __launch_bounds__(NT) void sum_join_kernel(Sum q) {
+  constexpr int OUTS = NT / LANES;
+  __shared__ float part[LANES][OUTS];
   const int64_t mn = (int64_t)q.M * q.N, total = mn + (q.gb != nullptr ? q.N : 0), pitch = mn + q.N;
-  for (int64_t i = (int64_t)blockIdx.x * NT + threadIdx.x; i < total; i += (int64_t)gridDim.x * NT) {
+  const int o = threadIdx.x % OUTS, l = threadIdx.x / OUTS;
+  for (int64_t first = (int64_t)blockIdx.x * OUTS; first < total; first += (int64_t)gridDim.x * OUTS) {
+    const int64_t i = first + o;
     float s = 0.f;
-    for (int k = 0; k < q.splits; ++k) s += q.slab[k * pitch + i];
+    if (i < total) {
+#pragma unroll 8
+      for (int k = l; k < q.splits; k += LANES) s += q.slab[k * pitch + i];
+    }
+    if constexpr (LANES > 1) {
+      __syncthreads();
+      part[l][o] = s;
+      __syncthreads();
+      s = 0.f;
+      for (int k = 0; k < LANES; ++k) s += part[k][o];
+    }
     s *= q.scale;
-    if (i < mn) q.g[i] = s;
-    else q.gb[i - mn] = s;
+    if (l == 0 && i < total) {
+      if (i < mn) q.g[i] = s;
+      else q.gb[i - mn] = s;
+    }
   }
+}
+
+void launch_sum_join(const Sum& q, hipStream_t s) {
+  const int64_t total = (int64_t)(q.M + 1) * q.N;
+  if (total < 16 * kNumCU * 64 && q.splits >= 16) sum_join_kernel<16><<<stream_grid(total, NT / 16), NT, 0, s>>>(q);
+  else sum_join_kernel<1><<<stream_grid(total, NT), NT, 0, s>>>(q);
 }
 
 enum class Path { kTile, kMfma, kGrouped, kFew };
@@ -398,7 +423,7 @@ int launch_sum(const Sum& q, hipStream_t s) {
   const int64_t wgs = (tiles + (q.gb != nullptr ? (q.N + 63) / 64 : 0)) * q.splits;
   if (wgs > 0x7fffffff) return (int)hipErrorInvalidValue;
   sum_kernel<T><<<(unsigned)wgs, NT, 0, s>>>(q, tiles_n, (int)tiles);
-  if (q.splits > 1) sum_join_kernel<<<stream_grid((int64_t)(q.M + 1) * q.N, NT), NT, 0, s>>>(q);
+  if (q.splits > 1) launch_sum_join(q, s);
   return last_launch_status();
 }
 
@@ -551,7 +576,7 @@ EVOX_API int evox_hip_lowrank_sum(const float* w, const void* a, const void* b, 
   hipStream_t s = (hipStream_t)stream;
   if (mfma) {
     if (const int st = sum_mfma(q, ints[3] ? 2 : 4, s)) return st;
-    if (q.splits > 1) sum_join_kernel<<<stream_grid((int64_t)(q.M + 1) * q.N, NT), NT, 0, s>>>(q);
+    if (q.splits > 1) launch_sum_join(q, s);
     return last_launch_status();
   }
   return ints[3] ? launch_sum<uint16_t>(q, s) : launch_sum<float>(q, s);

@@ -20,7 +20,7 @@ from typing import List, Sequence
 import torch
 
 from .. import _native
-from ._util import DTYPE_CODE, check, hip, launch_device, on_gpu, stream_of
+from ._util import DTYPE_CODE, check, hip, launch_device, stream_of
 
 ALIGN = 256
 BLOCK = 32
@@ -59,11 +59,12 @@ def adamw_init(params: Sequence[torch.Tensor], state_bits: int = 32) -> dict:
 def _check_leaves(leaves, what):
     if not leaves:
         raise ValueError(f"adamw needs at least one tensor in {what}")
+    device = getattr(leaves[0], "device", None)
     for t in leaves:
         if not isinstance(t, torch.Tensor) or t.dtype not in DTYPE_CODE:
             raise TypeError(f"adamw takes float32 or bfloat16 tensors, got "
                             f"{t.dtype if isinstance(t, torch.Tensor) else type(t).__name__} in {what}")
-        if t.device != leaves[0].device:
+        if t.device != device:
             raise ValueError(f"adamw: the tensors of {what} are on different devices")
 
 
@@ -91,46 +92,61 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], st
     to it (default: to all).  Arithmetic is float32 whatever the types, results have the parameters' types and are contiguous.
     Nothing is written in place, no autograd graph is built.  On a GPU all leaves take one launch per 72 of them."""
     _check_leaves(params, "params")
-    _check_leaves(grads, "grads")
     if len(params) != len(grads):
         raise ValueError(f"adamw: {len(params)} parameters but {len(grads)} gradients")
-    total = 0
-    for p, g in zip(params, grads):
-        if p.shape != g.shape:
-            raise ValueError(f"adamw: a parameter of shape {tuple(p.shape)} has a gradient of shape {tuple(g.shape)}")
-        total += padded(p.numel())
+    if decay is not None and len(decay) != len(params):
+        raise ValueError("adamw: decay needs one entry per parameter")
+    _check_leaves(grads, "grads")
     device = params[0].device
     if grads[0].device != device:
         raise ValueError("adamw: parameters and gradients are on different devices")
-    if decay is not None and len(decay) != len(params):
-        raise ValueError("adamw: decay needs one entry per parameter")
+    total, sizes = 0, []
+    for p, g in zip(params, grads):
+        if p.shape != g.shape:
+            raise ValueError(f"adamw: a parameter of shape {tuple(p.shape)} has a gradient of shape {tuple(g.shape)}")
+        n = p.numel()
+        sizes.append(n)
+        total += -(-n // ALIGN) * ALIGN
     bits = _check_state(state, device, total)
     hyper = (learning_rate, b1, b2, 1 - b1, 1 - b2, eps, weight_decay, math.log(b1) if b1 else -math.inf,
              math.log(b2) if b2 else -math.inf)
-    if not on_gpu(params[0]) or total == 0:
+    if device.type != "cuda" or total == 0:
         return adamw_step_reference(params, grads, state, hyper, bits, decay, updates)
-    return _step_hip(params, grads, state, hyper, bits, decay, updates, total, device)
+    return _step_hip(params, grads, sizes, state, hyper, bits, decay, updates, total, device)
 
 
-def _step_hip(params, grads, state, hyper, bits, decay, updates, total, device):
-    n = len(params)
-    params = [p if p.is_contiguous() else p.contiguous() for p in params]
-    grads = [g if g.is_contiguous() else g.contiguous() for g in grads]
-    out = [torch.empty(p.shape, dtype=p.dtype, device=device) for p in params]
-    new = {k: torch.empty_like(v) for k, v in state.items()}
-    table = (ctypes.c_int64 * (5 * n))(
-        *[p.data_ptr() for p in params], *[g.data_ptr() for g in grads], *[o.data_ptr() for o in out], *[p.numel() for p in params],
-        *[(p.dtype is torch.bfloat16) | (g.dtype is torch.bfloat16) << 1 | (decay is None or bool(decay[k])) << 2
-          for k, (p, g) in enumerate(zip(params, grads))])
+def _step_hip(params, grads, sizes, state, hyper, bits, decay, updates, total, device):
+    n, bf16 = len(params), torch.bfloat16
+    new, out = {}, []
+    ptrs = [0] * (5 * n)
+    kept = []                                       # contiguous copies, alive until the launch
+    for k, (p, g) in enumerate(zip(params, grads)):
+        if not p.is_contiguous():
+            p = p.contiguous()
+            kept.append(p)
+        if not g.is_contiguous():
+            g = g.contiguous()
+            kept.append(g)
+        o = torch.empty(p.shape, dtype=p.dtype, device=device)
+        out.append(o)
+        ptrs[k], ptrs[n + k], ptrs[2 * n + k], ptrs[3 * n + k] = p.data_ptr(), g.data_ptr(), o.data_ptr(), sizes[k]
+        ptrs[4 * n + k] = (p.dtype is bf16) | (g.dtype is bf16) << 1 | (decay is None or bool(decay[k])) << 2
+    new["count"] = torch.empty_like(state["count"])
+    new["mu"], new["nu"] = torch.empty((2, total), dtype=state["mu"].dtype, device=device).unbind(0)
+    if bits == 8:
+        new["mu_scale"], new["nu_scale"] = torch.empty((2, total // BLOCK), dtype=torch.uint8, device=device).unbind(0)
+        scales = (state["mu_scale"].data_ptr(), state["nu_scale"].data_ptr())
+        new_scales = (new["mu_scale"].data_ptr(), new["nu_scale"].data_ptr())
+    else:
+        scales = new_scales = (None, None)
+    table = (ctypes.c_int64 * (5 * n))(*ptrs)
     at = ctypes.addressof(table)
     h = (ctypes.c_float * 9)(*hyper)
-    scales = [state["mu_scale"].data_ptr(), state["nu_scale"].data_ptr()] if bits == 8 else [None, None]
-    new_scales = [new["mu_scale"].data_ptr(), new["nu_scale"].data_ptr()] if bits == 8 else [None, None]
     with launch_device(device):
         check(hip().evox_hip_adamw(bits, n, at, at + 8 * n, at + 16 * n, at + 24 * n, at + 32 * n, ctypes.addressof(h), int(updates),
                                    state["count"].data_ptr(), new["count"].data_ptr(), state["mu"].data_ptr(),
                                    state["nu"].data_ptr(), *scales, new["mu"].data_ptr(), new["nu"].data_ptr(), *new_scales,
-                                   total, stream_of(params[0])), "adamw")
+                                   total, stream_of(out[0])), "adamw")
     return out, new
 
 
@@ -145,7 +161,7 @@ def adamw_moments(state: dict):
     if total % ALIGN:
         raise ValueError(f"adamw: moments hold a multiple of {ALIGN} elements, got {total}")
     _check_state(state, device, total)
-    if not on_gpu(state["mu"]):
+    if device.type != "cuda":
         return tuple(decode(state[k], state[k + "_scale"], k == "mu").to(torch.bfloat16) for k in ("mu", "nu"))
     out = torch.empty((2, total), dtype=torch.bfloat16, device=device)
     mu, nu = out.unbind(0)

@@ -77,8 +77,9 @@ struct Linear {
   int64_t sa, sb;           // stride from one individual's A (B) to the next
   int64_t rows, pop, per;
   int K, N, R;
+  int ldw;                  // elements from one row of W to the next
   int own_bias, act, index64;
-  int vec;                  // bit 0: x and A, bit 1: B, bias and y, bit 2: W may be read four elements at a time
+  int vec;                  // bit 0: x and A, bit 1: B, bias and y, bit 2: W may be read four elements at a time, bit 3: x and A sixteen bytes
   float scale;
   int splits, k_per_split;
 
@@ -145,6 +146,83 @@ struct Linear {
       for (int l = 0; l < 4; ++l) if (n + l < N) st(o + l, v[l]);
   }
 };
+
+// t[row, j] = s * <x[row], A_p[j]> for the entries of one workgroup (`threads` threads): a group of G lanes along K shares a row and
+// four of its factors, G the power of two that 16-byte loads of a row keep busy.
+// (four at least: each writes one of the four results)
+__host__ __device__ __forceinline__ int shrink_lanes(const Linear& q, int elem) {
+  const int piece = (q.vec & 8) ? 16 / elem : (q.vec & 1) ? 4 : 1;
+  int g = 64;
+  while (g > 4 && (g >> 1) * piece >= q.K) g >>= 1;
+  return g;
+}
+template <typename T, int V>
+__device__ __forceinline__ void shrink_dot(const T* x, const T* a, int64_t K, int nj, int lane, int lanes, float (&acc)[4]) {
+  // (the loads of up to four factors and two pieces of K are in flight together)
+#pragma unroll 2
+  for (int64_t k = (int64_t)lane * V; k < K; k += (int64_t)lanes * V) {
+    float xv[V];
+    if constexpr (V == 8) {
+      const uint4 u = *reinterpret_cast<const uint4*>(x + k);
+      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+      for (int l = 0; l < 4; ++l) { xv[2 * l] = __uint_as_float(w[l] << 16); xv[2 * l + 1] = __uint_as_float(w[l] & 0xffff0000u); }
+    } else if constexpr (V == 4) {
+      const f32x4 u = ld4(x + k);
+#pragma unroll
+      for (int l = 0; l < 4; ++l) xv[l] = u[l];
+    } else {
+      xv[0] = ld(x + k);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (j < nj) {
+        const T* p = a + j * K + k;
+        if constexpr (V == 8) {
+          const uint4 u = *reinterpret_cast<const uint4*>(p);
+          const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+          for (int l = 0; l < 4; ++l)
+            acc[j] = fmaf(xv[2 * l + 1], __uint_as_float(w[l] & 0xffff0000u), fmaf(xv[2 * l], __uint_as_float(w[l] << 16), acc[j]));
+        } else if constexpr (V == 4) {
+          const f32x4 u = ld4(p);
+#pragma unroll
+          for (int l = 0; l < 4; ++l) acc[j] = fmaf(xv[l], u[l], acc[j]);
+        } else {
+          acc[j] = fmaf(xv[0], ld(p), acc[j]);
+        }
+      }
+  }
+}
+template <typename T>
+__device__ __forceinline__ void shrink_block(const Linear& q, int64_t block, int threads) {
+  const int lanes = shrink_lanes(q, sizeof(T)), chunks = (q.R + 3) / 4;
+  const int64_t item = block * (threads / lanes) + (int)threadIdx.x / lanes;
+  const int lane = (int)threadIdx.x % lanes;
+  const int64_t row = item / chunks;
+  const int j0 = (int)(item - row * chunks) * 4, nj = min(4, q.R - j0);
+  float acc[4] = {0.f, 0.f, 0.f, 0.f};
+  if (row < q.rows) {
+    const int64_t p = q.individual(row);
+    if (p >= 0) {
+      const T* x = q.row_of<T>(row);
+      const T* a = reinterpret_cast<const T*>(q.a) + p * q.sa + (int64_t)j0 * q.K;
+      if (q.vec & 8) shrink_dot<T, 16 / sizeof(T)>(x, a, q.K, nj, lane, lanes, acc);
+      else if (q.vec & 1) shrink_dot<T, 4>(x, a, q.K, nj, lane, lanes, acc);
+      else shrink_dot<T, 1>(x, a, q.K, nj, lane, lanes, acc);
+    }
+  }
+  for (int o = lanes >> 1; o > 0; o >>= 1)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[j] += __shfl_xor(acc[j], o, 64);
+  if (row < q.rows && lane < nj) {
+    const float v = lane == 0 ? acc[0] : lane == 1 ? acc[1] : lane == 2 ? acc[2] : acc[3];
+    q.t[row * q.R + j0 + lane] = q.scale * v;
+  }
+}
+inline int64_t shrink_blocks(const Linear& q, int elem, int threads) {
+  return (q.rows * ((q.R + 3) / 4) * shrink_lanes(q, elem) + threads - 1) / threads;
+}
 
 // One weighted sum.  K = pop * R products; k stands for individual k / R and row k % R of its factors.
 struct Sum {

@@ -23,46 +23,17 @@ namespace {
 constexpr int BM = 64, BN = 64, BK = 16, NT = 256;
 constexpr int PM = BM + 4;                         // LDS pitch: the four rows of a fragment read start 4 banks apart
 
-// t[row, j] = s * <x[row], A_p[j]>: one wavefront per row, its lanes along K, four factors at a time.
 template <typename T>
 __global__ __launch_bounds__(NT) void shrink_kernel(Linear q) {
-  const int lane = threadIdx.x & 63;
-  for (int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); row < q.rows; row += (int64_t)gridDim.x * 4) {
-    const int64_t p = q.individual(row);
-    float* tr = q.t + row * q.R;
-    if (p < 0) {
-      for (int j = lane; j < q.R; j += 64) tr[j] = 0.f;
-      continue;
-    }
-    const T* x = q.row_of<T>(row);
-    const T* a = reinterpret_cast<const T*>(q.a) + p * q.sa;
-    for (int j0 = 0; j0 < q.R; j0 += 4) {
-      const int nj = min(4, q.R - j0);
-      float acc[4] = {0.f, 0.f, 0.f, 0.f};
-      const T* aj = a + (int64_t)j0 * q.K;
-      if (q.vec & 1) {
-        for (int k = lane * 4; k < q.K; k += 256) {
-          const f32x4 xv = ld4(x + k);
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            if (j < nj) {
-              const f32x4 av = ld4(aj + (int64_t)j * q.K + k);
-              for (int l = 0; l < 4; ++l) acc[j] = fmaf(xv[l], av[l], acc[j]);
-            }
-        }
-      } else {
-        for (int k = lane; k < q.K; k += 64) {
-          const float xv = ld(x + k);
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            if (j < nj) acc[j] = fmaf(xv, ld(aj + (int64_t)j * q.K + k), acc[j]);
-        }
-      }
-#pragma unroll
-      for (int j = 0; j < 4; ++j) acc[j] = wave_sum(acc[j]);
-      if (lane == 0)
-        for (int j = 0; j < nj; ++j) tr[j0 + j] = q.scale * acc[j];
-    }
+  shrink_block<T>(q, blockIdx.x, NT);
+}
+
+// Rows of x or W that start or end off 16 bytes, copied to rows that do not: (rows x cols) at any strides to a pitch of `ld`.
+template <typename T>
+__global__ __launch_bounds__(NT) void pack_kernel(Linear q, const T* w, T* out, int64_t rows, int cols, int ld) {
+  for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
+    const T* s = w != nullptr ? w + r * cols : q.row_of<T>(r);
+    for (int c = threadIdx.x; c < ld; c += NT) out[r * ld + c] = c < cols ? s[c] : (T)0;
   }
 }
 
@@ -123,7 +94,7 @@ __global__ __launch_bounds__(NT) void linear_kernel(Linear q, int tiles_n) {
     const int n = n0 + (tid & 15) * 4;
     f32x4 v = {0.f, 0.f, 0.f, 0.f};
     if (k < k_end) {
-      const T* wr = w + k * q.N + n;
+      const T* wr = w + k * q.ldw + n;
       if ((q.vec & 4) && n + 4 <= q.N) v = ld4(wr);
       else
         for (int l = 0; l < 4; ++l) if (n + l < q.N) v[l] = ld(wr + l);
@@ -185,27 +156,7 @@ __global__ __launch_bounds__(FEW_NT) void linear_few_kernel(Linear q, int produc
   __shared__ __attribute__((aligned(16))) float red[PAIR][8][COLS];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   if ((int)blockIdx.x >= products) {
-    const int64_t e = (int64_t)((int)blockIdx.x - products) * 8 + wave;
-    if (e >= q.rows * q.R) return;
-    const int64_t row = e / q.R;
-    const int j = (int)(e - row * q.R);
-    const int64_t p = q.individual(row);
-    float s = 0.f;
-    if (p >= 0) {
-      const T* x = q.row_of<T>(row);
-      const T* a = reinterpret_cast<const T*>(q.a) + p * q.sa + (int64_t)j * q.K;
-      if (q.vec & 1) {
-#pragma unroll 4
-        for (int k = lane * 4; k < q.K; k += 256) {
-          const f32x4 xv = ld4(x + k), av = ld4(a + k);
-          for (int l = 0; l < 4; ++l) s = fmaf(xv[l], av[l], s);
-        }
-      } else {
-        for (int k = lane; k < q.K; k += 64) s = fmaf(ld(x + k), ld(a + k), s);
-      }
-    }
-    s = wave_sum(s);
-    if (lane == 0) q.t[e] = q.scale * s;
+    shrink_block<T>(q, (int)blockIdx.x - products, FEW_NT);
     return;
   }
   const int split = (int)blockIdx.x % q.splits, n0 = ((int)blockIdx.x / q.splits) * COLS, n = n0 + lane * CPL;
@@ -218,12 +169,12 @@ __global__ __launch_bounds__(FEW_NT) void linear_few_kernel(Linear q, int produc
   // this wavefront's 16 rows of W, all in flight before x is there
   constexpr int MINE = FEW_K / 8;
   uint4 w[MINE];
-  const T* wp = reinterpret_cast<const T*>(q.w) + (int64_t)k0 * q.N + n;
+  const T* wp = reinterpret_cast<const T*>(q.w) + (int64_t)k0 * q.ldw + n;
 #pragma unroll
   for (int i = 0; i < MINE; ++i) {
     w[i] = make_uint4(0, 0, 0, 0);
     const int k = i * 8 + wave;
-    if (k < kn && n < q.N) w[i] = *reinterpret_cast<const uint4*>(wp + (int64_t)k * q.N);
+    if (k < kn && n < q.N) w[i] = *reinterpret_cast<const uint4*>(wp + (int64_t)k * q.ldw);
   }
   for (int i = tid; i < TR * FEW_K; i += FEW_NT) {
     const int r = i / FEW_K, k = i % FEW_K;
@@ -382,36 +333,66 @@ void launch_sum_join(const Sum& q, hipStream_t s) {
 
 enum class Path { kTile, kMfma, kGrouped, kFew };
 
+// Where the operands of a call lie in its workspace.
+struct Layout {
+  bool pack_x = false, pack_w = false;
+  int64_t t = 0, slab = 0, x = 0, w = 0, floats = 0;
+};
+
 template <typename T>
-int launch_linear(const Linear& q, Path path, hipStream_t s) {
+int launch_linear(Linear q, Path path, const Layout& at, float* ws, hipStream_t s) {
+  q.t = ws + at.t;
+  q.slab = ws + at.slab;
   auto join = [&]() {
     const int64_t quads = q.rows * ((q.N + 3) / 4);
     // (few outputs: small workgroups, so that they spread over the chip)
     if (quads < 64 * kNumCU) linear_join_kernel<T><<<(unsigned)((quads + 63) / 64), 64, 0, s>>>(q);
     else linear_join_kernel<T><<<stream_grid(quads, NT), NT, 0, s>>>(q);
   };
+  auto shrink = [&]() { shrink_kernel<T><<<(unsigned)shrink_blocks(q, sizeof(T), NT), NT, 0, s>>>(q); };
+  if (shrink_blocks(q, sizeof(T), NT) > 0x7fffffff) return (int)hipErrorInvalidValue;
   if (path == Path::kFew) {
     constexpr int COLS = 64 * 16 / (int)sizeof(T);
     const int products = (q.N + COLS - 1) / COLS * q.splits;
-    const unsigned wgs = (unsigned)(products + (q.rows * q.R + 7) / 8);
+    const unsigned wgs = (unsigned)(products + shrink_blocks(q, sizeof(T), FEW_NT));
     if (q.rows == 1) linear_few_kernel<T, 1><<<wgs, FEW_NT, 0, s>>>(q, products);
-    else if (q.rows <= 4) linear_few_kernel<T, 4><<<wgs, FEW_NT, 0, s>>>(q, products);
-    else if (q.rows <= 8) linear_few_kernel<T, 8><<<wgs, FEW_NT, 0, s>>>(q, products);
-    else linear_few_kernel<T, 16><<<wgs, FEW_NT, 0, s>>>(q, products);
+    else linear_few_kernel<T, 4><<<wgs, FEW_NT, 0, s>>>(q, products);
     join();
     return last_launch_status();
   }
   if (path == Path::kGrouped) return linear_mfma<T>(q, true, s);
-  const int64_t sg = (q.rows + 3) / 4;
-  shrink_kernel<T><<<(unsigned)(sg < 65536 ? sg : 65536), NT, 0, s>>>(q);
   if (path == Path::kMfma) {
+    if (q.splits == 1 && q.rows > 16) shrink();
+    constexpr int E16 = 16 / sizeof(T);
+    auto grid = [](int64_t rows) { return (unsigned)(rows < 65536 ? rows : 65536); };
+    if (at.pack_x) {
+      const int ld = (q.K + E16 - 1) / E16 * E16;
+      T* to = reinterpret_cast<T*>(ws + at.x);
+      pack_kernel<T><<<grid(q.rows), NT, 0, s>>>(q, nullptr, to, q.rows, q.K, ld);
+      if (q.splits == 1 && q.rows > 16) {
+        q.x = to;
+        q.sx0 = ld * q.per;
+        q.sx1 = ld;
+      } else {                                   // (t is computed by the same launch, from rows as they were)
+        return (int)hipErrorInvalidValue;
+      }
+    }
+    if (at.pack_w) {
+      const int ld = (q.N + E16 - 1) / E16 * E16;
+      T* to = reinterpret_cast<T*>(ws + at.w);
+      pack_kernel<T><<<grid(q.K), NT, 0, s>>>(q, reinterpret_cast<const T*>(q.w), to, q.K, q.N, ld);
+      q.w = to;
+      q.ldw = ld;
+    }
     if (const int st = linear_mfma<T>(q, false, s)) return st;
-  } else {
-    const int tiles_n = (q.N + BN - 1) / BN;
-    const int64_t wgs = (q.rows + BM - 1) / BM * tiles_n * q.splits;
-    if (wgs > 0x7fffffff) return (int)hipErrorInvalidValue;
-    linear_kernel<T><<<(unsigned)wgs, NT, 0, s>>>(q, tiles_n);
+    if (q.splits > 1 || q.rows <= 16) join();
+    return last_launch_status();
   }
+  shrink();
+  const int tiles_n = (q.N + BN - 1) / BN;
+  const int64_t wgs = (q.rows + BM - 1) / BM * tiles_n * q.splits;
+  if (wgs > 0x7fffffff) return (int)hipErrorInvalidValue;
+  linear_kernel<T><<<(unsigned)wgs, NT, 0, s>>>(q, tiles_n);
   if (q.splits > 1) join();
   return last_launch_status();
 }
@@ -458,7 +439,7 @@ void plan_sum(Sum& q) {
 
 // Fills in a call and chooses its kernels.
 static int linear_call(const void* x, const void* w, const void* a, const void* b, const float* bias, const void* index, void* y,
-                       const int64_t* dims, const int* ints, float scale, Linear& q, Path& path) {
+                       const int64_t* dims, const int* ints, float scale, Linear& q, Path& path, Layout& at) {
   q = Linear{};
   q.x = x; q.w = w; q.a = a; q.b = b; q.bias = bias; q.y = y;
   q.rows = dims[0]; q.pop = dims[1]; q.per = dims[2];
@@ -474,30 +455,51 @@ static int linear_call(const void* x, const void* w, const void* a, const void* 
   if (q.K % 4 == 0 && q.sx0 % 4 == 0 && q.sx1 % 4 == 0 && q.sa % 4 == 0 && aligned4(x, el) && aligned4(a, el)) q.vec |= 1;
   if (q.N % 4 == 0 && q.sb % 4 == 0 && aligned4(b, el) && aligned4(y, el) && (!bias || aligned4(bias, 4))) q.vec |= 2;
   if (q.N % 4 == 0 && aligned4(w, el)) q.vec |= 4;
+  const int piece = 16 / el;
+  const bool x16 = q.K % piece == 0 && q.sx0 % piece == 0 && q.sx1 % piece == 0 && al(x);
+  const bool w16 = q.N % piece == 0 && al(w);
+  if (x16 && q.sa % piece == 0 && al(a)) q.vec |= 8;
+  q.ldw = q.N;
+  at = Layout{};
   path = Path::kTile;
-  // few rows: bound by W, where W is more than a few tiles
-  if (q.rows <= 16 && q.N * el % 16 == 0 && al(w) && (int64_t)q.K * q.N >= 1 << 16) {
+  const double flops = 2.0 * (double)q.rows * q.K * q.N;
+  if (q.rows <= 4 && w16 && flops >= 1 << 17) {
+    // up to four rows: W goes through registers once
     path = Path::kFew;
     q.splits = (q.K + FEW_K - 1) / FEW_K;
     q.k_per_split = FEW_K;
-    return 0;
+  } else if (q.rows <= 16 && x16 && w16 && (int64_t)q.K * q.N >= 1 << 16) {
+    path = Path::kMfma;
+    linear_mfma_plan(q, el);
+  } else if (q.rows > 16 && q.K * el >= 128) {
+    // the tiles of lowrank_mfma.hip: sixteen-byte pieces everywhere
+    if (x16 && w16 && al(y) && (q.vec & 2) && linear_mfma_grouped(q, el)) {
+      path = Path::kGrouped;
+      q.splits = 1;
+    } else if (x16 && w16) {
+      path = Path::kMfma;
+      linear_mfma_plan(q, el);
+    } else {
+      // ...or copies that have them: worth it where the product takes the kernels of any alignment longer than some 30 us
+      linear_mfma_plan(q, el);
+      if (flops >= 2e9 && (x16 || q.splits == 1)) {
+        path = Path::kMfma;
+        at.pack_x = !x16;
+        at.pack_w = !w16;
+      }
+    }
   }
-  // the tiles of lowrank_mfma.hip: sixteen-byte pieces everywhere, and enough rows to fill a good part of a tile
-  const int piece = 16 / el;
-  if (q.rows >= 48 && q.K * el >= 128 && q.K % piece == 0 && q.N % piece == 0 && q.sx0 % piece == 0 && q.sx1 % piece == 0 && al(x) &&
-      al(w) && al(y) && (q.vec & 2)) {
-    path = linear_mfma_grouped(q, el) ? Path::kGrouped : Path::kMfma;
-    if (path == Path::kMfma) linear_mfma_plan(q, el);
-    else q.splits = 1;
-    return 0;
+  if (path == Path::kTile) plan_linear(q);
+  auto up4 = [](int64_t v) { return (v + 3) / 4 * 4; };
+  if (path != Path::kGrouped) {
+    at.slab = up4(q.rows * q.R);
+    at.floats = at.slab + (q.splits > 1 || path == Path::kFew || (path == Path::kMfma && q.rows <= 16) ? up4((int64_t)q.splits * q.rows * q.N) : 0);
+    at.x = at.floats;
+    if (at.pack_x) at.floats += up4((q.rows * ((q.K + piece - 1) / piece * piece) * el + 3) / 4);
+    at.w = at.floats;
+    if (at.pack_w) at.floats += up4((q.K * (int64_t)((q.N + piece - 1) / piece * piece) * el + 3) / 4);
   }
-  plan_linear(q);
   return 0;
-}
-
-static int64_t linear_workspace(const Linear& q, Path path) {
-  if (path == Path::kGrouped) return 0;
-  return (q.rows * q.R + 3) / 4 * 4 + (q.splits > 1 || path == Path::kFew ? (int64_t)q.splits * q.rows * q.N : 0);
 }
 
 // Floats of workspace that the same call of evox_hip_lowrank_linear takes (negative: the call is refused): t and the partial
@@ -507,8 +509,9 @@ EVOX_API int64_t evox_hip_lowrank_linear_ws(const void* x, const void* w, const 
                                             const void* index, void* y, const int64_t* dims, const int* ints) {
   Linear q;
   Path path;
-  if (linear_call(x, w, a, b, bias, index, y, dims, ints, 1.f, q, path)) return -1;
-  return linear_workspace(q, path);
+  Layout at;
+  if (linear_call(x, w, a, b, bias, index, y, dims, ints, 1.f, q, path, at)) return -1;
+  return at.floats;
 }
 
 EVOX_API int evox_hip_lowrank_linear(const void* x, const void* w, const void* a, const void* b, const float* bias,
@@ -516,11 +519,11 @@ EVOX_API int evox_hip_lowrank_linear(const void* x, const void* w, const void* a
                                      float scale, void* stream) {
   Linear q;
   Path path;
-  if (const int st = linear_call(x, w, a, b, bias, index, y, dims, ints, scale, q, path)) return st;
-  if (ws_floats < linear_workspace(q, path)) return (int)hipErrorInvalidValue;
-  q.t = ws;
-  q.slab = ws + (q.rows * q.R + 3) / 4 * 4;
-  return ints[5] ? launch_linear<uint16_t>(q, path, (hipStream_t)stream) : launch_linear<float>(q, path, (hipStream_t)stream);
+  Layout at;
+  if (const int st = linear_call(x, w, a, b, bias, index, y, dims, ints, scale, q, path, at)) return st;
+  if (ws_floats < at.floats) return (int)hipErrorInvalidValue;
+  return ints[5] ? launch_linear<uint16_t>(q, path, at, ws, (hipStream_t)stream)
+                 : launch_linear<float>(q, path, at, ws, (hipStream_t)stream);
 }
 
 // Whether a sum takes the tiles of lowrank_sum_mfma.hip: pieces of sixteen bytes, sizes that fill a good part of a tile, and

@@ -29,10 +29,14 @@ constexpr int SLOT = 1024;   // bytes of one individual's A_p in a stage: 16 row
 
 __device__ const uint4 kZero = {0, 0, 0, 0};
 
+// LDS of one stage: x (tiles of 16 rows: once for every wavefront), W, A_p of the tile's individuals
+constexpr int stage_bytes(int bm, int bn, int waves, int slots) { return (bm == 16 ? waves : 1) * bm * 64 + bn * 64 + slots * SLOT; }
+
 struct Tiles {
   uint32_t frags;      // GROUPED: 16-row fragments of all individuals
   uint32_t frags_each; // GROUPED: fragments of one individual
   int tiles_n;
+  int products;        // ungrouped: workgroups that multiply
 };
 
 // permutation of the 16-byte pieces of a 64-byte row (x, A_p): eight neighbouring rows of one read fall on eight bank groups
@@ -61,10 +65,12 @@ __device__ __forceinline__ void activate_all(f32x4 (&v)[TN], int act) {
 template <typename T, int BM, int BN, int WM, int WN, int STAGES, int SLOTS>
 __global__ __launch_bounds__(WM* WN * 64) void linear_mfma_kernel(Linear q, Tiles g) {
   constexpr bool GROUPED = SLOTS > 0, BF = sizeof(T) == 2;
+  constexpr bool FEW = BM == 16;                                       // each wavefront brings the 16 rows of x for itself
   constexpr int BK = 64 / sizeof(T), E16 = 16 / sizeof(T);             // k of a step, elements of a 16-byte piece
   constexpr int NW = WM * WN;
   constexpr int TM = BM / WM / 16, TN = BN / WN / 16;
-  constexpr int X_BYTES = BM * 64, W_BYTES = BN * 64, W_ROW = BN * (int)sizeof(T), STAGE = X_BYTES + W_BYTES + SLOTS * SLOT;
+  constexpr int W_BYTES = BN * 64, W_ROW = BN * (int)sizeof(T), STAGE = stage_bytes(BM, BN, NW, SLOTS);
+  constexpr int X_BYTES = STAGE - W_BYTES - SLOTS * SLOT;
   constexpr int XI = X_BYTES / 1024 / NW, WI = W_BYTES / 1024 / NW, AI = SLOTS / NW;   // wave-instructions per stage
   constexpr int LOADS = XI + WI + AI;
   constexpr int TT = (TM + WN - 1) / WN;                              // t fragments of a wavefront
@@ -75,7 +81,13 @@ __global__ __launch_bounds__(WM* WN * 64) void linear_mfma_kernel(Linear q, Tile
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const int wm = wave / WN, wn = wave % WN;
-  const int u = xcd_remap((int)blockIdx.x, (int)gridDim.x);
+  if constexpr (!GROUPED) {
+    if ((int)blockIdx.x >= g.products) {                                // t, where it is wanted only by linear_join_kernel
+      shrink_block<T>(q, (int)blockIdx.x - g.products, NW * 64);
+      return;
+    }
+  }
+  const int u = xcd_remap((int)blockIdx.x, GROUPED ? (int)gridDim.x : g.products);
   const int split = GROUPED ? 0 : u % q.splits, tile = GROUPED ? u : u / q.splits;
   const int tm = tile / g.tiles_n;
   const int n0 = (tile % g.tiles_n) * BN;
@@ -106,7 +118,7 @@ __global__ __launch_bounds__(WM* WN * 64) void linear_mfma_kernel(Linear q, Tile
 #pragma unroll
   for (int j = 0; j < XI; ++j) {
     int64_t p, r;
-    if (!place((j * NW + wave) * 16 + (lane >> 2), p, r)) place(0, p, r);   // (results of such places are not stored)
+    if (!place((FEW ? 0 : (j * NW + wave) * 16) + (lane >> 2), p, r)) place(0, p, r);   // (results of such places are not stored)
     const T* x = reinterpret_cast<const T*>(q.x);
     if constexpr (GROUPED) x += p * q.sx0 + r * q.sx1;
     else x = q.row_of<T>(r);
@@ -117,9 +129,9 @@ __global__ __launch_bounds__(WM* WN * 64) void linear_mfma_kernel(Linear q, Tile
     const int byte = (j * NW + wave) * 1024 + lane * 16;
     const int row = byte / W_ROW, c16 = byte % W_ROW / 16;
     int n = n0 + (BF ? ((c16 >> 1) ^ tr_swizzle<BN>(row)) * 16 + (c16 & 1) * 8 : (c16 ^ w32_swizzle(row)) * 4);
-    if (n >= q.N) n = 0;                                              // columns that are not stored
+    if (n + E16 > q.ldw) n = 0;                                       // columns that are not stored
     wk[j] = row;
-    ws[j] = reinterpret_cast<const char*>(W + (int64_t)row * q.N + n);
+    ws[j] = reinterpret_cast<const char*>(W + (int64_t)row * q.ldw + n);
   }
 #pragma unroll
   for (int j = 0; j < AI; ++j) {
@@ -128,7 +140,7 @@ __global__ __launch_bounds__(WM* WN * 64) void linear_mfma_kernel(Linear q, Tile
     const int row = lane >> 2;
     as[j] = row < q.R && p <= end ? reinterpret_cast<const char*>(reinterpret_cast<const T*>(q.a) + (int64_t)p * q.sa + (int64_t)row * q.K + xk) : nullptr;
   }
-  const int64_t wstep = (int64_t)BK * q.N * sizeof(T);
+  const int64_t wstep = (int64_t)BK * q.ldw * sizeof(T);
   const char* const zero = reinterpret_cast<const char*>(&kZero);
   auto stage_x = [&](int buf, int kt) {
     char* s = smem + buf * STAGE;
@@ -200,7 +212,7 @@ __global__ __launch_bounds__(WM* WN * 64) void linear_mfma_kernel(Linear q, Tile
   auto read = [&](int buf) {
     const char* s = smem + buf * STAGE;
 #pragma unroll
-    for (int a = 0; a < TM; ++a) fx[a] = *reinterpret_cast<const F*>(s + (wm0 + a * 16) * 64 + xo);
+    for (int a = 0; a < TM; ++a) fx[a] = *reinterpret_cast<const F*>(s + (FEW ? wave * 1024 : (wm0 + a * 16) * 64) + xo);
     if constexpr (GROUPED) {
       // (which x fragments t needs depends on the wavefront: they are read again rather than chosen among registers; a branch
       // around the two instructions for each choice cost more, 408 against 377 us for the multiplying alone)
@@ -411,8 +423,14 @@ __global__ __launch_bounds__(WM* WN * 64) void linear_mfma_kernel(Linear q, Tile
         const int64_t row = (int64_t)tm * BM + wm0 + a * 16 + r;
         const f32x4 v = *reinterpret_cast<const f32x4*>(patch + r * PITCH + (lane % LPR) * 4);
         if (row < q.rows && n < q.N) {
-          if (q.splits == 1) q.finish<T>(row, n, v);
-          else *reinterpret_cast<f32x4*>(q.slab + ((int64_t)split * q.rows + row) * q.N + n) = v;
+          if (!FEW && q.splits == 1) {
+            q.finish<T>(row, n, v);
+          } else {
+            float* o = q.slab + ((int64_t)split * q.rows + row) * q.N + n;
+            if ((q.N & 3) == 0) *reinterpret_cast<f32x4*>(o) = v;
+            else
+              for (int l = 0; l < 4; ++l) if (n + l < q.N) o[l] = v[l];
+          }
         }
       }
     }
@@ -421,13 +439,15 @@ __global__ __launch_bounds__(WM* WN * 64) void linear_mfma_kernel(Linear q, Tile
 
 template <typename T, int BM, int BN, int WM, int WN, int STAGES, int SLOTS>
 int launch(const Linear& q, hipStream_t s) {
-  constexpr int LDS = STAGES * ((BM + BN) * 64 + SLOTS * SLOT);
+  constexpr int LDS = STAGES * stage_bytes(BM, BN, WM * WN, SLOTS);
   Tiles g{};
   g.tiles_n = (q.N + BN - 1) / BN;
   g.frags_each = (uint32_t)((q.per + 15) / 16);
   g.frags = SLOTS ? (uint32_t)(q.pop * g.frags_each) : 0;
   const int64_t tiles_m = SLOTS ? ((int64_t)g.frags * 16 + BM - 1) / BM : (q.rows + BM - 1) / BM;
-  const int64_t wgs = tiles_m * g.tiles_n * (SLOTS ? 1 : q.splits);
+  int64_t wgs = tiles_m * g.tiles_n * (SLOTS ? 1 : q.splits);
+  g.products = (int)wgs;
+  if (!SLOTS && (BM == 16 || q.splits > 1)) wgs += shrink_blocks(q, sizeof(T), WM * WN * 64);
   if (wgs > 0x7fffffff) return (int)hipErrorInvalidValue;
   auto* k = &linear_mfma_kernel<T, BM, BN, WM, WN, STAGES, SLOTS>;
   static const hipError_t attr =
@@ -451,15 +471,28 @@ bool linear_mfma_grouped(const Linear& q, int elem) {
 
 static int64_t tiles_of(const Linear& q, int side) { return ((q.rows + side - 1) / side) * ((q.N + side - 1) / side); }
 
-// Ungrouped: the largest tiles that fill the chip, else the smallest with K divided over as many workgroups as make about two for
-// each compute unit (256 k each at least).
+// The largest tiles that fill the chip and are not mostly outside of y.  (float32 products last sixteen times as long as the reads
+// that feed them: nothing is gained by the tiles of 256.)
+static int side_of(const Linear& q, int elem) {
+  if (elem == 2 && q.N > 128 && tiles_of(q, 256) >= kNumCU) return 256;
+  return q.N > 64 && tiles_of(q, 128) >= kNumCU ? 128 : 64;
+}
+
+// Ungrouped: where tiles of 64 do not fill the chip K is divided over as many workgroups as make about two for each compute unit (256
+// k each at least); 16 rows or fewer: tiles of 16 x 128 and four workgroups for each compute unit, to have enough of W in flight.
 void linear_mfma_plan(Linear& q, int elem) {
   const int bk = 64 / elem;
   q.splits = 1;
   q.k_per_split = (q.K + bk - 1) / bk * bk;
-  if (tiles_of(q, 128) >= kNumCU) return;
-  int64_t s = 2 * kNumCU / tiles_of(q, 64);
-  if (s > q.K / 256) s = q.K / 256;
+  int64_t s;
+  if (q.rows <= 16) {
+    s = 2 * kNumCU / ((q.N + 127) / 128);
+    if (s > q.K / 64) s = q.K / 64;
+  } else {
+    if (side_of(q, elem) > 64) return;
+    s = 2 * kNumCU / tiles_of(q, 64);
+    if (s > q.K / 256) s = q.K / 256;
+  }
   if (s <= 1) return;
   q.k_per_split = (int)(((q.K + s - 1) / s + bk - 1) / bk * bk);
   q.splits = (q.K + q.k_per_split - 1) / q.k_per_split;
@@ -467,18 +500,18 @@ void linear_mfma_plan(Linear& q, int elem) {
 
 template <typename T>
 int linear_mfma(const Linear& q, bool grouped, hipStream_t s) {
-  // (float32 products last sixteen times as long as the reads that feed them: nothing is gained by the largest tiles)
-  const bool big = sizeof(T) == 2 && tiles_of(q, 256) >= kNumCU, medium = tiles_of(q, 128) >= kNumCU;
+  const int side = side_of(q, sizeof(T));
   if (grouped) {
     // a tile of 256 rows holds A_p of eight individuals: 16 / each meet in it where they start together, else up to two more
     const int64_t each = (q.per + 15) / 16, meet = 16 % each == 0 ? 16 / each : 16 / each + 2;
     if constexpr (sizeof(T) == 2)
-      if (big && meet <= 8) return launch<T, 256, 256, 2, 4, 4, 8>(q, s);
-    return medium ? launch<T, 128, 128, 2, 2, 3, 8>(q, s) : launch<T, 64, 64, 2, 2, 4, 4>(q, s);
+      if (side == 256 && meet <= 8) return launch<T, 256, 256, 2, 4, 4, 8>(q, s);
+    return side >= 128 ? launch<T, 128, 128, 2, 2, 3, 8>(q, s) : launch<T, 64, 64, 2, 2, 4, 4>(q, s);
   }
+  if (q.rows <= 16) return launch<T, 16, 128, 1, 4, 4, 0>(q, s);
   if constexpr (sizeof(T) == 2)
-    if (big) return launch<T, 256, 256, 2, 4, 4, 0>(q, s);
-  return medium ? launch<T, 128, 128, 2, 2, 3, 0>(q, s) : launch<T, 64, 64, 2, 2, 4, 0>(q, s);
+    if (side == 256) return launch<T, 256, 256, 2, 4, 4, 0>(q, s);
+  return side >= 128 ? launch<T, 128, 128, 2, 2, 3, 0>(q, s) : launch<T, 64, 64, 2, 2, 4, 0>(q, s);
 }
 template int linear_mfma<uint16_t>(const Linear&, bool, hipStream_t);
 template int linear_mfma<float>(const Linear&, bool, hipStream_t);

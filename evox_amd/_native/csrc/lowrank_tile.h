@@ -10,9 +10,10 @@ using s16x8 = __attribute__((ext_vector_type(8))) short;
 typedef __attribute__((address_space(3))) void* lds_vp;
 typedef const __attribute__((address_space(1))) void* glb_vp;
 
+// at most N loads to LDS outstanding, and every read of LDS returned (its buffer may be refilled behind the next barrier)
 template <int N>
 __device__ __forceinline__ void wait_vmcnt() {
-  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory");
 }
 
 // Transposed reads of two adjacent 4-row blocks each for four columns blocks, waited for in place: the compiler would let no

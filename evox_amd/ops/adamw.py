@@ -59,12 +59,11 @@ def adamw_init(params: Sequence[torch.Tensor], state_bits: int = 32) -> dict:
 def _check_leaves(leaves, what):
     if not leaves:
         raise ValueError(f"adamw needs at least one tensor in {what}")
-    device = getattr(leaves[0], "device", None)
     for t in leaves:
         if not isinstance(t, torch.Tensor) or t.dtype not in DTYPE_CODE:
             raise TypeError(f"adamw takes float32 or bfloat16 tensors, got "
                             f"{t.dtype if isinstance(t, torch.Tensor) else type(t).__name__} in {what}")
-        if t.device != device:
+        if t.get_device() != leaves[0].get_device():
             raise ValueError(f"adamw: the tensors of {what} are on different devices")
 
 
@@ -127,14 +126,14 @@ def _step_hip(params, grads, sizes, state, hyper, bits, decay, updates, total, d
         if not g.is_contiguous():
             g = g.contiguous()
             kept.append(g)
-        o = torch.empty(p.shape, dtype=p.dtype, device=device)
+        o = torch.empty_like(p)                     # (two microseconds less than naming shape, type and device)
         out.append(o)
         ptrs[k], ptrs[n + k], ptrs[2 * n + k], ptrs[3 * n + k] = p.data_ptr(), g.data_ptr(), o.data_ptr(), sizes[k]
         ptrs[4 * n + k] = (p.dtype is bf16) | (g.dtype is bf16) << 1 | (decay is None or bool(decay[k])) << 2
     new["count"] = torch.empty_like(state["count"])
-    new["mu"], new["nu"] = torch.empty((2, total), dtype=state["mu"].dtype, device=device).unbind(0)
+    new["mu"], new["nu"] = torch.empty_like(state["mu"]), torch.empty_like(state["nu"])
     if bits == 8:
-        new["mu_scale"], new["nu_scale"] = torch.empty((2, total // BLOCK), dtype=torch.uint8, device=device).unbind(0)
+        new["mu_scale"], new["nu_scale"] = torch.empty_like(state["mu_scale"]), torch.empty_like(state["nu_scale"])
         scales = (state["mu_scale"].data_ptr(), state["nu_scale"].data_ptr())
         new_scales = (new["mu_scale"].data_ptr(), new["nu_scale"].data_ptr())
     else:
@@ -163,11 +162,10 @@ def adamw_moments(state: dict):
     _check_state(state, device, total)
     if device.type != "cuda":
         return tuple(decode(state[k], state[k + "_scale"], k == "mu").to(torch.bfloat16) for k in ("mu", "nu"))
-    out = torch.empty((2, total), dtype=torch.bfloat16, device=device)
-    mu, nu = out.unbind(0)
+    mu, nu = (torch.empty_like(state[k], dtype=torch.bfloat16) for k in ("mu", "nu"))
     with launch_device(device):
         check(hip().evox_hip_adamw_read(*(state[k].data_ptr() for k in names), mu.data_ptr(), nu.data_ptr(), total,
-                                        stream_of(out)), "adamw_read")
+                                        stream_of(mu)), "adamw_read")
     return mu, nu
 
 

@@ -52,8 +52,10 @@ def _check_factors(what, a, b):
 
 
 def _no_grad_wanted(what, *tensors):
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise ValueError(f"{what} builds no autograd graph: detach its inputs, or call it under torch.no_grad()")
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise ValueError(f"{what} builds no autograd graph: detach its inputs, or call it under torch.no_grad()")
 
 
 def _packed(t):
@@ -107,7 +109,7 @@ def lowrank_linear(x: torch.Tensor, weight: torch.Tensor, a: torch.Tensor, b: to
         raise ValueError("lowrank_linear: inputs on different devices")
     if not on_gpu(x):
         return lowrank_linear_reference(x, weight, a, b, index, bias, scale, activation)
-    y = torch.empty((*x.shape[:-1], n_out), dtype=x.dtype, device=dev)
+    y = x.new_empty((*x.shape[:-1], n_out))
     if y.numel() == 0:
         return y
     if x.stride(-1) != 1 and n_in > 1:
@@ -125,9 +127,9 @@ def lowrank_linear(x: torch.Tensor, weight: torch.Tensor, a: torch.Tensor, b: to
     call = (x.data_ptr(), weight.data_ptr(), a.data_ptr(), b.data_ptr(), None if bias is None else bias.data_ptr(),
             None if index is None else index.data_ptr(), y.data_ptr(), ctypes.addressof(dims), ctypes.addressof(ints))
     floats = lib.evox_hip_lowrank_linear_ws(*call)
-    ws = torch.empty(max(floats, 0), dtype=torch.float32, device=dev)
+    ws = torch.empty(floats, dtype=torch.float32, device=dev) if floats > 0 else None
     with launch_device(dev):
-        check(lib.evox_hip_lowrank_linear(*call, ws.data_ptr(), floats, float(scale), stream_of(y)), "lowrank_linear")
+        check(lib.evox_hip_lowrank_linear(*call, None if ws is None else ws.data_ptr(), floats, float(scale), stream_of(y)), "lowrank_linear")
     return y
 
 
@@ -176,8 +178,8 @@ def lowrank_weighted_sum(w: torch.Tensor, a: torch.Tensor, b: torch.Tensor, scal
     if not on_gpu(w):
         return lowrank_weighted_sum_reference(w, a, b, scale)
     n_in, n_out = a.shape[2], b.shape[2]
-    g = torch.empty((n_in, n_out), dtype=torch.float32, device=dev)
-    gb = torch.empty(n_out, dtype=torch.float32, device=dev) if own_bias else None
+    g = w.new_empty((n_in, n_out))
+    gb = w.new_empty(n_out) if own_bias else None
     if n_out == 0:
         return g, gb
     if pop == 0:
@@ -189,9 +191,9 @@ def lowrank_weighted_sum(w: torch.Tensor, a: torch.Tensor, b: torch.Tensor, scal
     call = (w.data_ptr(), a.data_ptr(), b.data_ptr(), g.data_ptr(), None if gb is None else gb.data_ptr(), ctypes.addressof(dims),
             ctypes.addressof(ints))
     floats = lib.evox_hip_lowrank_sum_ws(*call)
-    ws = torch.empty(max(floats, 0), dtype=torch.float32, device=dev)
+    ws = w.new_empty(floats) if floats > 0 else None
     with launch_device(dev):
-        check(lib.evox_hip_lowrank_sum(*call, ws.data_ptr(), floats, float(scale), stream_of(g)), "lowrank_weighted_sum")
+        check(lib.evox_hip_lowrank_sum(*call, None if ws is None else ws.data_ptr(), floats, float(scale), stream_of(g)), "lowrank_weighted_sum")
     return g, gb
 
 

@@ -71,6 +71,8 @@ LINEAR = [  # individuals, rows each, in, out, rank
     (1, 1, 1, 1, 1), (3, 1, 5, 7, 2), (2, 2, 4, 4, 3), (4, 3, 17, 33, 5), (1, 65, 63, 64, 1), (2, 70, 64, 65, 4), (5, 130, 100, 12, 16),
     (300, 1, 244, 90, 4), (64, 1, 32, 32, 1), (8, 16, 128, 256, 8), (1, 3, 3001, 40, 3), (2, 4, 2048, 512, 7), (3, 100, 256, 264, 16),
     (70, 33, 72, 136, 2), (1, 300, 520, 392, 33), (16, 48, 1024, 128, 17), (1, 1, 4096, 1000, 16), (1000, 1, 11, 3, 1),
+    (1400, 1, 1001, 1003, 3), (4100, 1, 244, 1024, 2), (70, 20, 1024, 1010, 20), (13, 1, 512, 264, 5), (5, 3, 1096, 136, 2),
+    (20, 1, 768, 1032, 4), (600, 1, 64, 520, 3), (9000, 1, 40, 260, 1),
 ]
 
 

@@ -148,7 +148,8 @@ struct Linear {
 };
 
 // t[row, j] = s * <x[row], A_p[j]> for the entries of one workgroup (`threads` threads): a group of G lanes along K shares a row and
-// four of its factors, G the power of two that 16-byte loads of a row keep busy.
+// four of its factors (one, where there are so few entries that the chip is not full otherwise), G the power of two that 16-byte
+// loads of a row keep busy.
 // (four at least: each writes one of the four results)
 __host__ __device__ __forceinline__ int shrink_lanes(const Linear& q, int elem) {
   const int piece = (q.vec & 8) ? 16 / elem : (q.vec & 1) ? 4 : 1;
@@ -156,10 +157,10 @@ __host__ __device__ __forceinline__ int shrink_lanes(const Linear& q, int elem) 
   while (g > 4 && (g >> 1) * piece >= q.K) g >>= 1;
   return g;
 }
-template <typename T, int V>
-__device__ __forceinline__ void shrink_dot(const T* x, const T* a, int64_t K, int nj, int lane, int lanes, float (&acc)[4]) {
-  // (the loads of up to four factors and two pieces of K are in flight together)
-#pragma unroll 2
+template <typename T, int V, int JC>
+__device__ __forceinline__ void shrink_dot(const T* x, const T* a, int64_t K, int nj, int lane, int lanes, float (&acc)[JC]) {
+  // (eight to ten loads in flight)
+#pragma unroll(JC == 1 ? 4 : 2)
   for (int64_t k = (int64_t)lane * V; k < K; k += (int64_t)lanes * V) {
     float xv[V];
     if constexpr (V == 8) {
@@ -175,8 +176,8 @@ __device__ __forceinline__ void shrink_dot(const T* x, const T* a, int64_t K, in
       xv[0] = ld(x + k);
     }
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (j < nj) {
+    for (int j = 0; j < JC; ++j)
+      if (JC == 1 || j < nj) {
         const T* p = a + j * K + k;
         if constexpr (V == 8) {
           const uint4 u = *reinterpret_cast<const uint4*>(p);
@@ -194,34 +195,44 @@ __device__ __forceinline__ void shrink_dot(const T* x, const T* a, int64_t K, in
       }
   }
 }
-template <typename T>
-__device__ __forceinline__ void shrink_block(const Linear& q, int64_t block, int threads) {
-  const int lanes = shrink_lanes(q, sizeof(T)), chunks = (q.R + 3) / 4;
+__host__ __device__ __forceinline__ int shrink_factors(const Linear& q) { return q.rows * q.R <= 8 * kNumCU ? 1 : 4; }
+
+template <typename T, int JC>
+__device__ __forceinline__ void shrink_items(const Linear& q, int64_t block, int threads) {
+  const int lanes = shrink_lanes(q, sizeof(T)), chunks = (q.R + JC - 1) / JC;
   const int64_t item = block * (threads / lanes) + (int)threadIdx.x / lanes;
   const int lane = (int)threadIdx.x % lanes;
   const int64_t row = item / chunks;
-  const int j0 = (int)(item - row * chunks) * 4, nj = min(4, q.R - j0);
-  float acc[4] = {0.f, 0.f, 0.f, 0.f};
+  const int j0 = (int)(item - row * chunks) * JC, nj = min(JC, q.R - j0);
+  float acc[JC];
+#pragma unroll
+  for (int j = 0; j < JC; ++j) acc[j] = 0.f;
   if (row < q.rows) {
     const int64_t p = q.individual(row);
     if (p >= 0) {
       const T* x = q.row_of<T>(row);
       const T* a = reinterpret_cast<const T*>(q.a) + p * q.sa + (int64_t)j0 * q.K;
-      if (q.vec & 8) shrink_dot<T, 16 / sizeof(T)>(x, a, q.K, nj, lane, lanes, acc);
-      else if (q.vec & 1) shrink_dot<T, 4>(x, a, q.K, nj, lane, lanes, acc);
-      else shrink_dot<T, 1>(x, a, q.K, nj, lane, lanes, acc);
+      if (q.vec & 8) shrink_dot<T, 16 / sizeof(T), JC>(x, a, q.K, nj, lane, lanes, acc);
+      else if (q.vec & 1) shrink_dot<T, 4, JC>(x, a, q.K, nj, lane, lanes, acc);
+      else shrink_dot<T, 1, JC>(x, a, q.K, nj, lane, lanes, acc);
     }
   }
   for (int o = lanes >> 1; o > 0; o >>= 1)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) acc[j] += __shfl_xor(acc[j], o, 64);
-  if (row < q.rows && lane < nj) {
-    const float v = lane == 0 ? acc[0] : lane == 1 ? acc[1] : lane == 2 ? acc[2] : acc[3];
-    q.t[row * q.R + j0 + lane] = q.scale * v;
-  }
+    for (int j = 0; j < JC; ++j) acc[j] += __shfl_xor(acc[j], o, 64);
+  float v = acc[0];
+#pragma unroll
+  for (int j = 1; j < JC; ++j) if (lane == j) v = acc[j];
+  if (row < q.rows && lane < nj) q.t[row * q.R + j0 + lane] = q.scale * v;
+}
+template <typename T>
+__device__ __forceinline__ void shrink_block(const Linear& q, int64_t block, int threads) {
+  if (shrink_factors(q) == 1) shrink_items<T, 1>(q, block, threads);
+  else shrink_items<T, 4>(q, block, threads);
 }
 inline int64_t shrink_blocks(const Linear& q, int elem, int threads) {
-  return (q.rows * ((q.R + 3) / 4) * shrink_lanes(q, elem) + threads - 1) / threads;
+  const int jc = shrink_factors(q);
+  return (q.rows * ((q.R + jc - 1) / jc) * shrink_lanes(q, elem) + threads - 1) / threads;
 }
 
 // One weighted sum.  K = pop * R products; k stands for individual k / R and row k % R of its factors.

@@ -145,21 +145,22 @@ __global__ __launch_bounds__(NT) void linear_join_kernel(Linear q) {
 
 // Few rows (requests, single tokens): W is read once and that is what the call takes.  A lane owns 16 bytes of a row of W (CPL
 // columns) for all TR rows of x, a workgroup of eight wavefronts FEW_K rows of W (each wavefront every eighth), whose partial
-// sums meet in LDS and then, over the workgroups that share the columns, in linear_join_kernel.  Workgroups behind the ones that
-// multiply compute t, one wavefront for each of its entries, so that it costs no launch of its own.
+// sums meet in LDS and then, over the workgroups that share the columns, in linear_join_kernel.  Workgroups in front of the ones
+// that multiply compute t, so that it costs no launch of its own.
 constexpr int FEW_K = 128, FEW_NT = 512;
 
 template <typename T, int TR>
-__global__ __launch_bounds__(FEW_NT) void linear_few_kernel(Linear q, int products) {
+__global__ __launch_bounds__(FEW_NT) void linear_few_kernel(Linear q, int shrink) {
   constexpr int CPL = 16 / sizeof(T), COLS = 64 * CPL, PAIR = TR > 1 ? 2 : 1;
   __shared__ float xs[FEW_K][TR];
   __shared__ __attribute__((aligned(16))) float red[PAIR][8][COLS];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  if ((int)blockIdx.x >= products) {
-    shrink_block<T>(q, (int)blockIdx.x - products, FEW_NT);
+  if ((int)blockIdx.x < shrink) {
+    shrink_block<T>(q, blockIdx.x, FEW_NT);
     return;
   }
-  const int split = (int)blockIdx.x % q.splits, n0 = ((int)blockIdx.x / q.splits) * COLS, n = n0 + lane * CPL;
+  const int u = (int)blockIdx.x - shrink;
+  const int split = u % q.splits, n0 = (u / q.splits) * COLS, n = n0 + lane * CPL;
   const int k0 = split * FEW_K, kn = min(FEW_K, q.K - k0);
   float acc[TR][CPL];
 #pragma unroll
@@ -353,10 +354,10 @@ int launch_linear(Linear q, Path path, const Layout& at, float* ws, hipStream_t 
   if (shrink_blocks(q, sizeof(T), NT) > 0x7fffffff) return (int)hipErrorInvalidValue;
   if (path == Path::kFew) {
     constexpr int COLS = 64 * 16 / (int)sizeof(T);
-    const int products = (q.N + COLS - 1) / COLS * q.splits;
-    const unsigned wgs = (unsigned)(products + shrink_blocks(q, sizeof(T), FEW_NT));
-    if (q.rows == 1) linear_few_kernel<T, 1><<<wgs, FEW_NT, 0, s>>>(q, products);
-    else linear_few_kernel<T, 4><<<wgs, FEW_NT, 0, s>>>(q, products);
+    const int first = (int)shrink_blocks(q, sizeof(T), FEW_NT);
+    const unsigned wgs = (unsigned)(first + (q.N + COLS - 1) / COLS * q.splits);
+    if (q.rows == 1) linear_few_kernel<T, 1><<<wgs, FEW_NT, 0, s>>>(q, first);
+    else linear_few_kernel<T, 4><<<wgs, FEW_NT, 0, s>>>(q, first);
     join();
     return last_launch_status();
   }

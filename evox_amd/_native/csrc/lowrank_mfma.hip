@@ -36,7 +36,7 @@ struct Tiles {
   uint32_t frags;      // GROUPED: 16-row fragments of all individuals
   uint32_t frags_each; // GROUPED: fragments of one individual
   int tiles_n;
-  int products;        // ungrouped: workgroups that multiply
+  int shrink;          // ungrouped: workgroups that compute t (a multiple of the number of XCDs)
 };
 
 // permutation of the 16-byte pieces of a 64-byte row (x, A_p): eight neighbouring rows of one read fall on eight bank groups
@@ -82,12 +82,13 @@ __global__ __launch_bounds__(WM* WN * 64) void linear_mfma_kernel(Linear q, Tile
   const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const int wm = wave / WN, wn = wave % WN;
   if constexpr (!GROUPED) {
-    if ((int)blockIdx.x >= g.products) {                                // t, where it is wanted only by linear_join_kernel
-      shrink_block<T>(q, (int)blockIdx.x - g.products, NW * 64);
+    // t, where it is wanted only by linear_join_kernel; in front, so that none of it is left when the products are done
+    if ((int)blockIdx.x < g.shrink) {
+      shrink_block<T>(q, (int)blockIdx.x, NW * 64);
       return;
     }
   }
-  const int u = xcd_remap((int)blockIdx.x, GROUPED ? (int)gridDim.x : g.products);
+  const int u = GROUPED ? xcd_remap((int)blockIdx.x, (int)gridDim.x) : xcd_remap((int)blockIdx.x - g.shrink, (int)gridDim.x - g.shrink);
   const int split = GROUPED ? 0 : u % q.splits, tile = GROUPED ? u : u / q.splits;
   const int tm = tile / g.tiles_n;
   const int n0 = (tile % g.tiles_n) * BN;
@@ -446,9 +447,10 @@ int launch(const Linear& q, hipStream_t s) {
   g.frags = SLOTS ? (uint32_t)(q.pop * g.frags_each) : 0;
   const int64_t tiles_m = SLOTS ? ((int64_t)g.frags * 16 + BM - 1) / BM : (q.rows + BM - 1) / BM;
   int64_t wgs = tiles_m * g.tiles_n * (SLOTS ? 1 : q.splits);
-  g.products = (int)wgs;
-  if (!SLOTS && (BM == 16 || q.splits > 1)) wgs += shrink_blocks(q, sizeof(T), WM * WN * 64);
+  const int64_t shrink = !SLOTS && (BM == 16 || q.splits > 1) ? (shrink_blocks(q, sizeof(T), WM * WN * 64) + kNumXCD - 1) / kNumXCD * kNumXCD : 0;
+  wgs += shrink;
   if (wgs > 0x7fffffff) return (int)hipErrorInvalidValue;
+  g.shrink = (int)shrink;
   auto* k = &linear_mfma_kernel<T, BM, BN, WM, WN, STAGES, SLOTS>;
   static const hipError_t attr =
       hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, LDS);

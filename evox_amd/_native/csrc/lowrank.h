@@ -82,6 +82,7 @@ struct Linear {
   int vec;                  // bit 0: x and A, bit 1: B, bias and y, bit 2: W may be read four elements at a time, bit 3: x and A sixteen bytes
   float scale;
   int splits, k_per_split;
+  int own_t;                // each workgroup computes t of its rows itself: they are no other workgroup's
 
   // row / per; a division of 64 bits takes a hundred instructions, so rows that fit are divided in 32
   __device__ __forceinline__ int64_t group(int64_t row) const {
@@ -198,16 +199,16 @@ __device__ __forceinline__ void shrink_dot(const T* x, const T* a, int64_t K, in
 __host__ __device__ __forceinline__ int shrink_factors(const Linear& q) { return q.rows * q.R <= 8 * kNumCU ? 1 : 4; }
 
 template <typename T, int JC>
-__device__ __forceinline__ void shrink_items(const Linear& q, int64_t block, int threads) {
+__device__ __forceinline__ void shrink_items(const Linear& q, int64_t first, int64_t end, int threads) {
   const int lanes = shrink_lanes(q, sizeof(T)), chunks = (q.R + JC - 1) / JC;
-  const int64_t item = block * (threads / lanes) + (int)threadIdx.x / lanes;
+  const int64_t item = first + (int)threadIdx.x / lanes;
   const int lane = (int)threadIdx.x % lanes;
   const int64_t row = item / chunks;
   const int j0 = (int)(item - row * chunks) * JC, nj = min(JC, q.R - j0);
   float acc[JC];
 #pragma unroll
   for (int j = 0; j < JC; ++j) acc[j] = 0.f;
-  if (row < q.rows) {
+  if (item < end) {
     const int64_t p = q.individual(row);
     if (p >= 0) {
       const T* x = q.row_of<T>(row);
@@ -223,12 +224,20 @@ __device__ __forceinline__ void shrink_items(const Linear& q, int64_t block, int
   float v = acc[0];
 #pragma unroll
   for (int j = 1; j < JC; ++j) if (lane == j) v = acc[j];
-  if (row < q.rows && lane < nj) q.t[row * q.R + j0 + lane] = q.scale * v;
+  if (item < end && lane < nj) q.t[row * q.R + j0 + lane] = q.scale * v;
+}
+// the entries of rows [row0, row0 + n), by one workgroup
+template <typename T>
+__device__ __forceinline__ void shrink_rows(const Linear& q, int64_t row0, int n, int threads) {
+  const int lanes = shrink_lanes(q, sizeof(T)), chunks = (q.R + 3) / 4, per = threads / lanes;
+  const int64_t first = row0 * chunks, end = min(row0 + n, q.rows) * chunks;
+  for (int64_t i = first; i < end; i += per) shrink_items<T, 4>(q, i, end, threads);
 }
 template <typename T>
 __device__ __forceinline__ void shrink_block(const Linear& q, int64_t block, int threads) {
-  if (shrink_factors(q) == 1) shrink_items<T, 1>(q, block, threads);
-  else shrink_items<T, 4>(q, block, threads);
+  const int64_t first = block * (threads / shrink_lanes(q, sizeof(T)));
+  if (shrink_factors(q) == 1) shrink_items<T, 1>(q, first, q.rows * q.R, threads);
+  else shrink_items<T, 4>(q, first, q.rows * ((q.R + 3) / 4), threads);
 }
 inline int64_t shrink_blocks(const Linear& q, int elem, int threads) {
   const int jc = shrink_factors(q);

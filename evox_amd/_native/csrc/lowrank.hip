@@ -11,6 +11,7 @@ namespace evox {
 namespace lr {
 bool linear_mfma_grouped(const Linear& q, int elem);             // lowrank_mfma.hip
 void linear_mfma_plan(Linear& q, int elem);
+int linear_mfma_side(const Linear& q, int elem);
 template <typename T>
 int linear_mfma(const Linear& q, bool grouped, hipStream_t s);
 void sum_mfma_plan(Sum& q, int elem);                            // lowrank_sum_mfma.hip
@@ -101,6 +102,7 @@ __global__ __launch_bounds__(NT) void linear_kernel(Linear q, int tiles_n) {
     }
     *reinterpret_cast<f32x4*>(&s[tid >> 4][(tid & 15) * 4]) = v;
   };
+  if (q.own_t) shrink_rows<T>(q, m0, BM, NT);                         // (read behind the barriers that follow)
   f32x4 acc[2][2];
   const int64_t kb = (int64_t)split * q.k_per_split;
   tile_product(kb, min((int64_t)q.K, kb + q.k_per_split), stage_x, stage_w, acc);
@@ -363,7 +365,7 @@ int launch_linear(Linear q, Path path, const Layout& at, float* ws, hipStream_t 
   }
   if (path == Path::kGrouped) return linear_mfma<T>(q, true, s);
   if (path == Path::kMfma) {
-    if (q.splits == 1 && q.rows > 16) shrink();
+    if (q.splits == 1 && q.rows > 16 && !q.own_t) shrink();
     constexpr int E16 = 16 / sizeof(T);
     auto grid = [](int64_t rows) { return (unsigned)(rows < 65536 ? rows : 65536); };
     if (at.pack_x) {
@@ -389,7 +391,7 @@ int launch_linear(Linear q, Path path, const Layout& at, float* ws, hipStream_t 
     if (q.splits > 1 || q.rows <= 16) join();
     return last_launch_status();
   }
-  shrink();
+  if (!q.own_t) shrink();
   const int tiles_n = (q.N + BN - 1) / BN;
   const int64_t wgs = (q.rows + BM - 1) / BM * tiles_n * q.splits;
   if (wgs > 0x7fffffff) return (int)hipErrorInvalidValue;
@@ -491,6 +493,8 @@ static int linear_call(const void* x, const void* w, const void* a, const void* 
     }
   }
   if (path == Path::kTile) plan_linear(q);
+  // one column of tiles of 64: no launch of its own for t
+  q.own_t = (path == Path::kTile || (path == Path::kMfma && q.rows > 16 && linear_mfma_side(q, el) == 64)) && q.splits == 1 && q.N <= 64;
   auto up4 = [](int64_t v) { return (v + 3) / 4 * 4; };
   if (path != Path::kGrouped) {
     at.slab = up4(q.rows * q.R);

@@ -295,6 +295,9 @@ __global__ __launch_bounds__(WM* WN * 64) void linear_mfma_kernel(Linear q, Tile
 #pragma unroll
     for (int i = 0; i < STAGES - 1; ++i)
       if (i < nk) { stage_x(i, k_first + i); stage_w(i, k_first + i); }
+    if constexpr (BM == 64 && !GROUPED) {
+      if (q.own_t) shrink_rows<T>(q, (int64_t)tm * BM, BM, NW * 64);  // (read behind the barriers that follow)
+    }
     for (int kt = 0; kt < nk; ++kt) {
       static_assert(STAGES <= 4, "the waits of the last steps");
       const int later = nk - 1 - kt;
@@ -475,7 +478,7 @@ static int64_t tiles_of(const Linear& q, int side) { return ((q.rows + side - 1)
 
 // The largest tiles that fill the chip and are not mostly outside of y.  (float32 products last sixteen times as long as the reads
 // that feed them: nothing is gained by the tiles of 256.)
-static int side_of(const Linear& q, int elem) {
+int linear_mfma_side(const Linear& q, int elem) {
   if (elem == 2 && q.N > 128 && tiles_of(q, 256) >= kNumCU) return 256;
   return q.N > 64 && tiles_of(q, 128) >= kNumCU ? 128 : 64;
 }
@@ -491,7 +494,7 @@ void linear_mfma_plan(Linear& q, int elem) {
     s = 2 * kNumCU / ((q.N + 127) / 128);
     if (s > q.K / 64) s = q.K / 64;
   } else {
-    if (side_of(q, elem) > 64) return;
+    if (linear_mfma_side(q, elem) > 64) return;
     s = 2 * kNumCU / tiles_of(q, 64);
     if (s > q.K / 256) s = q.K / 256;
   }
@@ -502,7 +505,7 @@ void linear_mfma_plan(Linear& q, int elem) {
 
 template <typename T>
 int linear_mfma(const Linear& q, bool grouped, hipStream_t s) {
-  const int side = side_of(q, sizeof(T));
+  const int side = linear_mfma_side(q, sizeof(T));
   if (grouped) {
     // a tile of 256 rows holds A_p of eight individuals: 16 / each meet in it where they start together, else up to two more
     const int64_t each = (q.per + 15) / 16, meet = 16 % each == 0 ? 16 / each : 16 / each + 2;

@@ -237,10 +237,7 @@ __global__ __launch_bounds__(WM* WN * 64) void linear_mfma_kernel(Linear q, Tile
     }
   };
   auto multiply = [&]() {
-#pragma unroll
-    for (int a = 0; a < TM; ++a)
-#pragma unroll
-      for (int b = 0; b < TN; ++b) acc[a][b] = mfma64(fw[b], fx[a], acc[a][b]);
+    mfma64_all(fw, fx, acc);
     if constexpr (GROUPED) {
 #pragma unroll
       for (int i = 0; i < TT; ++i) tacc[i] = mfma64(fa[i], ft[i], tacc[i]);
@@ -258,17 +255,11 @@ __global__ __launch_bounds__(WM* WN * 64) void linear_mfma_kernel(Linear q, Tile
     // them: the late group at the end of its reading half, the early one at the end of its multiplying half, which is the same
     // moment.  The buffer of step kt - 1 is refilled from the early group's reading half of step kt on; the late group has read
     // it in the half before.
-    auto wait_behind = [&](int later) {                               // at most the loads of the `later` youngest steps outstanding
-      static_assert(STAGES == 4, "the waits of the last steps");
-      if (later >= 2) wait_vmcnt<2 * LOADS>();
-      else if (later == 1) wait_vmcnt<LOADS>();
-      else wait_vmcnt<0>();
-    };
     const bool late = wave >= 4;
 #pragma unroll
     for (int i = 0; i < STAGES - 1; ++i)
       if (i < nk) { stage_x(i, k_first + i); stage_w(i, k_first + i); }
-    wait_behind(nk - 1);
+    wait_steps<LOADS, STAGES - 2>(nk - 1);
     barrier_no_fence();
     if (late) barrier_no_fence();
     for (int kt = 0; kt < nk; ++kt) {
@@ -278,12 +269,12 @@ __global__ __launch_bounds__(WM* WN * 64) void linear_mfma_kernel(Linear q, Tile
         stage_w((buf + 3) & 3, k_first + kt + 3);
       }
       const int later = min(nk - 1, kt + 3) - (kt + 1);
-      if (late) wait_behind(later);
+      if (late) wait_steps<LOADS, STAGES - 2>(later);
       barrier_no_fence();
       __builtin_amdgcn_s_setprio(1);
       multiply();
       __builtin_amdgcn_s_setprio(0);
-      if (!late) wait_behind(later);
+      if (!late) wait_steps<LOADS, STAGES - 2>(later);
       barrier_no_fence();
       buf = (buf + 1) & 3;
     }
@@ -299,11 +290,7 @@ __global__ __launch_bounds__(WM* WN * 64) void linear_mfma_kernel(Linear q, Tile
       if (q.own_t) shrink_rows<T>(q, (int64_t)tm * BM, BM, NW * 64);  // (read behind the barriers that follow)
     }
     for (int kt = 0; kt < nk; ++kt) {
-      static_assert(STAGES <= 4, "the waits of the last steps");
-      const int later = nk - 1 - kt;
-      if (later >= STAGES - 2) wait_vmcnt<LOADS * (STAGES - 2)>();
-      else if (later == 1) wait_vmcnt<LOADS>();
-      else wait_vmcnt<0>();
+      wait_steps<LOADS, STAGES - 2>(nk - 1 - kt);
       barrier_no_fence();
       if (kt + STAGES - 1 < nk) {
         const int b = buf == 0 ? STAGES - 1 : buf - 1;

@@ -101,7 +101,7 @@ __global__ __launch_bounds__(WM* WN * 64) void sum_mfma_kernel(Sum q, int tiles,
   constexpr int AI = A_BYTES / 1024 / NW, BI = B_BYTES / 1024 / NW, LOADS = AI + BI + 1;
   static_assert(BM == BN, "the rows of a load are those of both operands");
   static_assert(!BF || (TM == 4 && TN % 4 == 0), "fragments are read four at a time");
-  static_assert(STAGES >= 3 && STAGES <= 4 && LOADS * (STAGES - 2) <= 63 && STAGES * STAGE <= 160 * 1024, "counted waits and LDS");
+  static_assert(STAGES >= 3 && LOADS * (STAGES - 2) <= 63 && STAGES * STAGE <= 160 * 1024, "counted waits and LDS");
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
@@ -200,7 +200,7 @@ __global__ __launch_bounds__(WM* WN * 64) void sum_mfma_kernel(Sum q, int tiles,
     for (int b = 0; b < TN; ++b) bo[b] = base + A_BYTES + ((((wn * TN + b) * 4 + piece) ^ w32_swizzle(row)) << 4);
   }
   using F = typename Frag<T>::type;
-  F fa[TM][PLANES], fb[TN];
+  F fa[PLANES][TM], fb[TN];
   auto read = [&](int buf) {
     const uint32_t off = buf * STAGE;
     const float* ws = reinterpret_cast<const float*>(smem + off + A_BYTES + B_BYTES + wave * 256);
@@ -222,13 +222,18 @@ __global__ __launch_bounds__(WM* WN * 64) void sum_mfma_kernel(Sum q, int tiles,
         for (int b = 0; b < 4; ++b) fb[c * 4 + b] = part[b];
       }
 #pragma unroll
-      for (int a = 0; a < TM; ++a) split_planes<PLANES>(raw[a], w, fa[a]);
+      for (int a = 0; a < TM; ++a) {
+        bf16x8 planes[PLANES];
+        split_planes<PLANES>(raw[a], w, planes);
+#pragma unroll
+        for (int p = 0; p < PLANES; ++p) fa[p][a] = planes[p];
+      }
     } else {
       const f32x4 w = *reinterpret_cast<const f32x4*>(ws + (lane >> 4) * 4);
 #pragma unroll
       for (int a = 0; a < TM; ++a)
 #pragma unroll
-        for (int l = 0; l < 4; ++l) fa[a][0][l] = w[l] * *reinterpret_cast<const float*>(smem + off + ao[a] + l * ROW);
+        for (int l = 0; l < 4; ++l) fa[0][a][l] = w[l] * *reinterpret_cast<const float*>(smem + off + ao[a] + l * ROW);
 #pragma unroll
       for (int b = 0; b < TN; ++b)
 #pragma unroll
@@ -237,18 +242,9 @@ __global__ __launch_bounds__(WM* WN * 64) void sum_mfma_kernel(Sum q, int tiles,
   };
   auto multiply = [&]() {
 #pragma unroll
-    for (int p = PLANES - 1; p >= 0; --p)
-#pragma unroll
-      for (int a = 0; a < TM; ++a)
-#pragma unroll
-        for (int b = 0; b < TN; ++b) acc[a][b] = mfma64(fb[b], fa[a][p], acc[a][b]);
+    for (int p = PLANES - 1; p >= 0; --p) mfma64_all(fb, fa[p], acc);
   };
 
-  auto wait_behind = [&](int later) {                                 // at most the loads of the `later` youngest steps outstanding
-    if (later >= STAGES - 2) wait_vmcnt<LOADS * (STAGES - 2)>();
-    else if (later == 1) wait_vmcnt<LOADS>();
-    else wait_vmcnt<0>();
-  };
 #pragma unroll
   for (int i = 0; i < STAGES - 1; ++i)
     if (i < nk) stage(i);
@@ -258,26 +254,26 @@ __global__ __launch_bounds__(WM* WN * 64) void sum_mfma_kernel(Sum q, int tiles,
   if constexpr (NW == 8) {
     // two wavefronts a SIMD, half a step apart: one multiplies while the other reads and splits (as in lowrank_mfma.hip)
     const bool late = wave >= 4;
-    wait_behind(nk - 1);
+    wait_steps<LOADS, STAGES - 2>(nk - 1);
     barrier_no_fence();
     if (late) barrier_no_fence();
     for (int kt = 0; kt < nk; ++kt) {
       read(buf);
       if (kt + STAGES - 1 < nk) stage(before(buf));
       const int later = min(nk - 1, kt + STAGES - 1) - (kt + 1);
-      if (late) wait_behind(later);
+      if (late) wait_steps<LOADS, STAGES - 2>(later);
       barrier_no_fence();
       __builtin_amdgcn_s_setprio(1);
       multiply();
       __builtin_amdgcn_s_setprio(0);
-      if (!late) wait_behind(later);
+      if (!late) wait_steps<LOADS, STAGES - 2>(later);
       barrier_no_fence();
       buf = next(buf);
     }
     if (!late) barrier_no_fence();
   } else {
     for (int kt = 0; kt < nk; ++kt) {
-      wait_behind(nk - 1 - kt);
+      wait_steps<LOADS, STAGES - 2>(nk - 1 - kt);
       barrier_no_fence();
       if (kt + STAGES - 1 < nk) stage(before(buf));
       read(buf);

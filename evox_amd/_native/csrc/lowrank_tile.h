@@ -16,6 +16,17 @@ __device__ __forceinline__ void wait_vmcnt() {
   asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory");
 }
 
+// at most the loads (LOADS each) of the `later` youngest steps outstanding, MOST of them or fewer
+template <int LOADS, int MOST>
+__device__ __forceinline__ void wait_steps(int later) {
+  if constexpr (MOST == 0) {
+    wait_vmcnt<0>();
+  } else {
+    if (later >= MOST) wait_vmcnt<LOADS * MOST>();
+    else wait_steps<LOADS, MOST - 1>(later);
+  }
+}
+
 // Transposed reads of two adjacent 4-row blocks each for four columns blocks, waited for in place: the compiler would let no
 // such read (through its builtin) pass a load to LDS that is in flight, which is what the stages are for.
 template <int STEP>
@@ -65,6 +76,23 @@ __device__ __forceinline__ f32x4 mfma64(f32x4 a, f32x4 b, f32x4 c) {
 #pragma unroll
   for (int l = 0; l < 4; ++l) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[l], b[l], c, 0, 0, 0);
   return c;
+}
+// acc[a][b] += fragments second[a] x first[b].  (float32: the four instructions of an output lie apart, one would wait for the other)
+template <int TM, int TN>
+__device__ __forceinline__ void mfma64_all(const bf16x8 (&first)[TN], const bf16x8 (&second)[TM], f32x4 (&acc)[TM][TN]) {
+#pragma unroll
+  for (int a = 0; a < TM; ++a)
+#pragma unroll
+    for (int b = 0; b < TN; ++b) acc[a][b] = mfma64(first[b], second[a], acc[a][b]);
+}
+template <int TM, int TN>
+__device__ __forceinline__ void mfma64_all(const f32x4 (&first)[TN], const f32x4 (&second)[TM], f32x4 (&acc)[TM][TN]) {
+#pragma unroll
+  for (int l = 0; l < 4; ++l)
+#pragma unroll
+    for (int a = 0; a < TM; ++a)
+#pragma unroll
+      for (int b = 0; b < TN; ++b) acc[a][b] = __builtin_amdgcn_mfma_f32_16x16x4f32(first[b][l], second[a][l], acc[a][b], 0, 0, 0);
 }
 
 // float32: permutation of the 16-byte pieces of a row that is read by words down its columns: rows 4 g of the four lane groups of one read fall 16 banks apart

@@ -23,16 +23,39 @@ __device__ __forceinline__ float ld(const uint16_t* p) { return bf2f(*p); }
 __device__ __forceinline__ void st(float* p, float v) { *p = v; }
 __device__ __forceinline__ void st(uint16_t* p, float v) { *p = (uint16_t)f2bf(v); }
 
-// four consecutive elements; `vec`: the address is a multiple of four elements
-__device__ __forceinline__ f32x4 ld4(const float* p) { return *reinterpret_cast<const f32x4*>(p); }
+// Several consecutive elements of a tensor in memory: rows may start at any element (odd widths, views), and a load or store of up
+// to sixteen bytes takes any alignment of an element.
+template <typename V, int ALIGN>
+struct __attribute__((packed, aligned(ALIGN))) Loose { V v; };
+__device__ __forceinline__ f32x4 ld4(const float* p) { return reinterpret_cast<const Loose<f32x4, 4>*>(p)->v; }
 __device__ __forceinline__ f32x4 ld4(const uint16_t* p) {
-  const uint2 w = *reinterpret_cast<const uint2*>(p);
+  const uint2 w = reinterpret_cast<const Loose<uint2, 2>*>(p)->v;
   return f32x4{bf2f(w.x & 0xffffu), __uint_as_float(w.x & 0xffff0000u), bf2f(w.y & 0xffffu), __uint_as_float(w.y & 0xffff0000u)};
 }
-__device__ __forceinline__ void st4(float* p, f32x4 v) { *reinterpret_cast<f32x4*>(p) = v; }
-__device__ __forceinline__ void st4(uint16_t* p, f32x4 v) {
-  *reinterpret_cast<uint2*>(p) = make_uint2(f2bf(v[0]) | (f2bf(v[1]) << 16), f2bf(v[2]) | (f2bf(v[3]) << 16));
+__device__ __forceinline__ void st4(float* p, f32x4 v) { reinterpret_cast<Loose<f32x4, 4>*>(p)->v = v; }
+__device__ __forceinline__ uint2 pack4(f32x4 v) { return make_uint2(f2bf(v[0]) | (f2bf(v[1]) << 16), f2bf(v[2]) | (f2bf(v[3]) << 16)); }
+__device__ __forceinline__ void st4(uint16_t* p, f32x4 v) { reinterpret_cast<Loose<uint2, 2>*>(p)->v = pack4(v); }
+template <typename T>
+__device__ __forceinline__ uint4 ld16(const T* p) { return reinterpret_cast<const Loose<uint4, sizeof(T)>*>(p)->v; }
+template <typename T>
+__device__ __forceinline__ void st16(T* p, uint4 v) { reinterpret_cast<Loose<uint4, sizeof(T)>*>(p)->v = v; }
+// four elements of which `left` exist (at least one); the others are zero
+template <typename T>
+__device__ __forceinline__ f32x4 ld4(const T* p, int64_t left) {
+  if (left >= 4) return ld4(p);
+  f32x4 v = {0.f, 0.f, 0.f, 0.f};
+  for (int l = 0; l < 4; ++l) if (l < left) v[l] = ld(p + l);
+  return v;
 }
+template <typename T>
+__device__ __forceinline__ void st4(T* p, f32x4 v, int64_t left) {
+  if (left >= 4) st4(p, v);
+  else
+    for (int l = 0; l < 4; ++l) if (l < left) st(p + l, v[l]);
+}
+// the same in LDS, aligned
+__device__ __forceinline__ void st4_lds(float* p, f32x4 v) { *reinterpret_cast<f32x4*>(p) = v; }
+__device__ __forceinline__ void st4_lds(uint16_t* p, f32x4 v) { *reinterpret_cast<uint2*>(p) = pack4(v); }
 
 __device__ __forceinline__ float activate(float v, int act) {
   switch (act) {
@@ -77,9 +100,8 @@ struct Linear {
   int64_t sa, sb;           // stride from one individual's A (B) to the next
   int64_t rows, pop, per;
   int K, N, R;
-  int ldw;                  // elements from one row of W to the next
+  int ldw, lda;             // elements from one row of W, of an individual's A to the next
   int own_bias, act, index64;
-  int vec;                  // bit 0: x and A, bit 1: B, bias and y, bit 2: W may be read four elements at a time, bit 3: x and A sixteen bytes
   float scale;
   int splits, k_per_split;
   int own_t;                // each workgroup computes t of its rows itself: they are no other workgroup's
@@ -105,46 +127,29 @@ struct Linear {
   template <typename T>
   __device__ __forceinline__ void finish(int64_t row, int n, f32x4 v) const {
     const int64_t p = individual(row);
-    const bool whole = (vec & 2) && n + 4 <= N;
-    if (bias != nullptr) {
-      if (whole) v += *reinterpret_cast<const f32x4*>(bias + n);
-      else
-        for (int l = 0; l < 4; ++l) if (n + l < N) v[l] += bias[n + l];
-    }
+    const int left = N - n;
+    if (bias != nullptr) v += ld4(bias + n, left);
     if (p >= 0) {
       const T* bp = reinterpret_cast<const T*>(b) + p * sb + n;
       const float* tr = t + row * R;
       f32x4 d = {0.f, 0.f, 0.f, 0.f};
-      if (whole) {
-        // four rows of B in flight at a time
-        int j = 0;
+      // four rows of B in flight at a time
+      int j = 0;
+      if (left >= 4)
         for (; j + 4 <= R; j += 4, bp += 4 * (int64_t)N) {
           const f32x4 q0 = ld4(bp), q1 = ld4(bp + N), q2 = ld4(bp + 2 * (int64_t)N), q3 = ld4(bp + 3 * (int64_t)N);
           const float t0 = tr[j], t1 = tr[j + 1], t2 = tr[j + 2], t3 = tr[j + 3];
           for (int l = 0; l < 4; ++l) d[l] = fmaf(t3, q3[l], fmaf(t2, q2[l], fmaf(t1, q1[l], fmaf(t0, q0[l], d[l]))));
         }
-        for (; j < R; ++j, bp += N) {
-          const f32x4 q = ld4(bp);
-          const float tj = tr[j];
-          for (int l = 0; l < 4; ++l) d[l] = fmaf(tj, q[l], d[l]);
-        }
-        if (own_bias) {
-          const f32x4 q = ld4(bp);
-          for (int l = 0; l < 4; ++l) d[l] = fmaf(scale, q[l], d[l]);
-        }
-      } else {
-        for (int j = 0; j < R + own_bias; ++j, bp += N) {
-          const float tj = j < R ? tr[j] : scale;
-          for (int l = 0; l < 4; ++l) if (n + l < N) d[l] = fmaf(tj, ld(bp + l), d[l]);
-        }
+      for (; j < R + own_bias; ++j, bp += N) {
+        const f32x4 q = ld4(bp, left);
+        const float tj = j < R ? tr[j] : scale;
+        for (int l = 0; l < 4; ++l) d[l] = fmaf(tj, q[l], d[l]);
       }
       v += d;
     }
     for (int l = 0; l < 4; ++l) v[l] = activate_as<T>(v[l], act);
-    T* o = reinterpret_cast<T*>(y) + row * N + n;
-    if (whole) st4(o, v);
-    else
-      for (int l = 0; l < 4; ++l) if (n + l < N) st(o + l, v[l]);
+    st4(reinterpret_cast<T*>(y) + row * N + n, v, left);
   }
 };
 
@@ -153,47 +158,45 @@ struct Linear {
 // loads of a row keep busy.
 // (four at least: each writes one of the four results)
 __host__ __device__ __forceinline__ int shrink_lanes(const Linear& q, int elem) {
-  const int piece = (q.vec & 8) ? 16 / elem : (q.vec & 1) ? 4 : 1;
+  const int piece = 16 / elem;
   int g = 64;
   while (g > 4 && (g >> 1) * piece >= q.K) g >>= 1;
   return g;
 }
-template <typename T, int V, int JC>
-__device__ __forceinline__ void shrink_dot(const T* x, const T* a, int64_t K, int nj, int lane, int lanes, float (&acc)[JC]) {
+template <typename T, int JC>
+__device__ __forceinline__ void shrink_dot(const T* x, const T* a, int64_t K, int64_t lda, int nj, int lane, int lanes, float (&acc)[JC]) {
+  constexpr int V = 16 / sizeof(T);
+  const int64_t full = K / V * V;
+  auto widen = [](uint4 u, float (&v)[V]) {
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int l = 0; l < 4; ++l) {
+      if constexpr (V == 8) {
+        v[2 * l] = __uint_as_float(w[l] << 16);
+        v[2 * l + 1] = __uint_as_float(w[l] & 0xffff0000u);
+      } else {
+        v[l] = __uint_as_float(w[l]);
+      }
+    }
+  };
   // (eight to ten loads in flight)
 #pragma unroll(JC == 1 ? 4 : 2)
-  for (int64_t k = (int64_t)lane * V; k < K; k += (int64_t)lanes * V) {
-    float xv[V];
-    if constexpr (V == 8) {
-      const uint4 u = *reinterpret_cast<const uint4*>(x + k);
-      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-      for (int l = 0; l < 4; ++l) { xv[2 * l] = __uint_as_float(w[l] << 16); xv[2 * l + 1] = __uint_as_float(w[l] & 0xffff0000u); }
-    } else if constexpr (V == 4) {
-      const f32x4 u = ld4(x + k);
-#pragma unroll
-      for (int l = 0; l < 4; ++l) xv[l] = u[l];
-    } else {
-      xv[0] = ld(x + k);
-    }
+  for (int64_t k = (int64_t)lane * V; k < full; k += (int64_t)lanes * V) {
+    float xv[V], av[V];
+    widen(ld16(x + k), xv);
 #pragma unroll
     for (int j = 0; j < JC; ++j)
       if (JC == 1 || j < nj) {
-        const T* p = a + j * K + k;
-        if constexpr (V == 8) {
-          const uint4 u = *reinterpret_cast<const uint4*>(p);
-          const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+        widen(ld16(a + j * lda + k), av);
 #pragma unroll
-          for (int l = 0; l < 4; ++l)
-            acc[j] = fmaf(xv[2 * l + 1], __uint_as_float(w[l] & 0xffff0000u), fmaf(xv[2 * l], __uint_as_float(w[l] << 16), acc[j]));
-        } else if constexpr (V == 4) {
-          const f32x4 u = ld4(p);
-#pragma unroll
-          for (int l = 0; l < 4; ++l) acc[j] = fmaf(xv[l], u[l], acc[j]);
-        } else {
-          acc[j] = fmaf(xv[0], ld(p), acc[j]);
-        }
+        for (int l = 0; l < V; ++l) acc[j] = fmaf(xv[l], av[l], acc[j]);
       }
+  }
+  for (int64_t k = full + lane; k < K; k += lanes) {
+    const float xv = ld(x + k);
+#pragma unroll
+    for (int j = 0; j < JC; ++j)
+      if (j < nj) acc[j] = fmaf(xv, ld(a + j * lda + k), acc[j]);
   }
 }
 __host__ __device__ __forceinline__ int shrink_factors(const Linear& q) { return q.rows * q.R <= 8 * kNumCU ? 1 : 4; }
@@ -212,10 +215,8 @@ __device__ __forceinline__ void shrink_items(const Linear& q, int64_t first, int
     const int64_t p = q.individual(row);
     if (p >= 0) {
       const T* x = q.row_of<T>(row);
-      const T* a = reinterpret_cast<const T*>(q.a) + p * q.sa + (int64_t)j0 * q.K;
-      if (q.vec & 8) shrink_dot<T, 16 / sizeof(T), JC>(x, a, q.K, nj, lane, lanes, acc);
-      else if (q.vec & 1) shrink_dot<T, 4, JC>(x, a, q.K, nj, lane, lanes, acc);
-      else shrink_dot<T, 1, JC>(x, a, q.K, nj, lane, lanes, acc);
+      const T* a = reinterpret_cast<const T*>(q.a) + p * q.sa + (int64_t)j0 * q.lda;
+      shrink_dot<T, JC>(x, a, q.K, q.lda, nj, lane, lanes, acc);
     }
   }
   for (int o = lanes >> 1; o > 0; o >>= 1)
@@ -255,7 +256,9 @@ struct Sum {
   int64_t sa, sb;
   int64_t pop, K;
   int M, N, R;
-  int vec;                  // bit 0: A, bit 1: B, bit 2: g may be accessed four elements at a time
+  int lda, ldb;             // elements from one row of an individual's factors to the next
+  const void* c;            // the individuals' biases, at stride sc
+  int64_t sc;
   float scale;
   int splits;
   int64_t k_per_split;

@@ -9,7 +9,7 @@ using namespace evox::lr;
 
 namespace evox {
 namespace lr {
-bool linear_mfma_grouped(const Linear& q, int elem);             // lowrank_mfma.hip
+bool linear_mfma_grouped(const Linear& q);                       // lowrank_mfma.hip
 void linear_mfma_plan(Linear& q, int elem);
 int linear_mfma_side(const Linear& q, int elem);
 template <typename T>
@@ -29,14 +29,48 @@ __global__ __launch_bounds__(NT) void shrink_kernel(Linear q) {
   shrink_block<T>(q, blockIdx.x, NT);
 }
 
-// Rows of x or W that start or end off 16 bytes, copied to rows that do not: (rows x cols) at any strides to a pitch of `ld`.
+// Rows that start or end off 16 bytes, copied to rows of `ld` elements (a multiple of 16 bytes) that do not, with zeros behind their
+// end.  Source row r lies at base + (r / inner) outer_stride + (r % inner) inner_stride.  16 bytes a thread.
+struct Rows {
+  const void* base;
+  int64_t rows, inner, outer_stride, inner_stride;
+  int cols, ld;
+};
 template <typename T>
-__global__ __launch_bounds__(NT) void pack_kernel(Linear q, const T* w, T* out, int64_t rows, int cols, int ld) {
-  for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
-    const T* s = w != nullptr ? w + r * cols : q.row_of<T>(r);
-    for (int c = threadIdx.x; c < ld; c += NT) out[r * ld + c] = c < cols ? s[c] : (T)0;
+__global__ __launch_bounds__(NT) void pack_kernel(Rows q, T* __restrict__ out) {
+  constexpr int V = 16 / sizeof(T);
+  const int pieces = q.ld / V;
+  const int64_t total = q.rows * pieces;
+  for (int64_t i = (int64_t)blockIdx.x * NT + threadIdx.x; i < total; i += (int64_t)gridDim.x * NT) {
+    int64_t r, p;
+    if (total <= 0xffffffffll) {
+      r = (uint32_t)i / (uint32_t)pieces;
+      p = q.inner == 1 ? r : (uint32_t)r / (uint32_t)q.inner;
+    } else {
+      r = i / pieces;
+      p = r / q.inner;
+    }
+    const int c = (int)(i - r * pieces) * V;
+    const T* s = reinterpret_cast<const T*>(q.base) + p * q.outer_stride + (r - p * q.inner) * q.inner_stride + c;
+    uint4 v;
+    if (c + V <= q.cols) {
+      v = ld16(s);
+    } else {
+      T e[V];
+#pragma unroll
+      for (int l = 0; l < V; ++l) e[l] = c + l < q.cols ? s[l] : (T)0;
+      v = *reinterpret_cast<const uint4*>(e);
+    }
+    *reinterpret_cast<uint4*>(out + r * q.ld + c) = v;
   }
 }
+template <typename T>
+void launch_pack(const Rows& q, T* out, hipStream_t s) {
+  const int64_t pieces = q.rows * (q.ld / (16 / (int)sizeof(T)));
+  int64_t g = (pieces + NT - 1) / NT;
+  pack_kernel<T><<<(unsigned)(g < 32 * kNumCU ? (g < 1 ? 1 : g) : 32 * kNumCU), NT, 0, s>>>(q, out);
+}
+int up16(int cols, int elem) { return (cols * elem + 15) / 16 * 16 / elem; }
 
 // acc[a][b][i] = C[wm0 + 16 a + (lane & 15)][wn0 + 16 b + 4 (lane >> 4) + i] of the tile, given its operands' stagers:
 // stage_a(k, m), stage_b(k, n) return element (m0 + m, k) and (k, n0 + n) as floats, zero outside.
@@ -84,9 +118,7 @@ __global__ __launch_bounds__(NT) void linear_kernel(Linear q, int tiles_n) {
     const int64_t k = k0 + (tid & 3) * 4;
     f32x4 v = {0.f, 0.f, 0.f, 0.f};
     if (xrow < q.rows) {
-      if ((q.vec & 1) && k + 4 <= k_end) v = ld4(xr + k);
-      else
-        for (int l = 0; l < 4; ++l) if (k + l < k_end) v[l] = ld(xr + k + l);
+      if (k < k_end) v = ld4(xr + k, k_end - k);
     }
     for (int l = 0; l < 4; ++l) s[(tid & 3) * 4 + l][tid >> 2] = v[l];
   };
@@ -95,10 +127,7 @@ __global__ __launch_bounds__(NT) void linear_kernel(Linear q, int tiles_n) {
     const int n = n0 + (tid & 15) * 4;
     f32x4 v = {0.f, 0.f, 0.f, 0.f};
     if (k < k_end) {
-      const T* wr = w + k * q.ldw + n;
-      if ((q.vec & 4) && n + 4 <= q.N) v = ld4(wr);
-      else
-        for (int l = 0; l < 4; ++l) if (n + l < q.N) v[l] = ld(wr + l);
+      if (n < q.N) v = ld4(w + k * q.ldw + n, q.N - n);
     }
     *reinterpret_cast<f32x4*>(&s[tid >> 4][(tid & 15) * 4]) = v;
   };
@@ -118,7 +147,7 @@ __global__ __launch_bounds__(NT) void linear_kernel(Linear q, int tiles_n) {
         q.finish<T>(row, n, acc[a][b]);
       } else {
         float* o = q.slab + ((int64_t)split * q.rows + row) * q.N + n;
-        for (int l = 0; l < 4; ++l) if (n + l < q.N) o[l] = acc[a][b][l];
+        st4(o, acc[a][b], q.N - n);
       }
     }
 }
@@ -134,12 +163,11 @@ __global__ __launch_bounds__(NT) void linear_join_kernel(Linear q) {
     const int n = (int)(i - row * quads) * 4;
     f32x4 v = {0.f, 0.f, 0.f, 0.f};
     const float* p = q.slab + row * q.N + n;
-    if ((q.N & 3) == 0) {
+    if (n + 4 <= q.N) {
 #pragma unroll 8
-      for (int s = 0; s < q.splits; ++s) v += *reinterpret_cast<const f32x4*>(p + s * pitch);
+      for (int s = 0; s < q.splits; ++s) v += ld4(p + s * pitch);
     } else {
-      for (int s = 0; s < q.splits; ++s)
-        for (int l = 0; l < 4; ++l) if (n + l < q.N) v[l] += p[s * pitch + l];
+      for (int s = 0; s < q.splits; ++s) v += ld4(p + s * pitch, q.N - n);
     }
     q.finish<T>(row, n, v);
   }
@@ -242,7 +270,7 @@ __global__ __launch_bounds__(NT) void sum_kernel(Sum q, int tiles_n, int tiles) 
     float s = 0.f;
     if (n < q.N)
       for (int64_t p = split * per + (tid >> 6); p < end; p += 4)
-        s = fmaf(q.w[p], ld(reinterpret_cast<const T*>(q.b) + p * q.sb + (int64_t)q.R * q.N + n), s);
+        s = fmaf(q.w[p], ld(reinterpret_cast<const T*>(q.c) + p * q.sc + n), s);
     part[tid >> 6][tid & 63] = s;
     __syncthreads();
     if (tid < 64 && n < q.N) {
@@ -262,10 +290,7 @@ __global__ __launch_bounds__(NT) void sum_kernel(Sum q, int tiles_n, int tiles) 
     if (k < k_end) {
       const int64_t p = k / q.R;
       const T* r = reinterpret_cast<const T*>(q.a) + p * q.sa + (k - p * q.R) * q.M + m0 + c;
-      if ((q.vec & 1) && m0 + c + 4 <= q.M) v = ld4(r);
-      else
-        for (int l = 0; l < 4; ++l) if (m0 + c + l < q.M) v[l] = ld(r + l);
-      v *= q.w[p];
+      if (m0 + c < q.M) v = q.w[p] * ld4(r, q.M - m0 - c);
     }
     *reinterpret_cast<f32x4*>(&s[kk][c]) = v;
   };
@@ -275,9 +300,7 @@ __global__ __launch_bounds__(NT) void sum_kernel(Sum q, int tiles_n, int tiles) 
     if (k < k_end) {
       const int64_t p = k / q.R;
       const T* r = reinterpret_cast<const T*>(q.b) + p * q.sb + (k - p * q.R) * q.N + n0 + c;
-      if ((q.vec & 2) && n0 + c + 4 <= q.N) v = ld4(r);
-      else
-        for (int l = 0; l < 4; ++l) if (n0 + c + l < q.N) v[l] = ld(r + l);
+      if (n0 + c < q.N) v = ld4(r, q.N - n0 - c);
     }
     *reinterpret_cast<f32x4*>(&s[kk][c]) = v;
   };
@@ -338,8 +361,8 @@ enum class Path { kTile, kMfma, kGrouped, kFew };
 
 // Where the operands of a call lie in its workspace.
 struct Layout {
-  bool pack_x = false, pack_w = false;
-  int64_t t = 0, slab = 0, x = 0, w = 0, floats = 0;
+  bool pack_x = false, pack_w = false, pack_a = false;
+  int64_t t = 0, slab = 0, x = 0, w = 0, a = 0, floats = 0;
 };
 
 template <typename T>
@@ -363,30 +386,29 @@ int launch_linear(Linear q, Path path, const Layout& at, float* ws, hipStream_t 
     join();
     return last_launch_status();
   }
-  if (path == Path::kGrouped) return linear_mfma<T>(q, true, s);
-  if (path == Path::kMfma) {
-    if (q.splits == 1 && q.rows > 16 && !q.own_t) shrink();
-    constexpr int E16 = 16 / sizeof(T);
-    auto grid = [](int64_t rows) { return (unsigned)(rows < 65536 ? rows : 65536); };
+  if (path == Path::kGrouped || path == Path::kMfma) {
     if (at.pack_x) {
-      const int ld = (q.K + E16 - 1) / E16 * E16;
-      T* to = reinterpret_cast<T*>(ws + at.x);
-      pack_kernel<T><<<grid(q.rows), NT, 0, s>>>(q, nullptr, to, q.rows, q.K, ld);
-      if (q.splits == 1 && q.rows > 16) {
-        q.x = to;
-        q.sx0 = ld * q.per;
-        q.sx1 = ld;
-      } else {                                   // (t is computed by the same launch, from rows as they were)
-        return (int)hipErrorInvalidValue;
-      }
+      const int ld = up16(q.K, sizeof(T));
+      launch_pack<T>(Rows{q.x, q.rows, q.per, q.sx0, q.sx1, q.K, ld}, reinterpret_cast<T*>(ws + at.x), s);
+      q.x = ws + at.x;
+      q.sx0 = ld * q.per;
+      q.sx1 = ld;
     }
     if (at.pack_w) {
-      const int ld = (q.N + E16 - 1) / E16 * E16;
-      T* to = reinterpret_cast<T*>(ws + at.w);
-      pack_kernel<T><<<grid(q.K), NT, 0, s>>>(q, reinterpret_cast<const T*>(q.w), to, q.K, q.N, ld);
-      q.w = to;
+      const int ld = up16(q.N, sizeof(T));
+      launch_pack<T>(Rows{q.w, q.K, 1, q.N, 0, q.N, ld}, reinterpret_cast<T*>(ws + at.w), s);
+      q.w = ws + at.w;
       q.ldw = ld;
     }
+    if (at.pack_a) {
+      const int ld = up16(q.K, sizeof(T));
+      launch_pack<T>(Rows{q.a, q.pop * q.R, q.R, q.sa, q.K, q.K, ld}, reinterpret_cast<T*>(ws + at.a), s);
+      q.a = ws + at.a;
+      q.lda = ld;
+      q.sa = (int64_t)ld * q.R;
+    }
+    if (path == Path::kGrouped) return linear_mfma<T>(q, true, s);
+    if (q.splits == 1 && q.rows > 16 && !q.own_t) shrink();
     if (const int st = linear_mfma<T>(q, false, s)) return st;
     if (q.splits > 1 || q.rows <= 16) join();
     return last_launch_status();
@@ -410,8 +432,6 @@ int launch_sum(const Sum& q, hipStream_t s) {
   if (q.splits > 1) launch_sum_join(q, s);
   return last_launch_status();
 }
-
-bool aligned4(const void* p, int elem) { return (reinterpret_cast<uintptr_t>(p) & (uintptr_t)(4 * elem - 1)) == 0; }
 
 // How many workgroups share one tile's K: enough that about two workgroups per compute unit run, but at least 128 products each.
 int64_t splits_for(int64_t tiles, int64_t K) {
@@ -453,16 +473,13 @@ static int linear_call(const void* x, const void* w, const void* a, const void* 
   q.index64 = ints[6] == 2;
   q.scale = scale;
   if (q.rows <= 0 || q.N <= 0 || q.K <= 0 || q.R <= 0 || q.per <= 0 || dtype < 0 || dtype > 1) return (int)hipErrorInvalidValue;
-  const int el = dtype ? 2 : 4;
+  const int el = dtype ? 2 : 4, piece = 16 / el;
   auto al = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; };
-  if (q.K % 4 == 0 && q.sx0 % 4 == 0 && q.sx1 % 4 == 0 && q.sa % 4 == 0 && aligned4(x, el) && aligned4(a, el)) q.vec |= 1;
-  if (q.N % 4 == 0 && q.sb % 4 == 0 && aligned4(b, el) && aligned4(y, el) && (!bias || aligned4(bias, 4))) q.vec |= 2;
-  if (q.N % 4 == 0 && aligned4(w, el)) q.vec |= 4;
-  const int piece = 16 / el;
   const bool x16 = q.K % piece == 0 && q.sx0 % piece == 0 && q.sx1 % piece == 0 && al(x);
   const bool w16 = q.N % piece == 0 && al(w);
-  if (x16 && q.sa % piece == 0 && al(a)) q.vec |= 8;
+  const bool a16 = q.K % piece == 0 && q.sa % piece == 0 && al(a);
   q.ldw = q.N;
+  q.lda = q.K;
   at = Layout{};
   path = Path::kTile;
   const double flops = 2.0 * (double)q.rows * q.K * q.N;
@@ -475,21 +492,23 @@ static int linear_call(const void* x, const void* w, const void* a, const void* 
     path = Path::kMfma;
     linear_mfma_plan(q, el);
   } else if (q.rows > 16 && q.K * el >= 128) {
-    // the tiles of lowrank_mfma.hip: sixteen-byte pieces everywhere
-    if (x16 && w16 && al(y) && (q.vec & 2) && linear_mfma_grouped(q, el)) {
-      path = Path::kGrouped;
-      q.splits = 1;
-    } else if (x16 && w16) {
-      path = Path::kMfma;
-      linear_mfma_plan(q, el);
-    } else {
-      // ...or copies that have them: worth it where the product takes the kernels of any alignment longer than some 30 us
-      linear_mfma_plan(q, el);
-      if (flops >= 2e9 && (x16 || q.splits == 1)) {
-        path = Path::kMfma;
-        at.pack_x = !x16;
-        at.pack_w = !w16;
-      }
+    // The tiles of lowrank_mfma.hip take rows of whole 16-byte pieces; others are copied first, where that takes less time than is
+    // gained: the tiles of any alignment reach about 60 TFLOP/s (a column of tiles is 64 wide), these about 100 in float32 and
+    // 300 and more in bf16; a copy reads and writes at 4 TB/s and costs a launch.  Grouped tiles also save the pass over x for t.
+    const bool grouped = linear_mfma_grouped(q);
+    const double tiles_us = flops / q.N * ((q.N + 63) / 64 * 64) / 60e6 * (el == 2 ? 0.8 : 0.4) +
+                            (grouped ? (double)q.rows * q.K * el / 4e6 : 0.0);
+    double copy_us = 0.0;
+    if (!x16) copy_us += 4.0 + 2.0 * q.rows * q.K * el / 4e6;
+    if (!w16) copy_us += 4.0 + 2.0 * q.K * q.N * el / 4e6;
+    if (grouped && !a16) copy_us += 4.0 + 2.0 * q.pop * q.R * q.K * el / 4e6;
+    if (copy_us <= tiles_us) {
+      path = grouped ? Path::kGrouped : Path::kMfma;
+      at.pack_x = !x16;
+      at.pack_w = !w16;
+      at.pack_a = grouped && !a16;
+      if (grouped) q.splits = 1;
+      else linear_mfma_plan(q, el);
     }
   }
   if (path == Path::kTile) plan_linear(q);
@@ -499,11 +518,15 @@ static int linear_call(const void* x, const void* w, const void* a, const void* 
   if (path != Path::kGrouped) {
     at.slab = up4(q.rows * q.R);
     at.floats = at.slab + (q.splits > 1 || path == Path::kFew || (path == Path::kMfma && q.rows <= 16) ? up4((int64_t)q.splits * q.rows * q.N) : 0);
-    at.x = at.floats;
-    if (at.pack_x) at.floats += up4((q.rows * ((q.K + piece - 1) / piece * piece) * el + 3) / 4);
-    at.w = at.floats;
-    if (at.pack_w) at.floats += up4((q.K * (int64_t)((q.N + piece - 1) / piece * piece) * el + 3) / 4);
   }
+  auto copy = [&](bool wanted, int64_t rows, int cols) {
+    const int64_t from = at.floats;
+    if (wanted) at.floats += rows * up16(cols, el) * el / 4;
+    return from;
+  };
+  at.x = copy(at.pack_x, q.rows, q.K);
+  at.w = copy(at.pack_w, q.K, q.N);
+  at.a = copy(at.pack_a, q.pop * q.R, q.K);
   return 0;
 }
 
@@ -531,26 +554,19 @@ EVOX_API int evox_hip_lowrank_linear(const void* x, const void* w, const void* a
                  : launch_linear<float>(q, path, at, ws, (hipStream_t)stream);
 }
 
-// Whether a sum takes the tiles of lowrank_sum_mfma.hip: pieces of sixteen bytes, sizes that fill a good part of a tile, and
-// enough terms that a step of 32 is not mostly empty.
-static bool sum_takes_mfma(int64_t pop, int M, int N, int R, int dtype, int64_t sa, int64_t sb, const void* a, const void* b,
-                           const void* g) {
-  auto al = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; };
-  const int piece = dtype ? 8 : 4;
-  return M % piece == 0 && N % piece == 0 && M >= 48 && N >= 48 && pop * R >= 64 && sa % piece == 0 && sb % piece == 0 && al(a) &&
-         al(b) && al(g);
-}
-
-static int64_t sum_workspace(Sum& q, bool mfma, int dtype) {
-  if (mfma) sum_mfma_plan(q, dtype ? 2 : 4);
-  else plan_sum(q);
-  return q.splits > 1 ? (int64_t)q.splits * (q.M + 1) * q.N : 0;
-}
+// What a sum takes: the tiles of lowrank_sum_mfma.hip (rows of whole 16-byte pieces, sizes that fill a good part of a tile, enough
+// terms that a step is not mostly empty), after copying factors whose rows are off 16 bytes where that takes less time than is
+// gained (the tiles of any alignment reach about 30 TFLOP/s; a copy reads and writes at 4 TB/s and costs a launch).
+struct SumLayout {
+  bool mfma = false, pack_a = false, pack_b = false;
+  int64_t a = 0, b = 0, floats = 0;
+};
 
 // dims: pop, sa, sb.  ints: M, N, R, dtype
 static int sum_call(const float* w, const void* a, const void* b, float* g, float* gb, const int64_t* dims, const int* ints, float scale,
-                    Sum& q, bool& mfma) {
+                    Sum& q, SumLayout& at) {
   q = Sum{};
+  at = SumLayout{};
   q.w = w; q.a = a; q.b = b; q.g = g; q.gb = gb;
   q.pop = dims[0]; q.sa = dims[1]; q.sb = dims[2];
   q.M = ints[0]; q.N = ints[1]; q.R = ints[2];
@@ -558,34 +574,66 @@ static int sum_call(const float* w, const void* a, const void* b, float* g, floa
   if (q.M <= 0 || q.N <= 0 || q.R <= 0 || q.pop <= 0 || dtype < 0 || dtype > 1) return (int)hipErrorInvalidValue;
   q.K = q.pop * q.R;
   q.scale = scale;
-  const int el = dtype ? 2 : 4;
-  if (q.M % 4 == 0 && q.sa % 4 == 0 && aligned4(a, el)) q.vec |= 1;
-  if (q.N % 4 == 0 && q.sb % 4 == 0 && aligned4(b, el)) q.vec |= 2;
-  mfma = sum_takes_mfma(q.pop, q.M, q.N, q.R, dtype, q.sa, q.sb, a, b, g);
+  const int el = dtype ? 2 : 4, piece = 16 / el;
+  q.lda = q.M;
+  q.ldb = q.N;
+  q.c = reinterpret_cast<const char*>(b) + (int64_t)q.R * q.N * el;
+  q.sc = q.sb;
+  auto al = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; };
+  const bool a16 = q.M % piece == 0 && q.sa % piece == 0 && al(a), b16 = q.N % piece == 0 && q.sb % piece == 0 && al(b);
+  if (q.M >= 48 && q.N >= 48 && q.K >= 64) {
+    double copy_us = 0.0;
+    if (!a16) copy_us += 4.0 + 2.0 * q.K * q.M * el / 4e6;
+    if (!b16) copy_us += 4.0 + 2.0 * q.K * q.N * el / 4e6;
+    at.mfma = copy_us <= 2.0 * q.K * q.M * q.N / 30e6 * 0.6;
+    at.pack_a = at.mfma && !a16;
+    at.pack_b = at.mfma && !b16;
+  }
+  if (at.mfma) sum_mfma_plan(q, el);
+  else plan_sum(q);
+  at.floats = q.splits > 1 ? ((int64_t)q.splits * (q.M + 1) * q.N + 3) / 4 * 4 : 0;
+  at.a = at.floats;
+  if (at.pack_a) at.floats += q.K * up16(q.M, el) * el / 4;
+  at.b = at.floats;
+  if (at.pack_b) at.floats += q.K * up16(q.N, el) * el / 4;
   return 0;
+}
+
+template <typename T>
+static int launch_sum_call(Sum q, const SumLayout& at, float* ws, hipStream_t s) {
+  q.slab = ws;
+  if (!at.mfma) return launch_sum<T>(q, s);
+  if (at.pack_a) {
+    q.lda = up16(q.M, sizeof(T));
+    launch_pack<T>(Rows{q.a, q.K, q.R, q.sa, q.M, q.M, q.lda}, reinterpret_cast<T*>(ws + at.a), s);
+    q.a = ws + at.a;
+    q.sa = (int64_t)q.lda * q.R;
+  }
+  if (at.pack_b) {
+    q.ldb = up16(q.N, sizeof(T));
+    launch_pack<T>(Rows{q.b, q.K, q.R, q.sb, q.N, q.N, q.ldb}, reinterpret_cast<T*>(ws + at.b), s);
+    q.b = ws + at.b;
+    q.sb = (int64_t)q.ldb * q.R;
+  }
+  if (const int st = sum_mfma(q, sizeof(T), s)) return st;
+  if (q.splits > 1) launch_sum_join(q, s);
+  return last_launch_status();
 }
 
 // Floats of workspace that the same call of evox_hip_lowrank_sum takes (negative: the call is refused).
 EVOX_API int64_t evox_hip_lowrank_sum_ws(const float* w, const void* a, const void* b, float* g, float* gb, const int64_t* dims,
                                          const int* ints) {
   Sum q;
-  bool mfma;
-  if (sum_call(w, a, b, g, gb, dims, ints, 1.f, q, mfma)) return -1;
-  return sum_workspace(q, mfma, ints[3]);
+  SumLayout at;
+  if (sum_call(w, a, b, g, gb, dims, ints, 1.f, q, at)) return -1;
+  return at.floats;
 }
 
 EVOX_API int evox_hip_lowrank_sum(const float* w, const void* a, const void* b, float* g, float* gb, const int64_t* dims,
                                   const int* ints, float* ws, int64_t ws_floats, float scale, void* stream) {
   Sum q;
-  bool mfma;
-  if (const int st = sum_call(w, a, b, g, gb, dims, ints, scale, q, mfma)) return st;
-  if (ws_floats < sum_workspace(q, mfma, ints[3])) return (int)hipErrorInvalidValue;
-  q.slab = ws;
-  hipStream_t s = (hipStream_t)stream;
-  if (mfma) {
-    if (const int st = sum_mfma(q, ints[3] ? 2 : 4, s)) return st;
-    if (q.splits > 1) launch_sum_join(q, s);
-    return last_launch_status();
-  }
-  return ints[3] ? launch_sum<uint16_t>(q, s) : launch_sum<float>(q, s);
+  SumLayout at;
+  if (const int st = sum_call(w, a, b, g, gb, dims, ints, scale, q, at)) return st;
+  if (ws_floats < at.floats) return (int)hipErrorInvalidValue;
+  return ints[3] ? launch_sum_call<uint16_t>(q, at, ws, (hipStream_t)stream) : launch_sum_call<float>(q, at, ws, (hipStream_t)stream);
 }

@@ -139,7 +139,7 @@ __global__ __launch_bounds__(WM* WN * 64) void linear_mfma_kernel(Linear q, Tile
     // (a slot behind the individuals of this tile's last fragment holds zeros)
     const uint32_t p = first + j * NW + wave, end = (min(frag0 + BM / 16, g.frags) - 1) / g.frags_each;
     const int row = lane >> 2;
-    as[j] = row < q.R && p <= end ? reinterpret_cast<const char*>(reinterpret_cast<const T*>(q.a) + (int64_t)p * q.sa + (int64_t)row * q.K + xk) : nullptr;
+    as[j] = row < q.R && p <= end ? reinterpret_cast<const char*>(reinterpret_cast<const T*>(q.a) + (int64_t)p * q.sa + (int64_t)row * q.lda + xk) : nullptr;
   }
   const int64_t wstep = (int64_t)BK * q.ldw * sizeof(T);
   const char* const zero = reinterpret_cast<const char*>(&kZero);
@@ -327,8 +327,8 @@ __global__ __launch_bounds__(WM* WN * 64) void linear_mfma_kernel(Linear q, Tile
             rest[l] = v[l] - bf2f(f2bf(v[l]));
             if (rest[l] != rest[l]) rest[l] = 0.f;                    // (an infinite v leaves no rest)
           }
-          st4(reinterpret_cast<uint16_t*>(o) + g4, v);
-          st4(reinterpret_cast<uint16_t*>(o) + 16 + g4, rest);
+          st4_lds(reinterpret_cast<uint16_t*>(o) + g4, v);
+          st4_lds(reinterpret_cast<uint16_t*>(o) + 16 + g4, rest);
         } else {
           *reinterpret_cast<f32x4*>(reinterpret_cast<float*>(o) + g4) = v;
         }
@@ -366,8 +366,8 @@ __global__ __launch_bounds__(WM* WN * 64) void linear_mfma_kernel(Linear q, Tile
           const int nc = n + g4;
           own[b] = f32x4{0.f, 0.f, 0.f, 0.f};
           if (nc < q.N) {
-            if (q.bias != nullptr) own[b] = *reinterpret_cast<const f32x4*>(q.bias + nc);
-            if (q.own_bias) own[b] += q.scale * ld4(bp + (int64_t)q.R * q.N + nc);
+            if (q.bias != nullptr) own[b] = ld4(q.bias + nc, q.N - nc);
+            if (q.own_bias) own[b] += q.scale * ld4(bp + (int64_t)q.R * q.N + nc, q.N - nc);
           }
         }
       }
@@ -376,7 +376,7 @@ __global__ __launch_bounds__(WM* WN * 64) void linear_mfma_kernel(Linear q, Tile
       for (int b = 0; b < TN; ++b) acc[a][b] = mfma64(fb[b], ft, acc[a][b]) + own[b];
       if constexpr (BF) activate_all(acc[a], q.act);
 #pragma unroll
-      for (int b = 0; b < TN; ++b) st4(patch + j16 * PITCH + b * 16 + g4, acc[a][b]);
+      for (int b = 0; b < TN; ++b) st4_lds(patch + j16 * PITCH + b * 16 + g4, acc[a][b]);
       // whole rows of the wavefront's columns: 16 bytes a lane (float32: activated here, where the code stands once per fragment)
       constexpr int LPR = W16 / E16, RPS = 64 / LPR;
 #pragma unroll(BF ? 16 / RPS : 1)
@@ -391,8 +391,18 @@ __global__ __launch_bounds__(WM* WN * 64) void linear_mfma_kernel(Linear q, Tile
             v = __builtin_bit_cast(uint4, w);
           }
         }
-        if (r0 + r < q.per && n < q.N)
-          *reinterpret_cast<uint4*>(reinterpret_cast<T*>(q.y) + ((int64_t)p * q.per + r0 + r) * q.N + n) = v;
+        if (r0 + r < q.per && n < q.N) {
+          T* y = reinterpret_cast<T*>(q.y) + ((int64_t)p * q.per + r0 + r) * q.N + n;
+          if (n + E16 <= q.N) {
+            st16(y, v);
+          } else {
+            const T* from = patch + r * PITCH + (lane % LPR) * E16;
+            for (int l = 0; n + l < q.N; ++l) {
+              if constexpr (BF) y[l] = from[l];
+              else y[l] = activate(from[l], q.act);
+            }
+          }
+        }
       }
     }
   } else {
@@ -418,9 +428,7 @@ __global__ __launch_bounds__(WM* WN * 64) void linear_mfma_kernel(Linear q, Tile
             q.finish<T>(row, n, v);
           } else {
             float* o = q.slab + ((int64_t)split * q.rows + row) * q.N + n;
-            if ((q.N & 3) == 0) *reinterpret_cast<f32x4*>(o) = v;
-            else
-              for (int l = 0; l < 4; ++l) if (n + l < q.N) o[l] = v[l];
+            st4(o, v, q.N - n);
           }
         }
       }
@@ -454,11 +462,10 @@ int launch(const Linear& q, hipStream_t s) {
 namespace evox {
 namespace lr {
 
-bool linear_mfma_grouped(const Linear& q, int elem) {
+bool linear_mfma_grouped(const Linear& q) {
   // fragments at least 70 % full: the empty rows cost more than the separate pass over x otherwise
   const int64_t each = (q.per + 15) / 16;
-  return q.index == nullptr && q.R <= 16 && q.per >= 16 && 10 * q.per >= 7 * 16 * each && q.pop * each < 0x7fffffff / 16 &&
-         q.sa * elem % 16 == 0 && (reinterpret_cast<uintptr_t>(q.a) & 15) == 0;
+  return q.index == nullptr && q.R <= 16 && q.per >= 16 && 10 * q.per >= 7 * 16 * each && q.pop * each < 0x7fffffff / 16;
 }
 
 static int64_t tiles_of(const Linear& q, int side) { return ((q.rows + side - 1) / side) * ((q.N + side - 1) / side); }

@@ -29,14 +29,18 @@ __device__ __forceinline__ void sum_biases(const Sum& q, int u, char* smem) {
   const int tid = threadIdx.x;
   const int split = u % q.splits, c = (tid % LANES) * E16, n = (u / q.splits) * 64 + c;
   const int64_t per = (q.pop + q.splits - 1) / q.splits, end = min(q.pop, (split + 1) * per);
-  const T* b = reinterpret_cast<const T*>(q.b) + (int64_t)q.R * q.N + n;
+  const T* b = reinterpret_cast<const T*>(q.c) + n;
   float s[E16];
 #pragma unroll
   for (int i = 0; i < E16; ++i) s[i] = 0.f;
-  if (n < q.N) {
+  if (n < q.N && n + E16 > q.N) {
+    for (int64_t p = split * per + tid / LANES; p < end; p += ROWS)
+#pragma unroll
+      for (int i = 0; i < E16; ++i) if (n + i < q.N) s[i] = fmaf(q.w[p], ld(b + p * q.sc + i), s[i]);
+  } else if (n < q.N) {
 #pragma unroll 4
     for (int64_t p = split * per + tid / LANES; p < end; p += ROWS) {
-      const uint4 v = *reinterpret_cast<const uint4*>(b + p * q.sb);
+      const uint4 v = ld16(b + p * q.sc);
       const uint32_t x[4] = {v.x, v.y, v.z, v.w};
       const float w = q.w[p];
 #pragma unroll
@@ -124,8 +128,8 @@ __global__ __launch_bounds__(WM* WN * 64) void sum_mfma_kernel(Sum q, int tiles,
   const T* A = reinterpret_cast<const T*>(q.a);
   const T* B = reinterpret_cast<const T*>(q.b);
   const int pstep = BK / q.R, jstep = BK % q.R;
-  const int64_t da = (pstep * q.sa + (int64_t)jstep * q.M) * sizeof(T), wrap_a = (q.sa - (int64_t)q.R * q.M) * sizeof(T);
-  const int64_t db = (pstep * q.sb + (int64_t)jstep * q.N) * sizeof(T), wrap_b = (q.sb - (int64_t)q.R * q.N) * sizeof(T);
+  const int64_t da = (pstep * q.sa + (int64_t)jstep * q.lda) * sizeof(T), wrap_a = (q.sa - (int64_t)q.R * q.lda) * sizeof(T);
+  const int64_t db = (pstep * q.sb + (int64_t)jstep * q.ldb) * sizeof(T), wrap_b = (q.sb - (int64_t)q.R * q.ldb) * sizeof(T);
   const int left = (int)min(ke - kb, (int64_t)0x7fffffff);            // k of this split
   const char *pa[AI], *pb[AI];
   int kr[AI], jr[AI];
@@ -137,8 +141,8 @@ __global__ __launch_bounds__(WM* WN * 64) void sum_mfma_kernel(Sum q, int tiles,
     const int64_t p = (kb + row) / q.R;
     kr[j] = row;
     jr[j] = (int)(kb + row - p * q.R);
-    pa[j] = reinterpret_cast<const char*>(A + p * q.sa + (int64_t)jr[j] * q.M + (m0 + col < q.M ? m0 + col : 0));
-    pb[j] = reinterpret_cast<const char*>(B + p * q.sb + (int64_t)jr[j] * q.N + (n0 + col < q.N ? n0 + col : 0));
+    pa[j] = reinterpret_cast<const char*>(A + p * q.sa + (int64_t)jr[j] * q.lda + (m0 + col < q.M ? m0 + col : 0));
+    pb[j] = reinterpret_cast<const char*>(B + p * q.sb + (int64_t)jr[j] * q.ldb + (n0 + col < q.N ? n0 + col : 0));
   }
   // and its weight: k of lane mod 32 (16) (all parts of the wavefront bring the same)
   int kw = lane & (BK - 1), jw = (int)((kb + kw) % q.R);
@@ -289,7 +293,7 @@ __global__ __launch_bounds__(WM* WN * 64) void sum_mfma_kernel(Sum q, int tiles,
 #pragma unroll
     for (int b = 0; b < TN; ++b) {
       const int m = m0 + (wm * TM + a) * 16 + (lane & 15), n = n0 + (wn * TN + b) * 16 + (lane >> 4) * 4;
-      if (m < q.M && n < q.N) *reinterpret_cast<f32x4*>(out + (int64_t)m * q.N + n) = f * acc[a][b];
+      if (m < q.M && n < q.N) st4(out + (int64_t)m * q.N + n, f * acc[a][b], q.N - n);
     }
 }
 

@@ -256,7 +256,7 @@ template <int BITS, int VPT>
 int launch(int n_leaves, const int64_t* p, const int64_t* g, const int64_t* out, const int64_t* n, const int64_t* flags,
            const Hyper& h, const float* count_in, float* count_out, const void* mu, const void* nu, const uint8_t* mus,
            const uint8_t* nus, void* mu_out, void* nu_out, uint8_t* mus_out, uint8_t* nus_out, hipStream_t stream) {
-  constexpr int64_t kTile = VPT * 1024;
+  constexpr int64_t kTile = VPT * 1024, kMostTiles = 0xffffffffll / NT;      // (a launch counts its threads in 32 bits)
   int64_t state = 0;
   bool first = true;
   int k = 0;
@@ -267,8 +267,8 @@ int launch(int n_leaves, const int64_t* p, const int64_t* g, const int64_t* out,
     for (; k < n_leaves && c < kLeaves; ++k) {
       if (n[k] <= 0) continue;
       const int64_t mine = (n[k] + kTile - 1) / kTile;
-      if (mine > 0x7fffffff) return (int)hipErrorInvalidValue;
-      if (tiles + mine > 0x7fffffff) break;                // the next launch
+      if (mine > kMostTiles) return (int)hipErrorInvalidValue;
+      if (tiles + mine > kMostTiles) break;                // the next launch
       t.p[c] = reinterpret_cast<const void*>(p[k]);
       t.g[c] = reinterpret_cast<const void*>(g[k]);
       t.out[c] = reinterpret_cast<void*>(out[k]);

@@ -3,6 +3,7 @@
 // Products run on v_mfma_f32_16x16x4_f32 with operands in fp32 (bf16 ones are widened while they are staged), so nothing
 // is rounded before the end; a workgroup of four wavefronts owns 64 x 64 outputs and walks K in steps of 16 through LDS.
 #include "lowrank.h"
+#include "lowrank_tile.h"
 
 using namespace evox;
 using namespace evox::lr;
@@ -376,7 +377,7 @@ int launch_linear(Linear q, Path path, const Layout& at, float* ws, hipStream_t 
     else linear_join_kernel<T><<<stream_grid(quads, NT), NT, 0, s>>>(q);
   };
   auto shrink = [&]() { shrink_kernel<T><<<(unsigned)shrink_blocks(q, sizeof(T), NT), NT, 0, s>>>(q); };
-  if (shrink_blocks(q, sizeof(T), NT) > 0x7fffffff) return (int)hipErrorInvalidValue;
+  if (!fits_launch(shrink_blocks(q, sizeof(T), NT), NT)) return (int)hipErrorInvalidValue;
   if (path == Path::kFew) {
     constexpr int COLS = 64 * 16 / (int)sizeof(T);
     const int first = (int)shrink_blocks(q, sizeof(T), FEW_NT);
@@ -416,7 +417,7 @@ int launch_linear(Linear q, Path path, const Layout& at, float* ws, hipStream_t 
   if (!q.own_t) shrink();
   const int tiles_n = (q.N + BN - 1) / BN;
   const int64_t wgs = (q.rows + BM - 1) / BM * tiles_n * q.splits;
-  if (wgs > 0x7fffffff) return (int)hipErrorInvalidValue;
+  if (!fits_launch(wgs, NT)) return (int)hipErrorInvalidValue;
   linear_kernel<T><<<(unsigned)wgs, NT, 0, s>>>(q, tiles_n);
   if (q.splits > 1) join();
   return last_launch_status();
@@ -427,7 +428,7 @@ int launch_sum(const Sum& q, hipStream_t s) {
   const int tiles_n = (q.N + BN - 1) / BN;
   const int64_t tiles = (int64_t)((q.M + BM - 1) / BM) * tiles_n;
   const int64_t wgs = (tiles + (q.gb != nullptr ? (q.N + 63) / 64 : 0)) * q.splits;
-  if (wgs > 0x7fffffff) return (int)hipErrorInvalidValue;
+  if (!fits_launch(wgs, NT)) return (int)hipErrorInvalidValue;
   sum_kernel<T><<<(unsigned)wgs, NT, 0, s>>>(q, tiles_n, (int)tiles);
   if (q.splits > 1) launch_sum_join(q, s);
   return last_launch_status();

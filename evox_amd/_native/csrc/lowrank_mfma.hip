@@ -447,13 +447,11 @@ int launch(const Linear& q, hipStream_t s) {
   int64_t wgs = tiles_m * g.tiles_n * (SLOTS ? 1 : q.splits);
   const int64_t shrink = !SLOTS && (BM == 16 || q.splits > 1) ? (shrink_blocks(q, sizeof(T), WM * WN * 64) + kNumXCD - 1) / kNumXCD * kNumXCD : 0;
   wgs += shrink;
-  if (wgs > 0x7fffffff) return (int)hipErrorInvalidValue;
+  if (!fits_launch(wgs, WM * WN * 64)) return (int)hipErrorInvalidValue;
   g.shrink = (int)shrink;
-  auto* k = &linear_mfma_kernel<T, BM, BN, WM, WN, STAGES, SLOTS>;
-  static const hipError_t attr =
-      hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
-  if (attr != hipSuccess) return (int)attr;
-  k<<<(unsigned)wgs, WM * WN * 64, LDS, s>>>(q, g);
+  constexpr auto kernel = &linear_mfma_kernel<T, BM, BN, WM, WN, STAGES, SLOTS>;
+  if (const int st = allow_lds<kernel>(LDS)) return st;
+  kernel<<<(unsigned)wgs, WM * WN * 64, LDS, s>>>(q, g);
   return last_launch_status();
 }
 

@@ -303,11 +303,10 @@ int launch(const Sum& q, hipStream_t s) {
   const int tiles_n = (q.N + BM - 1) / BM;
   const int64_t tiles = (int64_t)((q.M + BM - 1) / BM) * tiles_n;
   const int64_t wgs = (tiles + (q.gb != nullptr ? (q.N + 63) / 64 : 0)) * q.splits;
-  if (wgs > 0x7fffffff) return (int)hipErrorInvalidValue;
-  auto* k = &sum_mfma_kernel<T, BM, BM, WM, WN, STAGES, PLANES>;
-  static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
-  if (attr != hipSuccess) return (int)attr;
-  k<<<(unsigned)wgs, WM * WN * 64, LDS, s>>>(q, (int)tiles, tiles_n);
+  if (!fits_launch(wgs, WM * WN * 64)) return (int)hipErrorInvalidValue;
+  constexpr auto kernel = &sum_mfma_kernel<T, BM, BM, WM, WN, STAGES, PLANES>;
+  if (const int st = allow_lds<kernel>(LDS)) return st;
+  kernel<<<(unsigned)wgs, WM * WN * 64, LDS, s>>>(q, (int)tiles, tiles_n);
   return last_launch_status();
 }
 

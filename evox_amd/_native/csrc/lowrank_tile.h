@@ -1,6 +1,7 @@
 // Tiles in LDS for the bf16 matrix instructions: counted waits, transposed reads, permuted rows.
 #pragma once
 #include "lowrank.h"
+#include <atomic>
 
 namespace evox {
 namespace lr {
@@ -9,6 +10,20 @@ using bf16x8 = __attribute__((ext_vector_type(8))) __bf16;
 using s16x8 = __attribute__((ext_vector_type(8))) short;
 typedef __attribute__((address_space(3))) void* lds_vp;
 typedef const __attribute__((address_space(1))) void* glb_vp;
+
+// Lets a kernel ask for `bytes` of LDS on the current device (set once a device; a launch may be the first on any of them).
+template <auto KERNEL>
+inline int allow_lds(int bytes) {
+  static std::atomic<uint32_t> done{0};
+  int dev = 0;
+  if (const hipError_t e = hipGetDevice(&dev)) return (int)e;
+  if (dev < 32 && (done.load(std::memory_order_relaxed) >> dev & 1u)) return 0;
+  if (const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(KERNEL), hipFuncAttributeMaxDynamicSharedMemorySize, bytes)) return (int)e;
+  if (dev < 32) done.fetch_or(1u << dev, std::memory_order_relaxed);
+  return 0;
+}
+// whether a grid fits a launch: its threads are counted in 32 bits
+inline bool fits_launch(int64_t workgroups, int threads) { return workgroups > 0 && workgroups <= 0xffffffffll / threads; }
 
 // at most N loads to LDS outstanding, and every read of LDS returned (its buffer may be refilled behind the next barrier)
 template <int N>

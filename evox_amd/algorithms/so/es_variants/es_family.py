@@ -150,12 +150,14 @@ class _ESBase(Algorithm):
 
     def _step_center(self, state, grad):
         """center ← center + optimizer(grad); returns (center, state)."""
+        if isinstance(self.optimizer, optim.OptaxWrapper):
+            return use_state(self.optimizer.step)(state, grad, state.center)
         updates, state = use_state(self.optimizer.update)(state, grad, state.center)
         return state.center + updates, state
 
 
 class OpenES(_ESBase):
-    """OpenAI-ES (Salimans et al. 2017).  ``optimizer="adam"`` applies Adam to the estimated
+    """OpenAI-ES (Salimans et al. 2017).  ``optimizer="adam"`` (or ``"adamw"``) applies Adam to the estimated
     gradient (the reference passes the parameters instead of the gradient to Adam,
     ``open_es.py:80``; the gradient is used here)."""
 
@@ -169,7 +171,7 @@ class OpenES(_ESBase):
         self._center(center_init)
         self.pop_size, self.learning_rate, self.noise_stdev = pop_size, learning_rate, noise_stdev
         self.mirrored_sampling = mirrored_sampling
-        self.optimizer = _make_optimizer("adam", learning_rate, self.center_init) if optimizer == "adam" else None
+        self.optimizer = _make_optimizer(optimizer, learning_rate, self.center_init) if optimizer in ("adam", "adamw") else None
 
     def setup(self, key):
         key = key.to(self.center_init.device)
@@ -229,7 +231,8 @@ class PGPE(_ESBase):
 
     @property
     def dimension_separable(self):
-        return isinstance(self.optimizer, optim.OptaxWrapper)      # ClipUp caps the norm of the whole update vector
+        # (ClipUp caps the norm of the whole update vector, 8-bit moments share units among neighbours)
+        return isinstance(self.optimizer, optim.OptaxWrapper) and getattr(self.optimizer.optimizer, "separable", True)
 
     def __init__(self, pop_size, center_init, optimizer: Union[str, Stateful, optim.GradientTransformation],
                  stdev_init=0.1, center_learning_rate=0.15, stdev_learning_rate=0.1, stdev_max_change=0.2):
@@ -265,8 +268,7 @@ class PGPE(_ESBase):
         return self._apply(state, delta_x, delta_stdev)
 
     def _apply(self, state, delta_x, delta_stdev):
-        updates, state = use_state(self.optimizer.update)(state, delta_x, state.center)
-        center = state.center + updates
+        center, state = self._step_center(state, delta_x)
         bound = (state.stdev * self.stdev_max_change).abs()
         step = torch.clamp(self.stdev_learning_rate * delta_stdev, -bound, bound)
         return state.replace(center=center, stdev=state.stdev - step)
@@ -318,9 +320,9 @@ class ARS(_ESBase):
         self._center(center_init)
         self.pop_size, self.lr, self.sigma, self.elite_ratio = pop_size, lr, sigma, elite_ratio
         self.elite_pop_size = max(1, int(pop_size / 2 * elite_ratio))
-        if optimizer != "adam":
+        if optimizer not in ("adam", "adamw"):
             raise NotImplementedError(optimizer)
-        self.optimizer = _make_optimizer("adam", lr, self.center_init)
+        self.optimizer = _make_optimizer(optimizer, lr, self.center_init)
 
     def setup(self, key):
         key = key.to(self.center_init.device)
@@ -424,7 +426,7 @@ class ESMC(_ESBase):
         self._center(center_init)
         self.popsize = self.pop_size = pop_size
         self.lr, self.sigma, self.sigma_decay, self.sigma_limit = lr, sigma, sigma_decay, sigma_limit
-        if optimizer not in ("adam", "sgd"):
+        if optimizer not in ("adam", "adamw", "sgd"):
             raise NotImplementedError(optimizer)
         self.optimizer = _make_optimizer(optimizer, lr, self.center_init)
 
@@ -609,7 +611,7 @@ class GuidedES(_ESBase):
         self.sigma, self.subspace_dims = sigma_init, subspace_dims
         self.sigma_decay, self.sigma_limit = sigma_decay, sigma_limit
         self.alpha, self.beta = 0.5, 1.0
-        if optimizer not in ("adam", "sgd"):
+        if optimizer not in ("adam", "adamw", "sgd"):
             raise NotImplementedError(optimizer)
         self.optimizer = _make_optimizer(optimizer, lrate_init, self.center_init)
 
@@ -653,12 +655,12 @@ class ASEBO(_ESBase):
                  sigma_decay=1.0, sigma_limit=0.01, mean_decay=0.0, subspace_dims=50):
         if pop_size % 2:
             raise ValueError("pop_size must be even")
-        if optimizer != "adam":
+        if optimizer not in ("adam", "adamw"):
             raise NotImplementedError(optimizer)
         self._center(center_init)
         self.pop_size, self.lr, self.sigma = pop_size, lr, sigma
         self.sigma_decay, self.sigma_limit, self.subspace_dims = sigma_decay, sigma_limit, subspace_dims
-        self.optimizer = _make_optimizer("adam", lr, self.center_init)
+        self.optimizer = _make_optimizer(optimizer, lr, self.center_init)
 
     def setup(self, key):
         dev = self.center_init.device
@@ -728,7 +730,7 @@ class Noise_reuse_es(_ESBase):
         self.popsize = self.pop_size = pop_size
         self.lr, self.sigma, self.T, self.K = lr, sigma, T, K
         self.sigma_decay, self.sigma_limit = sigma_decay, sigma_limit
-        if optimizer not in ("adam", "sgd"):
+        if optimizer not in ("adam", "adamw", "sgd"):
             raise NotImplementedError(optimizer)
         self.optimizer = _make_optimizer(optimizer, lr, self.center_init)
 
@@ -778,7 +780,7 @@ class PersistentES(_ESBase):
         self.popsize = self.pop_size = pop_size
         self.lr, self.sigma, self.T, self.K = lr, sigma, T, K
         self.sigma_decay, self.sigma_limit = sigma_decay, sigma_limit
-        if optimizer not in ("adam", "sgd"):
+        if optimizer not in ("adam", "adamw", "sgd"):
             raise NotImplementedError(optimizer)
         self.optimizer = _make_optimizer(optimizer, lr, self.center_init)
 

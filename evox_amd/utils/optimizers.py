@@ -82,6 +82,7 @@ class AdamW(GradientTransformation):
 
     step: Callable
     moments: Callable
+    separable: bool      # every variable's step depends on its own gradients alone (8-bit moments share a unit among 32)
 
 
 def adamw(learning_rate: float, b1: float = 0.9, b2: float = 0.999, eps: float = 1e-8, weight_decay: float = 1e-2,
@@ -141,7 +142,7 @@ def adamw(learning_rate: float, b1: float = 0.9, b2: float = 0.999, eps: float =
         return tuple(trees)
 
     opt = AdamW(init, update)
-    opt.step, opt.moments = step, moments
+    opt.step, opt.moments, opt.separable = step, moments, state_bits == 32
     return opt
 
 
@@ -167,6 +168,16 @@ class OptaxWrapper(Stateful):
     def update(self, state, grads, params=None):
         updates, opt_state = self.optimizer.update(grads, state.opt_state, params)
         return updates, state.replace(opt_state=opt_state)
+
+    def step(self, state, grads, params):
+        """Parameters after the update: the optimizer's own whole step where it has one."""
+        fused = getattr(self.optimizer, "step", None)
+        if fused is not None:
+            params, opt_state = fused(grads, state.opt_state, params)
+        else:
+            updates, opt_state = self.optimizer.update(grads, state.opt_state, params)
+            params = apply_updates(params, updates)
+        return params, state.replace(opt_state=opt_state)
 
 
 def tree_l2_norm(tree):

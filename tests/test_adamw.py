@@ -346,6 +346,26 @@ def test_in_evolution_strategies(device):
     assert bool(torch.isfinite(state.get_child_state("algorithm").center).all())
 
 
+def test_named_in_every_strategy():
+    """"adamw" where "adam" is taken, and the wrapper's whole step equals update + apply for optimizers without one."""
+    center = torch.full((6,), 2.0)
+    for algo in (algorithms.OpenES(center, 8, 0.1, 0.1, optimizer="adamw"), algorithms.ARS(8, center, optimizer="adamw"),
+                 algorithms.ESMC(9, center, optimizer="adamw"), algorithms.GuidedES(8, center, optimizer="adamw", lrate_init=0.1),
+                 algorithms.ASEBO(8, center, optimizer="adamw", subspace_dims=6), algorithms.Noise_reuse_es(8, center, optimizer="adamw"),
+                 algorithms.PersistentES(8, center, optimizer="adamw"), algorithms.PGPE(8, center, "adamw")):
+        wf = workflows.StdWorkflow(algo, problems.numerical.Sphere())
+        state = wf.step(wf.init(PRNGKey(1)))
+        moved = state.get_child_state("algorithm").center
+        assert bool(torch.isfinite(moved).all()) and not torch.equal(moved, center), type(algo).__name__
+    assert algorithms.PGPE(8, center, optimizers.adamw(0.1)).dimension_separable
+    assert not algorithms.PGPE(8, center, optimizers.adamw(0.1, state_bits=8)).dimension_separable
+    wrapper = optimizers.OptaxWrapper(optimizers.adam(0.1), center)
+    state = wrapper.init(PRNGKey(0))
+    updates, after = wrapper.update(state, torch.ones(6), center)
+    new, after2 = wrapper.step(state, torch.ones(6), center)
+    assert torch.equal(new, center + updates) and torch.equal(after.opt_state["mu"], after2.opt_state["mu"])
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("bits", [32, 8])
 def test_recorded_step(cuda, bits):

@@ -73,6 +73,7 @@ LINEAR = [  # individuals, rows each, in, out, rank
     (70, 33, 72, 136, 2), (1, 300, 520, 392, 33), (16, 48, 1024, 128, 17), (1, 1, 4096, 1000, 16), (1000, 1, 11, 3, 1),
     (1400, 1, 1001, 1003, 3), (4100, 1, 244, 1024, 2), (70, 20, 1024, 1010, 20), (13, 1, 512, 264, 5), (5, 3, 1096, 136, 2),
     (20, 1, 768, 1032, 4), (600, 1, 64, 520, 3), (9000, 1, 40, 260, 1),
+    (200, 24, 1001, 259, 5),
 ]
 
 
@@ -211,7 +212,7 @@ def check_sum(got, w, a, b, scale=1.0):
 
 SUM = [  # individuals, in, out, rank
     (1, 1, 1, 1), (2, 3, 5, 1), (7, 64, 64, 1), (33, 65, 63, 2), (100, 11, 32, 1), (500, 32, 3, 3), (64, 256, 128, 4), (31, 250, 136, 5),
-    (1000, 130, 264, 2), (3, 1000, 700, 16), (200, 512, 512, 8), (5000, 17, 9, 1), (40, 8, 2000, 33), (129, 384, 72, 16),
+    (1000, 130, 264, 2), (3, 1000, 700, 16), (200, 512, 512, 8), (5000, 17, 9, 1), (40, 8, 2000, 33), (129, 384, 72, 16), (700, 250, 333, 7),
 ]
 
 

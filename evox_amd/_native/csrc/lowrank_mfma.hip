@@ -1,22 +1,27 @@
 // Low-rank population layer on v_mfma_f32_16x16x32_bf16 and v_mfma_f32_16x16x4_f32: y = act(x W + bias + s (x A_p^T) B_p + s c_p).
 //
-// A workgroup of WM x WN wavefronts owns BM x BN outputs and walks K in steps of 64.  Both operands go from memory to LDS
-// without passing registers (16 bytes a lane, two stages: the next step's loads are in flight while a step is multiplied).
-//   x  (K contiguous): rows of 128 bytes, 16-byte pieces permuted by the row (XOR), read as they are (ds_read_b128);
-//   W  (N contiguous): rows of 2 BN bytes, 32-byte pieces permuted by the row, read transposed (ds_read_b64_tr_b16: 16 lanes
-//      exchange a 4 x 16 block so that a lane holds four consecutive k of its column).  No transposed copy of W is made, which
-//      a step of evolution that changes W every generation would pay for every time.
+// A workgroup of WM x WN wavefronts owns BM x BN outputs and walks K in steps of 64 bytes (32 bf16, 16 floats).  Both operands go
+// from memory to LDS without passing registers (16 bytes a lane; STAGES - 1 steps in flight behind counted waits).
+//   x  (K contiguous): rows of 64 bytes, 16-byte pieces permuted by the row (XOR), a fragment is one 16-byte read;
+//   W  (N contiguous): bf16: 32-byte pieces permuted by the row, read transposed (ds_read_b64_tr_b16: 16 lanes exchange a 4 x 16
+//      block so that a lane holds four consecutive k of its column); float32: four words down a column.  No transposed copy of
+//      W is made, which a step of evolution, that changes W every generation, would pay for every time.
 // The permutations are applied to the source addresses (the LDS image of a load is linear); they spread the rows that one read
-// touches over all banks.  Pieces behind K come from a zero in memory, so any K that is a multiple of 8 works.
+// touches over all banks.  Pieces behind K come from a zero in memory.
 // The matrix instruction takes W's fragment as its first operand: a lane then holds four consecutive columns of one row.
+// Tiles: 256 x 256 (bf16, eight wavefronts, the two of a SIMD half a step apart) where they fill the chip, else 128 x 128 or
+// 64 x 64 with K divided over workgroups; 16 x 128 for requests.  65536 x 2048 x 2048 bf16 with 256 individuals of rank 16: 612 us
+// (0.91 PFLOP/s; 530 without the tiles' ends, 377 without loads, 388 with nothing but loads); 16384 x 1024 x 1024 float32, rank 8:
+// 343 us (the matrix pipe is busy 75 % of the time); 4096 x 1024 x 720 bf16, single rows, rank 4: 25 us and 9 for t (its tiles of 64
+// move 200 MB from the second-level cache, 16 us; tiles of 128 half of that, with idle compute units: 33 to 43 us).
 //
 // The individuals' part:
-//   GROUPED (an individual has at least 16 rows): the 16-row fragments of a tile each belong to one individual (its last one may
-//     be partly empty).  t = x A_p^T is one more matrix product of the x fragment that is in registers anyway, against A_p read
-//     straight from memory (K contiguous) — 1/16 more instructions per wavefront, no second pass over x and no launch of
-//     its own.  At the end s t is split into two bf16 halves (together 16 bits), [t_hi | t_lo] times [B_p; B_p] is one
-//     instruction per fragment of outputs.  Rank at most 16.
-//   otherwise (single rows, requests): t comes from shrink_kernel, every lane adds its row's R products to its columns.
+//   GROUPED (an individual has at least 16 rows, rank at most 16): the 16-row fragments of a tile each belong to one individual
+//     (its last one may be partly empty).  t = x A_p^T is one more matrix product of x's fragments, against A_p's rows in the stage
+//     (a slot for each individual that meets in the tile) - no second pass over x and no launch of its own.  At the end s t
+//     (bf16: in two halves, together 16 bits) times B_p is one product per fragment of outputs.
+//   otherwise (single rows, requests): t comes from shrink_block - workgroups of their own in front, a launch before, or the
+//     workgroup itself where its rows are nobody else's - and every lane adds its row's R products to its columns.
 #include "lowrank.h"
 #include "lowrank_tile.h"
 

@@ -9,6 +9,9 @@
 // 16384 terms or more take two: the float32 accumulation of such sums leaves more than that by itself (1.6e-6 of the result at
 // 16384 random terms, 4.6e-6 at 65536), and a third plane costs half as much time again.
 // The wavefronts of a workgroup are laid out so that each splits few fragments of A and uses each split for many of B.
+// K = 65536, 2048 x 2048 bf16: 925 to 975 us (1.15 PFLOP/s of plane products; a library product of this card reaches 1.10 at 8192^3,
+// the tensor form takes 4040 us); K = 16384, 1024 x 720: 71 us; the latter in float32: 247 us.  A factor that is not finite makes
+// its row or column not finite (an infinite bf16 factor: NaN where the exact sum would be infinite).
 // K is divided over as many workgroups as fill the chip; the partial sums are added by sum_join_kernel in a fixed order.
 #include "lowrank.h"
 #include "lowrank_tile.h"

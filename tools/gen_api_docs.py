@@ -18,7 +18,7 @@ MODULES = [
     "evox_amd.utils", "evox_amd.vis_tools.plot", "evox_amd.models", "evox_amd.ops.blas", "evox_amd.ops.sort",
     "evox_amd.ops.gemm", "evox_amd.ops.cma", "evox_amd.ops.nds", "evox_amd.ops.es", "evox_amd.ops.de",
     "evox_amd.ops.variation", "evox_amd.ops.de_adapt", "evox_amd.parallel.p2p", "evox_amd.ops.fitness", "evox_amd.ops.swarm", "evox_amd.ops.moselect", "evox_amd.ops.hv",
-    "evox_amd.ops.distance", "evox_amd.ops.linalg_small",
+    "evox_amd.ops.distance", "evox_amd.ops.linalg_small", "evox_amd.ops.lowrank", "evox_amd.ops.adamw", "evox_amd.utils.optimizers",
     "evox_amd.utils.graph", "evox_amd.utils.profiling",
 ]
 

@@ -68,14 +68,14 @@ def _check_leaves(leaves, what):
 
 
 def _check_state(state, device, total):
-    bits = 8 if state["mu"].dtype == torch.uint8 else 32
-    want = {"count": (torch.float32, 1), "mu": (torch.float32 if bits == 32 else torch.uint8, total)}
-    want["nu"] = want["mu"]
+    bits = 8 if state["mu"].dtype is torch.uint8 else 32
+    moment = torch.uint8 if bits == 8 else torch.float32
+    want = (("count", torch.float32, 1), ("mu", moment, total), ("nu", moment, total))
     if bits == 8:
-        want["mu_scale"] = want["nu_scale"] = (torch.uint8, total // BLOCK)
-    for name, (dtype, n) in want.items():
+        want += (("mu_scale", torch.uint8, total // BLOCK), ("nu_scale", torch.uint8, total // BLOCK))
+    for name, dtype, n in want:
         t = state.get(name)
-        if t is None or t.dtype != dtype or t.numel() != n or t.device != device or not t.is_contiguous():
+        if t is None or t.dtype is not dtype or t.numel() != n or t.device != device or not t.is_contiguous():
             raise ValueError(f"adamw: the state's {name!r} does not belong to these parameters "
                              f"(expected {n} contiguous {dtype} elements on {device})")
     return bits
@@ -97,7 +97,7 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], st
         raise ValueError("adamw: decay needs one entry per parameter")
     _check_leaves(grads, "grads")
     device = params[0].device
-    if grads[0].device != device:
+    if grads[0].get_device() != params[0].get_device():
         raise ValueError("adamw: parameters and gradients are on different devices")
     total, sizes = 0, []
     for p, g in zip(params, grads):

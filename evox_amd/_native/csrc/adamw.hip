@@ -130,8 +130,9 @@ __device__ __forceinline__ uint32_t finite_bits(float v) {
   return m < 0x7f800000u ? m : 0u;
 }
 
-// BITS: 32 or 8.  A workgroup owns VPT * 1024 consecutive elements of one leaf, a lane four consecutive ones of each 1024.
-template <int BITS, int VPT>
+// BITS: 32 or 8.  A workgroup owns 1024 consecutive elements of one leaf, a lane four of them (eight a lane: 297 us against 287 for
+// the 67 M parameters, 444 against 420 for the 134 M).
+template <int BITS>
 __global__ __launch_bounds__(NT) void adamw_kernel(Leaves t, Hyper h, const float* __restrict__ count_in,
                                                    float* __restrict__ count_out, const void* __restrict__ mu_in,
                                                    const void* __restrict__ nu_in, const uint8_t* __restrict__ mus_in,
@@ -150,87 +151,79 @@ __global__ __launch_bounds__(NT) void adamw_kernel(Leaves t, Hyper h, const floa
   const int64_t n = t.n[lo], padded = (n + kAlign - 1) / kAlign * kAlign, s0 = t.state[lo] * kAlign;
   const void* p = t.p[lo];
   const void* g = t.g[lo];
-  const int64_t base = (int64_t)(blockIdx.x - t.tile[lo]) * (VPT * 1024) + threadIdx.x * 4;
+  const int64_t i = (int64_t)(blockIdx.x - t.tile[lo]) * (4 * NT) + threadIdx.x * 4;
 
-  float pv[VPT][4], gv[VPT][4], m[VPT][4], v[VPT][4];
-#pragma unroll
-  for (int k = 0; k < VPT; ++k) {
-    const int64_t i = base + k * 1024;
-    if (i < padded) {
-      load4(p, flags & kParamBf16, flags & kParamVec, i, n, pv[k]);
-      load4(g, flags & kGradBf16, flags & kGradVec, i, n, gv[k]);
-      if constexpr (BITS == 32) {
-        const float4 a = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(mu_in) + s0 + i);
-        const float4 b = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(nu_in) + s0 + i);
-        m[k][0] = a.x; m[k][1] = a.y; m[k][2] = a.z; m[k][3] = a.w;
-        v[k][0] = b.x; v[k][1] = b.y; v[k][2] = b.z; v[k][3] = b.w;
-      } else {
-        const uint32_t a = *reinterpret_cast<const uint32_t*>(reinterpret_cast<const uint8_t*>(mu_in) + s0 + i);
-        const uint32_t b = *reinterpret_cast<const uint32_t*>(reinterpret_cast<const uint8_t*>(nu_in) + s0 + i);
-        const int qa = mus_in[(s0 + i) / kBlock], qb = nus_in[(s0 + i) / kBlock];
-#pragma unroll
-        for (int l = 0; l < 4; ++l) {
-          m[k][l] = decode<true>((a >> (8 * l)) & 0xffu, qa);
-          v[k][l] = decode<false>((b >> (8 * l)) & 0xffu, qb);
-        }
-      }
+  float pv[4], gv[4], m[4], v[4];
+  if (i < padded) {
+    load4(p, flags & kParamBf16, flags & kParamVec, i, n, pv);
+    load4(g, flags & kGradBf16, flags & kGradVec, i, n, gv);
+    if constexpr (BITS == 32) {
+      const float4 a = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(mu_in) + s0 + i);
+      const float4 b = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(nu_in) + s0 + i);
+      m[0] = a.x; m[1] = a.y; m[2] = a.z; m[3] = a.w;
+      v[0] = b.x; v[1] = b.y; v[2] = b.z; v[3] = b.w;
     } else {
+      const uint32_t a = *reinterpret_cast<const uint32_t*>(reinterpret_cast<const uint8_t*>(mu_in) + s0 + i);
+      const uint32_t b = *reinterpret_cast<const uint32_t*>(reinterpret_cast<const uint8_t*>(nu_in) + s0 + i);
+      const int qa = mus_in[(s0 + i) / kBlock], qb = nus_in[(s0 + i) / kBlock];
 #pragma unroll
-      for (int l = 0; l < 4; ++l) pv[k][l] = gv[k][l] = m[k][l] = v[k][l] = 0.f;
+      for (int l = 0; l < 4; ++l) {
+        m[l] = decode<true>((a >> (8 * l)) & 0xffu, qa);
+        v[l] = decode<false>((b >> (8 * l)) & 0xffu, qb);
+      }
     }
+  } else {
+#pragma unroll
+    for (int l = 0; l < 4; ++l) pv[l] = gv[l] = m[l] = v[l] = 0.f;
   }
   const float c1 = -expm1f(step * h.log_b1), c2 = -expm1f(step * h.log_b2);      // 1 - b^t without cancellation
   const float wd = flags & kDecay ? h.wd : 0.f;
+  float o[4];
 #pragma unroll
-  for (int k = 0; k < VPT; ++k) {
-    const int64_t i = base + k * 1024;
-    float o[4];
+  for (int l = 0; l < 4; ++l) {
+    m[l] = h.b1 * m[l] + h.omb1 * gv[l];
+    v[l] = h.b2 * v[l] + h.omb2 * gv[l] * gv[l];
+    float d = (m[l] / c1) / (sqrtf(v[l] / c2) + h.eps);
+    if (wd != 0.f) d += wd * pv[l];
+    o[l] = h.updates ? -h.lr * d : pv[l] - h.lr * d;
+  }
+  if (i < n) store4(t.out[lo], flags & kParamBf16, flags & kOutVec, i, n, o);
+  // the moments behind a leaf's last element stay zero
+#pragma unroll
+  for (int l = 0; l < 4; ++l)
+    if (i + l >= n) m[l] = v[l] = 0.f;
+  if constexpr (BITS == 32) {
+    if (i < padded) {
+      *reinterpret_cast<float4*>(reinterpret_cast<float*>(mu_out) + s0 + i) = make_float4(m[0], m[1], m[2], m[3]);
+      *reinterpret_cast<float4*>(reinterpret_cast<float*>(nu_out) + s0 + i) = make_float4(v[0], v[1], v[2], v[3]);
+    }
+  } else {
+    // eight neighbouring lanes hold a block of 32
+    uint32_t bm = 0, bv = 0;
 #pragma unroll
     for (int l = 0; l < 4; ++l) {
-      m[k][l] = h.b1 * m[k][l] + h.omb1 * gv[k][l];
-      v[k][l] = h.b2 * v[k][l] + h.omb2 * gv[k][l] * gv[k][l];
-      float d = (m[k][l] / c1) / (sqrtf(v[k][l] / c2) + h.eps);
-      if (wd != 0.f) d += wd * pv[k][l];
-      o[l] = h.updates ? -h.lr * d : pv[k][l] - h.lr * d;
+      bm = max(bm, finite_bits(m[l]));
+      bv = max(bv, finite_bits(v[l]));
     }
-    if (i < n) store4(t.out[lo], flags & kParamBf16, flags & kOutVec, i, n, o);
-    // the moments behind a leaf's last element stay zero
 #pragma unroll
-    for (int l = 0; l < 4; ++l)
-      if (i + l >= n) m[k][l] = v[k][l] = 0.f;
-    if constexpr (BITS == 32) {
-      if (i < padded) {
-        *reinterpret_cast<float4*>(reinterpret_cast<float*>(mu_out) + s0 + i) = make_float4(m[k][0], m[k][1], m[k][2], m[k][3]);
-        *reinterpret_cast<float4*>(reinterpret_cast<float*>(nu_out) + s0 + i) = make_float4(v[k][0], v[k][1], v[k][2], v[k][3]);
-      }
-    } else {
-      // eight neighbouring lanes hold a block of 32
-      uint32_t bm = 0, bv = 0;
+    for (int o2 = 1; o2 < 8; o2 <<= 1) {
+      bm = max(bm, (uint32_t)__shfl_xor((int)bm, o2, 64));
+      bv = max(bv, (uint32_t)__shfl_xor((int)bv, o2, 64));
+    }
+    const int qm = unit_of<true>(bm), qv = unit_of<false>(bv);
+    const uint32_t e0 = (uint32_t)(s0 + i) * kPhase, ti = (uint32_t)step;
+    uint32_t cm = 0, cv = 0;
 #pragma unroll
-      for (int l = 0; l < 4; ++l) {
-        bm = max(bm, finite_bits(m[k][l]));
-        bv = max(bv, finite_bits(v[k][l]));
-      }
-#pragma unroll
-      for (int o2 = 1; o2 < 8; o2 <<= 1) {
-        bm = max(bm, (uint32_t)__shfl_xor((int)bm, o2, 64));
-        bv = max(bv, (uint32_t)__shfl_xor((int)bv, o2, 64));
-      }
-      const int qm = unit_of<true>(bm), qv = unit_of<false>(bv);
-      const uint32_t e0 = (uint32_t)(s0 + i) * kPhase, ti = (uint32_t)step;
-      uint32_t cm = 0, cv = 0;
-#pragma unroll
-      for (int l = 0; l < 4; ++l) {
-        cm |= encode<true>(m[k][l], qm, (e0 + l * kPhase + ti * kStepMu) >> 16) << (8 * l);
-        cv |= encode<false>(v[k][l], qv, (e0 + l * kPhase + ti * kStepNu) >> 16) << (8 * l);
-      }
-      if (i < padded) {
-        *reinterpret_cast<uint32_t*>(reinterpret_cast<uint8_t*>(mu_out) + s0 + i) = cm;
-        *reinterpret_cast<uint32_t*>(reinterpret_cast<uint8_t*>(nu_out) + s0 + i) = cv;
-        if ((threadIdx.x & 7) == 0) {
-          mus_out[(s0 + i) / kBlock] = (uint8_t)qm;
-          nus_out[(s0 + i) / kBlock] = (uint8_t)qv;
-        }
+    for (int l = 0; l < 4; ++l) {
+      cm |= encode<true>(m[l], qm, (e0 + l * kPhase + ti * kStepMu) >> 16) << (8 * l);
+      cv |= encode<false>(v[l], qv, (e0 + l * kPhase + ti * kStepNu) >> 16) << (8 * l);
+    }
+    if (i < padded) {
+      *reinterpret_cast<uint32_t*>(reinterpret_cast<uint8_t*>(mu_out) + s0 + i) = cm;
+      *reinterpret_cast<uint32_t*>(reinterpret_cast<uint8_t*>(nu_out) + s0 + i) = cv;
+      if ((threadIdx.x & 7) == 0) {
+        mus_out[(s0 + i) / kBlock] = (uint8_t)qm;
+        nus_out[(s0 + i) / kBlock] = (uint8_t)qv;
       }
     }
   }
@@ -254,11 +247,11 @@ __global__ __launch_bounds__(NT) void adamw_read_kernel(const uint8_t* __restric
   }
 }
 
-template <int BITS, int VPT>
+template <int BITS>
 int launch(int n_leaves, const int64_t* p, const int64_t* g, const int64_t* out, const int64_t* n, const int64_t* flags,
            const Hyper& h, const float* count_in, float* count_out, const void* mu, const void* nu, const uint8_t* mus,
            const uint8_t* nus, void* mu_out, void* nu_out, uint8_t* mus_out, uint8_t* nus_out, hipStream_t stream) {
-  constexpr int64_t kTile = VPT * 1024, kMostTiles = 0xffffffffll / NT;      // (a launch counts its threads in 32 bits)
+  constexpr int64_t kTile = 4 * NT, kMostTiles = 0xffffffffll / NT;      // (a launch counts its threads in 32 bits)
   int64_t state = 0;
   bool first = true;
   int k = 0;
@@ -289,7 +282,7 @@ int launch(int n_leaves, const int64_t* p, const int64_t* g, const int64_t* out,
     if (c == 0) break;
     t.tile[c] = (uint32_t)tiles;
     t.count = c;
-    adamw_kernel<BITS, VPT><<<(unsigned)tiles, NT, 0, stream>>>(t, h, count_in, first ? count_out : nullptr, mu, nu, mus, nus,
+    adamw_kernel<BITS><<<(unsigned)tiles, NT, 0, stream>>>(t, h, count_in, first ? count_out : nullptr, mu, nu, mus, nus,
                                                                 mu_out, nu_out, mus_out, nus_out);
     if (const int st = last_launch_status()) return st;
     first = false;
@@ -314,8 +307,8 @@ EVOX_API int evox_hip_adamw(int bits, int n_leaves, const int64_t* p, const int6
   if (need != total || (bits != 8 && bits != 32)) return (int)hipErrorInvalidValue;
   const Hyper h{hyper[0], hyper[1], hyper[2], hyper[3], hyper[4], hyper[5], hyper[6], hyper[7], hyper[8], updates};
   hipStream_t s = (hipStream_t)stream;
-#define EVOX_ADAMW(B, V) launch<B, V>(n_leaves, p, g, out, n, flags, h, count_in, count_out, mu, nu, mus, nus, mu_out, nu_out, mus_out, nus_out, s)
-  return bits == 32 ? EVOX_ADAMW(32, 1) : EVOX_ADAMW(8, 1);
+#define EVOX_ADAMW(B) launch<B>(n_leaves, p, g, out, n, flags, h, count_in, count_out, mu, nu, mus, nus, mu_out, nu_out, mus_out, nus_out, s)
+  return bits == 32 ? EVOX_ADAMW(32) : EVOX_ADAMW(8);
 #undef EVOX_ADAMW
 }
 

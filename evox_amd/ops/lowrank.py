@@ -33,22 +33,23 @@ _MOST = 2 ** 31 - 1
 
 
 def _check_factors(what, a, b):
-    for name, t in (("a", a), ("b", b)):
-        if t.dim() != 3:
-            raise ValueError(f"{what}: {name} has three dimensions (individuals, rank, features), got shape {tuple(t.shape)}")
-        if t.dtype not in DTYPE_CODE:
-            raise TypeError(f"{what} takes float32 or bfloat16 factors, got {t.dtype}")
-    r = a.shape[1]
-    if b.shape[0] != a.shape[0] or b.shape[1] not in (r, r + 1) or r < 1:
+    sa, sb = a.shape, b.shape
+    for name, shape in (("a", sa), ("b", sb)):
+        if len(shape) != 3:
+            raise ValueError(f"{what}: {name} has three dimensions (individuals, rank, features), got shape {tuple(shape)}")
+    if a.dtype not in DTYPE_CODE or b.dtype not in DTYPE_CODE:
+        raise TypeError(f"{what} takes float32 or bfloat16 factors, got {a.dtype} and {b.dtype}")
+    r = sa[1]
+    if sb[0] != sa[0] or not r <= sb[1] <= r + 1 or r < 1:
         raise ValueError(f"{what}: a is (P, r, in) and b (P, r, out) or, with own biases, (P, r + 1, out), r >= 1; got "
-                         f"{tuple(a.shape)} and {tuple(b.shape)}")
-    if a.dtype != b.dtype:
+                         f"{tuple(sa)} and {tuple(sb)}")
+    if a.dtype is not b.dtype:
         raise TypeError(f"{what}: the factors have different types, {a.dtype} and {b.dtype}")
-    if a.shape[2] < 1:
+    if sa[2] < 1:
         raise ValueError(f"{what} needs at least one input feature")
-    if max(a.shape[1:]) > _MOST or max(b.shape[1:]) > _MOST:
+    if r > _MOST or sa[2] > _MOST or sb[2] > _MOST:
         raise ValueError(f"{what}: a factor's rank and features lie below 2^31")
-    return r, b.shape[1] - r
+    return r, sb[1] - r
 
 
 def _no_grad_wanted(what, *tensors):
@@ -105,8 +106,10 @@ def lowrank_linear(x: torch.Tensor, weight: torch.Tensor, a: torch.Tensor, b: to
         raise ValueError(f"lowrank_linear: activation is one of {sorted(_ACT)}, got {activation!r}")
     _no_grad_wanted("lowrank_linear", x, weight, a, b, bias)
     dev = x.device
-    if any(t is not None and t.device != dev for t in (weight, a, b, index, bias)):
-        raise ValueError("lowrank_linear: inputs on different devices")
+    where = x.get_device()
+    for t in (weight, a, b, index, bias):
+        if t is not None and t.get_device() != where:
+            raise ValueError("lowrank_linear: inputs on different devices")
     if not on_gpu(x):
         return lowrank_linear_reference(x, weight, a, b, index, bias, scale, activation)
     y = x.new_empty((*x.shape[:-1], n_out))
@@ -127,7 +130,7 @@ def lowrank_linear(x: torch.Tensor, weight: torch.Tensor, a: torch.Tensor, b: to
     call = (x.data_ptr(), weight.data_ptr(), a.data_ptr(), b.data_ptr(), None if bias is None else bias.data_ptr(),
             None if index is None else index.data_ptr(), y.data_ptr(), ctypes.addressof(dims), ctypes.addressof(ints))
     floats = lib.evox_hip_lowrank_linear_ws(*call)
-    ws = torch.empty(floats, dtype=torch.float32, device=dev) if floats > 0 else None
+    ws = x.new_empty(floats, dtype=torch.float32) if floats > 0 else None
     with launch_device(dev):
         check(lib.evox_hip_lowrank_linear(*call, None if ws is None else ws.data_ptr(), floats, float(scale), stream_of(y)), "lowrank_linear")
     return y

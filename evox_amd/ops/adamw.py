@@ -90,36 +90,43 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], st
     from leaf to leaf and between a parameter and its gradient), ``decay`` says for each leaf whether ``weight_decay`` applies
     to it (default: to all).  Arithmetic is float32 whatever the types, results have the parameters' types and are contiguous.
     Nothing is written in place, no autograd graph is built.  On a GPU all leaves take one launch per 72 of them."""
-    _check_leaves(params, "params")
     if len(params) != len(grads):
         raise ValueError(f"adamw: {len(params)} parameters but {len(grads)} gradients")
     if decay is not None and len(decay) != len(params):
         raise ValueError("adamw: decay needs one entry per parameter")
-    _check_leaves(grads, "grads")
+    if not params:
+        raise ValueError("adamw needs at least one tensor in params")
+    # one pass over the leaves: a tree of many small ones is bound by it
+    total, sizes, flags = 0, [], []
+    try:
+        where = params[0].get_device()
+        for p, g in zip(params, grads):
+            flags.append(DTYPE_CODE[p.dtype] | DTYPE_CODE[g.dtype] << 1)
+            if p.shape != g.shape:
+                raise ValueError(f"adamw: a parameter of shape {tuple(p.shape)} has a gradient of shape {tuple(g.shape)}")
+            if p.get_device() != where or g.get_device() != where:
+                raise ValueError("adamw: parameters and gradients are on different devices")
+            n = p.numel()
+            sizes.append(n)
+            total += -(-n // ALIGN) * ALIGN
+    except (AttributeError, KeyError):
+        _check_leaves(params, "params")
+        _check_leaves(grads, "grads")
+        raise
     device = params[0].device
-    if grads[0].get_device() != params[0].get_device():
-        raise ValueError("adamw: parameters and gradients are on different devices")
-    total, sizes = 0, []
-    for p, g in zip(params, grads):
-        if p.shape != g.shape:
-            raise ValueError(f"adamw: a parameter of shape {tuple(p.shape)} has a gradient of shape {tuple(g.shape)}")
-        n = p.numel()
-        sizes.append(n)
-        total += -(-n // ALIGN) * ALIGN
     bits = _check_state(state, device, total)
     hyper = (learning_rate, b1, b2, 1 - b1, 1 - b2, eps, weight_decay, math.log(b1) if b1 else -math.inf,
              math.log(b2) if b2 else -math.inf)
-    if device.type != "cuda" or total == 0:
+    if where < 0 or total == 0:
         return adamw_step_reference(params, grads, state, hyper, bits, decay, updates)
-    return _step_hip(params, grads, sizes, state, hyper, bits, decay, updates, total, device)
+    return _step_hip(params, grads, sizes, flags, state, hyper, bits, decay, updates, total, device)
 
 
-def _step_hip(params, grads, sizes, state, hyper, bits, decay, updates, total, device):
-    n, bf16 = len(params), torch.bfloat16
-    new, out = {}, []
-    ptrs = [0] * (5 * n)
+def _step_hip(params, grads, sizes, flags, state, hyper, bits, decay, updates, total, device):
+    n = len(params)
+    new, out, p_at, g_at, o_at = {}, [], [], [], []
     kept = []                                       # contiguous copies, alive until the launch
-    for k, (p, g) in enumerate(zip(params, grads)):
+    for p, g in zip(params, grads):
         if not p.is_contiguous():
             p = p.contiguous()
             kept.append(p)
@@ -128,17 +135,18 @@ def _step_hip(params, grads, sizes, state, hyper, bits, decay, updates, total, d
             kept.append(g)
         o = torch.empty_like(p)                     # (two microseconds less than naming shape, type and device)
         out.append(o)
-        ptrs[k], ptrs[n + k], ptrs[2 * n + k], ptrs[3 * n + k] = p.data_ptr(), g.data_ptr(), o.data_ptr(), sizes[k]
-        ptrs[4 * n + k] = (p.dtype is bf16) | (g.dtype is bf16) << 1 | (decay is None or bool(decay[k])) << 2
+        p_at.append(p.data_ptr())
+        g_at.append(g.data_ptr())
+        o_at.append(o.data_ptr())
+    flags = [f | 4 for f in flags] if decay is None else [f | bool(d) << 2 for f, d in zip(flags, decay)]
     new["count"] = torch.empty_like(state["count"])
     new["mu"], new["nu"] = torch.empty_like(state["mu"]), torch.empty_like(state["nu"])
+    scales = new_scales = (None, None)
     if bits == 8:
         new["mu_scale"], new["nu_scale"] = torch.empty_like(state["mu_scale"]), torch.empty_like(state["nu_scale"])
         scales = (state["mu_scale"].data_ptr(), state["nu_scale"].data_ptr())
         new_scales = (new["mu_scale"].data_ptr(), new["nu_scale"].data_ptr())
-    else:
-        scales = new_scales = (None, None)
-    table = (ctypes.c_int64 * (5 * n))(*ptrs)
+    table = (ctypes.c_int64 * (5 * n))(*p_at, *g_at, *o_at, *sizes, *flags)
     at = ctypes.addressof(table)
     h = (ctypes.c_float * 9)(*hyper)
     with launch_device(device):

@@ -73,33 +73,39 @@ void launch_pack(const Rows& q, T* out, hipStream_t s) {
 }
 int up16(int cols, int elem) { return (cols * elem + 15) / 16 * 16 / elem; }
 
-// acc[a][b][i] = C[wm0 + 16 a + (lane & 15)][wn0 + 16 b + 4 (lane >> 4) + i] of the tile, given its operands' stagers:
-// stage_a(k, m), stage_b(k, n) return element (m0 + m, k) and (k, n0 + n) as floats, zero outside.
-template <class SA, class SB>
-__device__ __forceinline__ void tile_product(int64_t k_begin, int64_t k_end, SA stage_a, SB stage_b, f32x4 (&acc)[2][2]) {
-  __shared__ float sa[BK][PM], sb[BK][PM];
+// acc[a][b][i] = C[wm0 + 16 a + (lane & 15)][wn0 + 16 b + 4 (lane >> 4) + i] of the tile, given its operands: load_a(k0, k_end) and
+// load_b(k0, k_end) return this thread's four elements of the step's tiles (zero outside), put_a and put_b place them in LDS.
+// A step's loads are on their way while the step before is multiplied.
+template <class LA, class LB, class PA, class PB>
+__device__ __forceinline__ void tile_product(int64_t k_begin, int64_t k_end, LA load_a, LB load_b, PA put_a, PB put_b, f32x4 (&acc)[2][2]) {
+  __shared__ __attribute__((aligned(16))) float sa[2][BK][PM], sb[2][BK][PM];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int wm0 = (wave >> 1) * 32, wn0 = (wave & 1) * 32;
   for (int a = 0; a < 2; ++a)
     for (int b = 0; b < 2; ++b) acc[a][b] = f32x4{0.f, 0.f, 0.f, 0.f};
-  for (int64_t k0 = k_begin; k0 < k_end; k0 += BK) {
-    stage_a(sa, k0, k_end);
-    stage_b(sb, k0, k_end);
-    __syncthreads();
+  f32x4 va = load_a(k_begin, k_end), vb = load_b(k_begin, k_end);
+  int buf = 0;
+  for (int64_t k0 = k_begin; k0 < k_end; k0 += BK, buf ^= 1) {
+    put_a(sa[buf], va);
+    put_b(sb[buf], vb);
+    __syncthreads();                               // (the other buffer is written next, behind everybody's reads of it)
+    if (k0 + BK < k_end) {
+      va = load_a(k0 + BK, k_end);
+      vb = load_b(k0 + BK, k_end);
+    }
 #pragma unroll
     for (int k = 0; k < BK; k += 4) {
       float fa[2], fb[2];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        fa[i] = sa[k + (lane >> 4)][wm0 + 16 * i + (lane & 15)];
-        fb[i] = sb[k + (lane >> 4)][wn0 + 16 * i + (lane & 15)];
+        fa[i] = sa[buf][k + (lane >> 4)][wm0 + 16 * i + (lane & 15)];
+        fb[i] = sb[buf][k + (lane >> 4)][wn0 + 16 * i + (lane & 15)];
       }
 #pragma unroll
       for (int a = 0; a < 2; ++a)
 #pragma unroll
         for (int b = 0; b < 2; ++b) acc[a][b] = __builtin_amdgcn_mfma_f32_16x16x4f32(fb[b], fa[a], acc[a][b], 0, 0, 0);
     }
-    __syncthreads();
   }
 }
 
@@ -115,27 +121,23 @@ __global__ __launch_bounds__(NT) void linear_kernel(Linear q, int tiles_n) {
   // x: thread (m = tid / 4, k = 4 (tid % 4)); W: thread (k = tid / 16, n = 4 (tid % 16))
   const int64_t xrow = m0 + (tid >> 2);
   const T* xr = q.row_of<T>(xrow < q.rows ? xrow : q.rows - 1);
-  auto stage_x = [&](float (&s)[BK][PM], int64_t k0, int64_t k_end) {
+  auto load_x = [&](int64_t k0, int64_t k_end) {
     const int64_t k = k0 + (tid & 3) * 4;
-    f32x4 v = {0.f, 0.f, 0.f, 0.f};
-    if (xrow < q.rows) {
-      if (k < k_end) v = ld4(xr + k, k_end - k);
-    }
-    for (int l = 0; l < 4; ++l) s[(tid & 3) * 4 + l][tid >> 2] = v[l];
+    return xrow < q.rows && k < k_end ? ld4(xr + k, k_end - k) : f32x4{0.f, 0.f, 0.f, 0.f};
   };
-  auto stage_w = [&](float (&s)[BK][PM], int64_t k0, int64_t k_end) {
+  auto load_w = [&](int64_t k0, int64_t k_end) {
     const int64_t k = k0 + (tid >> 4);
     const int n = n0 + (tid & 15) * 4;
-    f32x4 v = {0.f, 0.f, 0.f, 0.f};
-    if (k < k_end) {
-      if (n < q.N) v = ld4(w + k * q.ldw + n, q.N - n);
-    }
-    *reinterpret_cast<f32x4*>(&s[tid >> 4][(tid & 15) * 4]) = v;
+    return k < k_end && n < q.N ? ld4(w + k * q.ldw + n, q.N - n) : f32x4{0.f, 0.f, 0.f, 0.f};
   };
+  auto put_x = [&](float (&s)[BK][PM], f32x4 v) {
+    for (int l = 0; l < 4; ++l) s[(tid & 3) * 4 + l][tid >> 2] = v[l];
+  };
+  auto put_w = [&](float (&s)[BK][PM], f32x4 v) { *reinterpret_cast<f32x4*>(&s[tid >> 4][(tid & 15) * 4]) = v; };
   if (q.own_t) shrink_rows<T>(q, m0, BM, NT);                         // (read behind the barriers that follow)
   f32x4 acc[2][2];
   const int64_t kb = (int64_t)split * q.k_per_split;
-  tile_product(kb, min((int64_t)q.K, kb + q.k_per_split), stage_x, stage_w, acc);
+  tile_product(kb, min((int64_t)q.K, kb + q.k_per_split), load_x, load_w, put_x, put_w, acc);
   const int lane = tid & 63, wave = tid >> 6;
 #pragma unroll
   for (int a = 0; a < 2; ++a)
@@ -285,29 +287,22 @@ __global__ __launch_bounds__(NT) void sum_kernel(Sum q, int tiles_n, int tiles) 
   const int tile = u / q.splits, split = u % q.splits;
   const int m0 = (tile / tiles_n) * BM, n0 = (tile % tiles_n) * BN;
   const int kk = tid >> 4, c = (tid & 15) * 4;
-  auto stage_a = [&](float (&s)[BK][PM], int64_t k0, int64_t k_end) {
+  auto load_a = [&](int64_t k0, int64_t k_end) {
     const int64_t k = k0 + kk;
-    f32x4 v = {0.f, 0.f, 0.f, 0.f};
-    if (k < k_end) {
-      const int64_t p = k / q.R;
-      const T* r = reinterpret_cast<const T*>(q.a) + p * q.sa + (k - p * q.R) * q.M + m0 + c;
-      if (m0 + c < q.M) v = q.w[p] * ld4(r, q.M - m0 - c);
-    }
-    *reinterpret_cast<f32x4*>(&s[kk][c]) = v;
+    if (k >= k_end || m0 + c >= q.M) return f32x4{0.f, 0.f, 0.f, 0.f};
+    const int64_t p = q.K <= 0xffffffffll ? (uint32_t)k / (uint32_t)q.R : k / q.R;
+    return q.w[p] * ld4(reinterpret_cast<const T*>(q.a) + p * q.sa + (k - p * q.R) * q.M + m0 + c, q.M - m0 - c);
   };
-  auto stage_b = [&](float (&s)[BK][PM], int64_t k0, int64_t k_end) {
+  auto load_b = [&](int64_t k0, int64_t k_end) {
     const int64_t k = k0 + kk;
-    f32x4 v = {0.f, 0.f, 0.f, 0.f};
-    if (k < k_end) {
-      const int64_t p = k / q.R;
-      const T* r = reinterpret_cast<const T*>(q.b) + p * q.sb + (k - p * q.R) * q.N + n0 + c;
-      if (n0 + c < q.N) v = ld4(r, q.N - n0 - c);
-    }
-    *reinterpret_cast<f32x4*>(&s[kk][c]) = v;
+    if (k >= k_end || n0 + c >= q.N) return f32x4{0.f, 0.f, 0.f, 0.f};
+    const int64_t p = q.K <= 0xffffffffll ? (uint32_t)k / (uint32_t)q.R : k / q.R;
+    return ld4(reinterpret_cast<const T*>(q.b) + p * q.sb + (k - p * q.R) * q.N + n0 + c, q.N - n0 - c);
   };
+  auto put = [&](float (&s)[BK][PM], f32x4 v) { *reinterpret_cast<f32x4*>(&s[kk][c]) = v; };
   f32x4 acc[2][2];
   const int64_t kb = split * q.k_per_split;
-  tile_product(kb, min(q.K, kb + q.k_per_split), stage_a, stage_b, acc);
+  tile_product(kb, min(q.K, kb + q.k_per_split), load_a, load_b, put, put, acc);
   const int lane = tid & 63, wave = tid >> 6;
 #pragma unroll
   for (int a = 0; a < 2; ++a)
@@ -434,9 +429,10 @@ int launch_sum(const Sum& q, hipStream_t s) {
   return last_launch_status();
 }
 
-// How many workgroups share one tile's K: enough that about two workgroups per compute unit run, but at least 128 products each.
+// How many workgroups share one tile's K: enough that about six run on each compute unit (a step waits for memory most of its time:
+// 71436 x 1944 x 25 took 520 us with two), but at least 128 products each.
 int64_t splits_for(int64_t tiles, int64_t K) {
-  int64_t s = (2 * kNumCU) / (tiles < 1 ? 1 : tiles);
+  int64_t s = (6 * kNumCU) / (tiles < 1 ? 1 : tiles);
   if (s > (K + 127) / 128) s = (K + 127) / 128;
   return s < 1 ? 1 : s;
 }

@@ -170,13 +170,12 @@ class OptaxWrapper(Stateful):
         return updates, state.replace(opt_state=opt_state)
 
     def step(self, state, grads, params):
-        """Parameters after the update: the optimizer's own whole step where it has one."""
-        fused = getattr(self.optimizer, "step", None)
-        if fused is not None:
-            params, opt_state = fused(grads, state.opt_state, params)
-        else:
-            updates, opt_state = self.optimizer.update(grads, state.opt_state, params)
-            params = apply_updates(params, updates)
+        """Parameters after the update: the optimizer's own whole step where it has one (and no subclass its own update)."""
+        fused = getattr(self.optimizer, "step", None) if type(self).update is OptaxWrapper.update else None
+        if fused is None:
+            updates, state = self.update(state, grads, params)
+            return apply_updates(params, updates), state
+        params, opt_state = fused(grads, state.opt_state, params)
         return params, state.replace(opt_state=opt_state)
 
 

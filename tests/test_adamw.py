@@ -366,6 +366,24 @@ def test_named_in_every_strategy():
     assert torch.equal(new, center + updates) and torch.equal(after.opt_state["mu"], after2.opt_state["mu"])
 
 
+def test_step_of_a_wrapper_with_its_own_update():
+    """A wrapper that changes the updates keeps its change in the strategies, whatever optimizer it holds."""
+    class Halved(optimizers.OptaxWrapper):
+        def update(self, state, grads, params=None):
+            updates, state = super().update(state, grads, params)
+            return 0.5 * updates, state
+
+    center = torch.linspace(-1, 1, 6)
+    for make_one in (optimizers.adam, optimizers.adamw):
+        wrapper = Halved(make_one(0.1), center)
+        state = wrapper.init(PRNGKey(0))
+        updates, _ = wrapper.update(state, torch.ones(6), center)
+        plain, _ = make_one(0.1).update(torch.ones(6), make_one(0.1).init(center), center)
+        assert torch.equal(updates, 0.5 * plain)
+        new, _ = wrapper.step(state, torch.ones(6), center)
+        assert torch.equal(new, center + updates)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("bits", [32, 8])
 def test_recorded_step(cuda, bits):

@@ -71,7 +71,7 @@ void launch_pack(const Rows& q, T* out, hipStream_t s) {
   int64_t g = (pieces + NT - 1) / NT;
   pack_kernel<T><<<(unsigned)(g < 32 * kNumCU ? (g < 1 ? 1 : g) : 32 * kNumCU), NT, 0, s>>>(q, out);
 }
-int up16(int cols, int elem) { return (cols * elem + 15) / 16 * 16 / elem; }
+int up16(int cols, int elem) { return (int)(((int64_t)cols * elem + 15) / 16 * 16 / elem); }
 
 // acc[a][b][i] = C[wm0 + 16 a + (lane & 15)][wn0 + 16 b + 4 (lane >> 4) + i] of the tile, given its operands: load_a(k0, k_end) and
 // load_b(k0, k_end) return this thread's four elements of the step's tiles (zero outside), put_a and put_b place them in LDS.
@@ -488,7 +488,7 @@ static int linear_call(const void* x, const void* w, const void* a, const void* 
   } else if (q.rows <= 16 && x16 && w16 && (int64_t)q.K * q.N >= 1 << 16) {
     path = Path::kMfma;
     linear_mfma_plan(q, el);
-  } else if (q.rows > 16 && q.K * el >= 128) {
+  } else if (q.rows > 16 && (int64_t)q.K * el >= 128) {
     // The tiles of lowrank_mfma.hip take rows of whole 16-byte pieces; others are copied first, where that takes less time than is
     // gained: the tiles of any alignment reach about 60 TFLOP/s (a column of tiles is 64 wide), these about 100 in float32 and
     // 300 and more in bf16; a copy reads and writes at 4 TB/s and costs a launch.  Grouped tiles also save the pass over x for t.

@@ -29,7 +29,7 @@ _native.register_hip_api({
 _ACT = {"identity": 0, "tanh": 1, "relu": 2, "sigmoid": 3}
 _ACT_FN = {"identity": lambda v: v, "tanh": torch.tanh, "relu": torch.relu, "sigmoid": torch.sigmoid}
 _INDEX = {torch.int32: 1, torch.int64: 2}
-_MOST = 2 ** 31 - 1
+_MOST = 2 ** 31 - 2 ** 16          # features are indexed in 32 bits, up to the end of the last tile
 
 
 def _check_factors(what, a, b):
@@ -47,8 +47,8 @@ def _check_factors(what, a, b):
         raise TypeError(f"{what}: the factors have different types, {a.dtype} and {b.dtype}")
     if sa[2] < 1:
         raise ValueError(f"{what} needs at least one input feature")
-    if r > _MOST or sa[2] > _MOST or sb[2] > _MOST:
-        raise ValueError(f"{what}: a factor's rank and features lie below 2^31")
+    if r >= _MOST or sa[2] >= _MOST or sb[2] >= _MOST:
+        raise ValueError(f"{what}: a factor's rank and features lie below 2^31 - 2^16")
     return r, sb[1] - r
 
 

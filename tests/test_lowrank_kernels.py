@@ -1,0 +1,69 @@
+"""The low-rank kernels where they are large: workspaces, launches, precision, and every variant that a size chooses."""
+import ctypes
+import math
+
+import pytest
+import torch
+
+from evox_amd import _native
+from evox_amd._native import build
+from evox_amd.ops.lowrank import lowrank_linear, lowrank_weighted_sum
+from test_lowrank import DEVICES, DTYPES, U, check_linear, check_sum, layer, randn
+
+needs_library = pytest.mark.skipif(not (build.HIP_LIB.exists() or build.have_hipcc()), reason="no kernel library")
+
+
+# ------------------------------------------------------------------ what a call asks for, on the host (nothing is launched)
+
+def host_call(dims, ints):
+    """The arguments of an entry point up to its sizes, with addresses that are never read."""
+    at = 1 << 40
+    return at, (ctypes.c_int64 * len(dims))(*dims), (ctypes.c_int * len(ints))(*ints)
+
+
+def linear_workspace(rows, n_in, n_out, r, dtype=torch.float32, pop=1, per=1):
+    at, dims, ints = host_call((rows, pop, per, per * n_in, n_in, r * n_in, r * n_out), (n_in, n_out, r, 0, 0, int(dtype == torch.bfloat16), 0))
+    return _native.hip().evox_hip_lowrank_linear_ws(at, at, at, at, None, None, at, ctypes.addressof(dims), ctypes.addressof(ints))
+
+
+def sum_workspace(pop, n_in, n_out, r, dtype=torch.float32):
+    at, dims, ints = host_call((pop, r * n_in, r * n_out), (n_in, n_out, r, int(dtype == torch.bfloat16)))
+    return _native.hip().evox_hip_lowrank_sum_ws(at, at, at, at, None, ctypes.addressof(dims), ctypes.addressof(ints))
+
+
+@needs_library
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_workspace_of_wide_rows(dtype):
+    """Rows of 2^31 bytes and more that are copied to aligned ones have room for their copies."""
+    size = torch.finfo(dtype).bits // 8
+    for n in (2 ** 31 // size - 5, 2 ** 31 // size + 1, 2 ** 30 + 1):
+        assert linear_workspace(17, n, 1024, 1, dtype, pop=17) >= 17 * n * size // 4
+        assert sum_workspace(64, n, 256, 1, dtype) >= 64 * n * size // 4
+        assert sum_workspace(64, 256, n, 1, dtype) >= 64 * n * size // 4
+
+
+def test_refuses_features_near_2_to_31():
+    """Tiles are counted in 32 bits beyond a tensor's last feature."""
+    n = 2 ** 31 - 2 ** 16
+    one = torch.zeros(1, 1, 1)
+    wide, weight = one.expand(1, 1, n), torch.zeros(1, 1).expand(n, 1)
+    with pytest.raises(ValueError, match="2\\^31"):
+        lowrank_linear(wide, weight, wide, one)
+    with pytest.raises(ValueError, match="2\\^31"):
+        lowrank_linear(one, weight.t(), one, wide)
+    with pytest.raises(ValueError, match="2\\^31"):
+        lowrank_weighted_sum(torch.zeros(1), wide, one)
+
+
+@pytest.mark.gpu
+def test_copied_rows_beyond_2_to_31_bytes(cuda):
+    """17 rows (one, expanded) of 2^30 + 1 bf16 inputs, copied to aligned rows of 2 GiB each; all but a few inputs are zero."""
+    n = 2 ** 30 + 1
+    at = torch.tensor([0, 1, 7, 8, 2 ** 29 + 3, 2 ** 30 - 1, 2 ** 30], device=cuda)
+    gen = torch.Generator().manual_seed(29)
+    few = [randn(gen, 1, 7, dtype=torch.bfloat16).to(cuda), randn(gen, 7, 8, dtype=torch.bfloat16).to(cuda), randn(gen, 1, 1, 7, dtype=torch.bfloat16).to(cuda)]
+    x, weight, a = (torch.zeros(s, dtype=torch.bfloat16, device=cuda) for s in ((1, n), (n, 8), (1, 1, n)))
+    x[:, at], weight[at], a[:, :, at] = few
+    b = randn(gen, 1, 1, 8, dtype=torch.bfloat16).to(cuda)
+    y = lowrank_linear(x.expand(17, n), weight, a.expand(17, 1, n), b.expand(17, 1, 8))
+    check_linear(y, few[0].expand(17, 7), few[1], few[2].expand(17, 1, 7), b.expand(17, 1, 8))

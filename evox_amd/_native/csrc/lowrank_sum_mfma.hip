@@ -133,7 +133,7 @@ __global__ __launch_bounds__(WM* WN * 64) void sum_mfma_kernel(Sum q, int tiles,
   const int pstep = BK / q.R, jstep = BK % q.R;
   const int64_t da = (pstep * q.sa + (int64_t)jstep * q.lda) * sizeof(T), wrap_a = (q.sa - (int64_t)q.R * q.lda) * sizeof(T);
   const int64_t db = (pstep * q.sb + (int64_t)jstep * q.ldb) * sizeof(T), wrap_b = (q.sb - (int64_t)q.R * q.ldb) * sizeof(T);
-  const int left = (int)min(ke - kb, (int64_t)0x7fffffff);            // k of this split
+  const int left = (int)(ke - kb);                                    // k of this split
   const char *pa[AI], *pb[AI];
   int kr[AI], jr[AI];
 #pragma unroll
@@ -322,7 +322,8 @@ bool big_tiles(const Sum& q, int elem) { return elem == 2 && (int64_t)((q.M + 25
 namespace evox {
 namespace lr {
 
-// K is split so that the chip is filled once (256 x 256: one workgroup a compute unit, else two); a split has 128 k at least.
+// K is split so that the chip is filled once (256 x 256: one workgroup a compute unit, else two); a split has 128 k at least, and
+// 2^30 at most: the kernel counts a split's k in 32 bits.
 void sum_mfma_plan(Sum& q, int elem) {
   const bool big = big_tiles(q, elem);
   const int bk = 64 / elem;
@@ -330,7 +331,8 @@ void sum_mfma_plan(Sum& q, int elem) {
   int64_t s = (big ? kNumCU : 2 * kNumCU) / tiles;
   const int64_t most = (q.K + 127) / 128;
   if (s > most) s = most;
-  if (s < 1) s = 1;
+  const int64_t least = (q.K + (1 << 30) - 1) >> 30;
+  if (s < least) s = least;
   const int64_t per = (q.K + s - 1) / s;
   q.k_per_split = (per + bk - 1) / bk * bk;
   q.splits = (int)((q.K + q.k_per_split - 1) / q.k_per_split);

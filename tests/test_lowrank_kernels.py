@@ -42,6 +42,16 @@ def test_workspace_of_wide_rows(dtype):
         assert sum_workspace(64, 256, n, 1, dtype) >= 64 * n * size // 4
 
 
+@needs_library
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_long_sums_are_divided(dtype):
+    """A workgroup counts its terms in 32 bits: sums of more than 2^31 terms are divided (each part has its partial sums) even where
+    the outputs alone fill the chip."""
+    for pop in (2 ** 31, 2 ** 31 + 17, 2 ** 33):
+        assert sum_workspace(pop, 8192, 8192, 1, dtype) >= pop // 2 ** 30 * 8193 * 8192
+    assert sum_workspace(2 ** 30, 8192, 8192, 1, dtype) == 0
+
+
 def test_refuses_features_near_2_to_31():
     """Tiles are counted in 32 bits beyond a tensor's last feature."""
     n = 2 ** 31 - 2 ** 16

@@ -234,15 +234,24 @@ __device__ __forceinline__ void shrink_rows(const Linear& q, int64_t row0, int n
   const int64_t first = row0 * chunks, end = min(row0 + n, q.rows) * chunks;
   for (int64_t i = first; i < end; i += per) shrink_items<T, 4>(q, i, end, threads);
 }
-template <typename T>
-__device__ __forceinline__ void shrink_block(const Linear& q, int64_t block, int threads) {
-  const int64_t first = block * (threads / shrink_lanes(q, sizeof(T)));
-  if (shrink_factors(q) == 1) shrink_items<T, 1>(q, first, q.rows * q.R, threads);
-  else shrink_items<T, 4>(q, first, q.rows * ((q.R + 3) / 4), threads);
+// all entries, by `blocks` workgroups
+template <typename T, int JC>
+__device__ __forceinline__ void shrink_share(const Linear& q, int64_t block, int64_t blocks, int threads) {
+  const int per = threads / shrink_lanes(q, sizeof(T));
+  const int64_t end = q.rows * ((q.R + JC - 1) / JC);
+  for (int64_t first = block * per; first < end; first += blocks * per) shrink_items<T, JC>(q, first, end, threads);
 }
+template <typename T>
+__device__ __forceinline__ void shrink_block(const Linear& q, int64_t block, int64_t blocks, int threads) {
+  if (shrink_factors(q) == 1) shrink_share<T, 1>(q, block, blocks, threads);
+  else shrink_share<T, 4>(q, block, blocks, threads);
+}
+// workgroups for all entries: one pass each, up to a number that any launch holds
+constexpr int64_t kShrinkMost = 1 << 22;
 inline int64_t shrink_blocks(const Linear& q, int elem, int threads) {
-  const int jc = shrink_factors(q);
-  return (q.rows * ((q.R + jc - 1) / jc) * shrink_lanes(q, elem) + threads - 1) / threads;
+  const int jc = shrink_factors(q), per = threads / shrink_lanes(q, elem);
+  const int64_t blocks = (q.rows * ((q.R + jc - 1) / jc) + per - 1) / per;
+  return blocks < kShrinkMost ? blocks : kShrinkMost;
 }
 
 // One weighted sum.  K = pop * R products; k stands for individual k / R and row k % R of its factors.

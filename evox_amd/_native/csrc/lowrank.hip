@@ -14,7 +14,7 @@ bool linear_mfma_grouped(const Linear& q);                       // lowrank_mfma
 void linear_mfma_plan(Linear& q, int elem);
 int linear_mfma_side(const Linear& q, int elem);
 template <typename T>
-int linear_mfma(const Linear& q, bool grouped, hipStream_t s);
+int linear_mfma(const Linear& q, bool grouped, hipStream_t s, int* tile = nullptr);
 void sum_mfma_plan(Sum& q, int elem);                            // lowrank_sum_mfma.hip
 int sum_mfma(const Sum& q, int elem, hipStream_t s);
 }  // namespace lr
@@ -27,7 +27,7 @@ constexpr int PM = BM + 4;                         // LDS pitch: the four rows o
 
 template <typename T>
 __global__ __launch_bounds__(NT) void shrink_kernel(Linear q) {
-  shrink_block<T>(q, blockIdx.x, NT);
+  shrink_block<T>(q, blockIdx.x, gridDim.x, NT);
 }
 
 // Rows that start or end off 16 bytes, copied to rows of `ld` elements (a multiple of 16 bytes) that do not, with zeros behind their
@@ -189,7 +189,7 @@ __global__ __launch_bounds__(FEW_NT) void linear_few_kernel(Linear q, int shrink
   __shared__ __attribute__((aligned(16))) float red[PAIR][8][COLS];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   if ((int)blockIdx.x < shrink) {
-    shrink_block<T>(q, blockIdx.x, FEW_NT);
+    shrink_block<T>(q, blockIdx.x, shrink, FEW_NT);
     return;
   }
   const int u = (int)blockIdx.x - shrink;
@@ -361,6 +361,9 @@ struct Layout {
   int64_t t = 0, slab = 0, x = 0, w = 0, a = 0, floats = 0;
 };
 
+// workgroups of the any-size tiles
+int64_t tile_workgroups(const Linear& q) { return (q.rows + BM - 1) / BM * ((q.N + BN - 1) / BN) * q.splits; }
+
 template <typename T>
 int launch_linear(Linear q, Path path, const Layout& at, float* ws, hipStream_t s) {
   q.t = ws + at.t;
@@ -372,7 +375,6 @@ int launch_linear(Linear q, Path path, const Layout& at, float* ws, hipStream_t 
     else linear_join_kernel<T><<<stream_grid(quads, NT), NT, 0, s>>>(q);
   };
   auto shrink = [&]() { shrink_kernel<T><<<(unsigned)shrink_blocks(q, sizeof(T), NT), NT, 0, s>>>(q); };
-  if (!fits_launch(shrink_blocks(q, sizeof(T), NT), NT)) return (int)hipErrorInvalidValue;
   if (path == Path::kFew) {
     constexpr int COLS = 64 * 16 / (int)sizeof(T);
     const int first = (int)shrink_blocks(q, sizeof(T), FEW_NT);
@@ -411,9 +413,7 @@ int launch_linear(Linear q, Path path, const Layout& at, float* ws, hipStream_t 
   }
   if (!q.own_t) shrink();
   const int tiles_n = (q.N + BN - 1) / BN;
-  const int64_t wgs = (q.rows + BM - 1) / BM * tiles_n * q.splits;
-  if (!fits_launch(wgs, NT)) return (int)hipErrorInvalidValue;
-  linear_kernel<T><<<(unsigned)wgs, NT, 0, s>>>(q, tiles_n);
+  linear_kernel<T><<<(unsigned)tile_workgroups(q), NT, 0, s>>>(q, tiles_n);
   if (q.splits > 1) join();
   return last_launch_status();
 }
@@ -524,11 +524,14 @@ static int linear_call(const void* x, const void* w, const void* a, const void* 
   at.x = copy(at.pack_x, q.rows, q.K);
   at.w = copy(at.pack_w, q.K, q.N);
   at.a = copy(at.pack_a, q.pop * q.R, q.K);
-  return 0;
+  if (path == Path::kTile) return fits_launch(tile_workgroups(q), NT) ? 0 : (int)hipErrorInvalidValue;
+  if (path == Path::kFew) return 0;
+  int tile;
+  return el == 2 ? linear_mfma<uint16_t>(q, path == Path::kGrouped, nullptr, &tile) : linear_mfma<float>(q, path == Path::kGrouped, nullptr, &tile);
 }
 
-// Floats of workspace that the same call of evox_hip_lowrank_linear takes (negative: the call is refused): t and the partial
-// products.  dims: rows, pop, per, sx0, sx1, sa, sb.  ints: K, N, R, own_bias, act, dtype (0 fp32, 1 bf16), index type (0 none,
+// Floats of workspace that the same call of evox_hip_lowrank_linear takes (negative: the call is refused, y has more tiles than a
+// launch holds): t and the partial products.  dims: rows, pop, per, sx0, sx1, sa, sb.  ints: K, N, R, own_bias, act, dtype (0 fp32, 1 bf16), index type (0 none,
 // 1 int32, 2 int64)
 EVOX_API int64_t evox_hip_lowrank_linear_ws(const void* x, const void* w, const void* a, const void* b, const float* bias,
                                             const void* index, void* y, const int64_t* dims, const int* ints) {

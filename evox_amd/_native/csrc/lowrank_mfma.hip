@@ -89,7 +89,7 @@ __global__ __launch_bounds__(WM* WN * 64) void linear_mfma_kernel(Linear q, Tile
   if constexpr (!GROUPED) {
     // t, where it is wanted only by linear_join_kernel; in front, so that none of it is left when the products are done
     if ((int)blockIdx.x < g.shrink) {
-      shrink_block<T>(q, (int)blockIdx.x, NW * 64);
+      shrink_block<T>(q, (int)blockIdx.x, g.shrink, NW * 64);
       return;
     }
   }
@@ -441,8 +441,9 @@ __global__ __launch_bounds__(WM* WN * 64) void linear_mfma_kernel(Linear q, Tile
   }
 }
 
+// (with `tile` nothing is launched: it receives the tile's rows, the status tells whether the launch would be refused)
 template <typename T, int BM, int BN, int WM, int WN, int STAGES, int SLOTS>
-int launch(const Linear& q, hipStream_t s) {
+int launch(const Linear& q, hipStream_t s, int* tile) {
   constexpr int LDS = STAGES * stage_bytes(BM, BN, WM * WN, SLOTS);
   Tiles g{};
   g.tiles_n = (q.N + BN - 1) / BN;
@@ -453,6 +454,10 @@ int launch(const Linear& q, hipStream_t s) {
   const int64_t shrink = !SLOTS && (BM == 16 || q.splits > 1) ? (shrink_blocks(q, sizeof(T), WM * WN * 64) + kNumXCD - 1) / kNumXCD * kNumXCD : 0;
   wgs += shrink;
   if (!fits_launch(wgs, WM * WN * 64)) return (int)hipErrorInvalidValue;
+  if (tile != nullptr) {
+    *tile = BM;
+    return 0;
+  }
   g.shrink = (int)shrink;
   constexpr auto kernel = &linear_mfma_kernel<T, BM, BN, WM, WN, STAGES, SLOTS>;
   if (const int st = allow_lds<kernel>(LDS)) return st;
@@ -501,22 +506,22 @@ void linear_mfma_plan(Linear& q, int elem) {
 }
 
 template <typename T>
-int linear_mfma(const Linear& q, bool grouped, hipStream_t s) {
+int linear_mfma(const Linear& q, bool grouped, hipStream_t s, int* tile) {
   const int side = linear_mfma_side(q, sizeof(T));
   if (grouped) {
     // a tile of 256 rows holds A_p of eight individuals: 16 / each meet in it where they start together, else up to two more
     const int64_t each = (q.per + 15) / 16, meet = 16 % each == 0 ? 16 / each : 16 / each + 2;
     if constexpr (sizeof(T) == 2)
-      if (side == 256 && meet <= 8) return launch<T, 256, 256, 2, 4, 4, 8>(q, s);
-    return side >= 128 ? launch<T, 128, 128, 2, 2, 3, 8>(q, s) : launch<T, 64, 64, 2, 2, 4, 4>(q, s);
+      if (side == 256 && meet <= 8) return launch<T, 256, 256, 2, 4, 4, 8>(q, s, tile);
+    return side >= 128 ? launch<T, 128, 128, 2, 2, 3, 8>(q, s, tile) : launch<T, 64, 64, 2, 2, 4, 4>(q, s, tile);
   }
-  if (q.rows <= 16) return launch<T, 16, 128, 1, 4, 4, 0>(q, s);
+  if (q.rows <= 16) return launch<T, 16, 128, 1, 4, 4, 0>(q, s, tile);
   if constexpr (sizeof(T) == 2)
-    if (side == 256) return launch<T, 256, 256, 2, 4, 4, 0>(q, s);
-  return side >= 128 ? launch<T, 128, 128, 2, 2, 3, 0>(q, s) : launch<T, 64, 64, 2, 2, 4, 0>(q, s);
+    if (side == 256) return launch<T, 256, 256, 2, 4, 4, 0>(q, s, tile);
+  return side >= 128 ? launch<T, 128, 128, 2, 2, 3, 0>(q, s, tile) : launch<T, 64, 64, 2, 2, 4, 0>(q, s, tile);
 }
-template int linear_mfma<uint16_t>(const Linear&, bool, hipStream_t);
-template int linear_mfma<float>(const Linear&, bool, hipStream_t);
+template int linear_mfma<uint16_t>(const Linear&, bool, hipStream_t, int*);
+template int linear_mfma<float>(const Linear&, bool, hipStream_t, int*);
 
 }  // namespace lr
 }  // namespace evox

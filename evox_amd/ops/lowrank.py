@@ -77,7 +77,8 @@ def lowrank_linear(x: torch.Tensor, weight: torch.Tensor, a: torch.Tensor, b: to
 
     ``x``, ``weight``, ``a``, ``b`` are all float32 or all bfloat16; sums are float32 and the result is rounded once.  ``x`` may be
     strided or expanded over individuals, the factors may be views of wider rows (``MLP.lowrank_factors``).  No autograd graph
-    is built: inputs that ask for a gradient are refused."""
+    is built: inputs that ask for a gradient are refused, and so is a y of 2^24 tiles or more, which are 64 x 64 at least (2^30 rows of up
+    to 64 outputs)."""
     r, own_bias = _check_factors("lowrank_linear", a, b)
     if weight.dim() != 2 or weight.shape[0] != a.shape[2] or weight.shape[1] != b.shape[2]:
         raise ValueError(f"lowrank_linear: a weight of shape {tuple(weight.shape)} does not fit factors of {a.shape[2]} inputs and "
@@ -130,6 +131,8 @@ def lowrank_linear(x: torch.Tensor, weight: torch.Tensor, a: torch.Tensor, b: to
     call = (x.data_ptr(), weight.data_ptr(), a.data_ptr(), b.data_ptr(), None if bias is None else bias.data_ptr(),
             None if index is None else index.data_ptr(), y.data_ptr(), ctypes.addressof(dims), ctypes.addressof(ints))
     floats = lib.evox_hip_lowrank_linear_ws(*call)
+    if floats < 0:
+        raise ValueError(f"lowrank_linear: {rows} rows of {n_out} outputs are more tiles than one launch holds (2^24 of 64 x 64)")
     ws = x.new_empty(floats, dtype=torch.float32) if floats > 0 else None
     with launch_device(dev):
         check(lib.evox_hip_lowrank_linear(*call, None if ws is None else ws.data_ptr(), floats, float(scale), stream_of(y)), "lowrank_linear")

@@ -77,3 +77,37 @@ def test_copied_rows_beyond_2_to_31_bytes(cuda):
     b = randn(gen, 1, 1, 8, dtype=torch.bfloat16).to(cuda)
     y = lowrank_linear(x.expand(17, n), weight, a.expand(17, 1, n), b.expand(17, 1, 8))
     check_linear(y, few[0].expand(17, 7), few[1], few[2].expand(17, 1, 7), b.expand(17, 1, 8))
+
+
+# ------------------------------------------------------------------ launches
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("grouped", [True, False])
+def test_more_rows_than_threads_of_one_launch(cuda, grouped):
+    """16.8 M rows of rank 16 (all of them one individual's 256, expanded): sixty-four lanes for each four of a row's entries of t
+    are more threads than a launch counts."""
+    gen = torch.Generator().manual_seed(31)
+    n_in, n_out, r, per, pop = 264, 72, 16, 256, 65537
+    weight, a, b = layer(gen, 1, n_in, n_out, r, 1, torch.bfloat16, cuda)
+    x = randn(gen, 1, per, n_in, dtype=torch.bfloat16).to(cuda)
+    if grouped:
+        want = lowrank_linear(x, weight, a, b, activation="tanh")
+        y = lowrank_linear(x.expand(pop, per, n_in), weight, a.expand(pop, -1, -1), b.expand(pop, -1, -1), activation="tanh")
+        check_linear(y[-1:], x, weight, a, b, activation="tanh")
+        assert torch.equal(y, y[-1:].expand(pop, per, n_out)) and torch.allclose(y[:1].float(), want.float(), atol=0.02)
+    else:
+        x = x[0, :1].expand(pop * per, n_in)
+        index = torch.zeros(pop * per, dtype=torch.int32, device=cuda)
+        y = lowrank_linear(x, weight, a, b, index=index, activation="tanh")
+        check_linear(y[-3:], x[-3:], weight, a, b, index=index[-3:], activation="tanh")
+        assert torch.equal(y, y[-1:].expand(pop * per, n_out))
+
+
+@needs_library
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_launches_of_many_rows(dtype):
+    """Any number of rows whose tiles fit a launch, whatever their rank; 2^24 tiles and more are refused."""
+    for r in (1, 16, 64, 20000):
+        assert linear_workspace(2 ** 24, 264, 72, r, dtype, pop=2 ** 16, per=2 ** 8) >= 0
+        assert linear_workspace(2 ** 28, 8, 8, r, dtype, pop=2 ** 28) >= 0
+        assert linear_workspace(2 ** 30 + 64, 8, 8, r, dtype, pop=2 ** 30 + 64) < 0

@@ -4,14 +4,14 @@
 // permuted by the row) and are read transposed (bf16: ds_read_b64_tr_b16; float32: four words), so no transposed copy of the
 // factors is made.  Float32 factors are multiplied by their weight as they are read.
 // bf16: the weights are float32 and so is the result, so w a must not be rounded to the factors' 8 bits: it is formed in float32
-// after the fragment is in registers and split into bf16 planes by rounding, hi + mid (+ lo), each multiplied by b with one
-// matrix instruction.  Two planes hold w a to 2^-18 (deviation 1.5e-6 of it at random mantissas), three to 2^-26.  Sums of
-// 16384 terms or more take two: the float32 accumulation of such sums leaves more than that by itself (1.6e-6 of the result at
-// 16384 random terms, 4.6e-6 at 65536), and a third plane costs half as much time again.
+// after the fragment is in registers and split into three bf16 planes by rounding, hi + mid + lo, which hold it to 2^-26; each is
+// multiplied by b with one matrix instruction.  (Two planes hold it to 2^-18 and take two thirds of the time.  However long the sum,
+// they left 2.5e-6 of it, where float32 leaves 4e-7 or, with few weights that are not zero, 6e-8.)
 // The wavefronts of a workgroup are laid out so that each splits few fragments of A and uses each split for many of B.
-// K = 65536, 2048 x 2048 bf16: 925 to 975 us (1.15 PFLOP/s of plane products; a library product of this card reaches 1.10 at 8192^3,
-// the tensor form takes 4040 us); K = 16384, 1024 x 720: 71 us; the latter in float32: 247 us.  A factor that is not finite makes
-// its row or column not finite (an infinite bf16 factor: NaN where the exact sum would be infinite).
+// K = 65536, 2048 x 2048 bf16: 1230 us (1.34 PFLOP/s of plane products; a library product of this card reaches 1.10 at 8192^3, the
+// tensor form takes 4040 us); K = 16384, 1024 x 720: 84 us; the latter in float32: 247 us.  A factor that is not finite makes
+// its row or column not finite (an infinite bf16 factor: NaN where the exact sum would be infinite, and so does a product w a of
+// 3.39e38 or more, bfloat16's largest value).
 // K is divided over as many workgroups as fill the chip; the partial sums are added by sum_join_kernel in a fixed order.
 #include "lowrank.h"
 #include "lowrank_tile.h"
@@ -98,9 +98,9 @@ __device__ __forceinline__ void split_planes(const bf16x8 f, const float (&w)[8]
   for (int p = 0; p < PLANES; ++p) out[p] = __builtin_bit_cast(bf16x8, make_uint4(o[p][0], o[p][1], o[p][2], o[p][3]));
 }
 
-template <typename T, int BM, int BN, int WM, int WN, int STAGES, int PLANES>
+template <typename T, int BM, int BN, int WM, int WN, int STAGES>
 __global__ __launch_bounds__(WM* WN * 64) void sum_mfma_kernel(Sum q, int tiles, int tiles_n) {
-  constexpr int NW = WM * WN;
+  constexpr int NW = WM * WN, PLANES = sizeof(T) == 2 ? 3 : 1;
   constexpr int TM = BM / WM / 16, TN = BN / WN / 16;
   constexpr bool BF = sizeof(T) == 2;
   constexpr int BK = 64 / sizeof(T), ROW = BM * (int)sizeof(T);        // k of a step, bytes of a row of a tile
@@ -127,7 +127,7 @@ __global__ __launch_bounds__(WM* WN * 64) void sum_mfma_kernel(Sum q, int tiles,
 
   // This lane's rows.  The factors of an individual lie apart from the next one's: a row's address moves on by a fixed amount per
   // step and by what lies between two individuals whenever its rank row wraps.
-  static_assert(1024 % ROW == 0 && AI == BI && (BF || PLANES == 1), "whole rows per wave-instruction");
+  static_assert(1024 % ROW == 0 && AI == BI, "whole rows per wave-instruction");
   const T* A = reinterpret_cast<const T*>(q.a);
   const T* B = reinterpret_cast<const T*>(q.b);
   const int pstep = BK / q.R, jstep = BK % q.R;
@@ -300,14 +300,14 @@ __global__ __launch_bounds__(WM* WN * 64) void sum_mfma_kernel(Sum q, int tiles,
     }
 }
 
-template <typename T, int BM, int WM, int WN, int STAGES, int PLANES>
+template <typename T, int BM, int WM, int WN, int STAGES>
 int launch(const Sum& q, hipStream_t s) {
   constexpr int LDS = STAGES * (2 * BM * 64 + WM * WN * 256);
   const int tiles_n = (q.N + BM - 1) / BM;
   const int64_t tiles = (int64_t)((q.M + BM - 1) / BM) * tiles_n;
   const int64_t wgs = (tiles + (q.gb != nullptr ? (q.N + 63) / 64 : 0)) * q.splits;
   if (!fits_launch(wgs, WM * WN * 64)) return (int)hipErrorInvalidValue;
-  constexpr auto kernel = &sum_mfma_kernel<T, BM, BM, WM, WN, STAGES, PLANES>;
+  constexpr auto kernel = &sum_mfma_kernel<T, BM, BM, WM, WN, STAGES>;
   if (const int st = allow_lds<kernel>(LDS)) return st;
   kernel<<<(unsigned)wgs, WM * WN * 64, LDS, s>>>(q, (int)tiles, tiles_n);
   return last_launch_status();
@@ -339,10 +339,8 @@ void sum_mfma_plan(Sum& q, int elem) {
 }
 
 int sum_mfma(const Sum& q, int elem, hipStream_t s) {
-  if (elem == 4) return launch<float, 128, 2, 2, 4, 1>(q, s);
-  const bool two = q.K >= 16384;
-  if (big_tiles(q, elem)) return two ? launch<uint16_t, 256, 4, 2, 4, 2>(q, s) : launch<uint16_t, 256, 4, 2, 4, 3>(q, s);
-  return two ? launch<uint16_t, 128, 2, 2, 4, 2>(q, s) : launch<uint16_t, 128, 2, 2, 4, 3>(q, s);
+  if (elem == 4) return launch<float, 128, 2, 2, 4>(q, s);
+  return big_tiles(q, elem) ? launch<uint16_t, 256, 4, 2, 4>(q, s) : launch<uint16_t, 128, 2, 2, 4>(q, s);
 }
 
 }  // namespace lr

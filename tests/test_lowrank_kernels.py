@@ -111,3 +111,58 @@ def test_launches_of_many_rows(dtype):
         assert linear_workspace(2 ** 24, 264, 72, r, dtype, pop=2 ** 16, per=2 ** 8) >= 0
         assert linear_workspace(2 ** 28, 8, 8, r, dtype, pop=2 ** 28) >= 0
         assert linear_workspace(2 ** 30 + 64, 8, 8, r, dtype, pop=2 ** 30 + 64) < 0
+
+
+# ------------------------------------------------------------------ precision of the weighted sum
+
+PRECISION = [(16384, 136, 130, 1), (4096, 1024, 720, 4), (16384, 512, 520, 1), (20000, 256, 128, 3)]   # individuals, in, out, rank
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", PRECISION, ids=str)
+def test_sums_of_few_weights_keep_their_precision(device, dtype, shape):
+    """Weights that are zero for all individuals but n (truncation, elites) leave n r terms and their roundings, however long the sum is.
+
+    A term's factors: w a is rounded once and b multiplies it exactly or with one more rounding; each of at most three parts of it is
+    added to the running sum, U of that at most whichever way it rounds, and the scale rounds once.  One individual: at most
+    3 r + 3 roundings of the terms' magnitudes, entry by entry.  16 individuals: an instruction may round once for each term of
+    its step, 24 n times in all; the running sums of signed terms grow with the root of their number, so these errors add up to
+    U sqrt(24 n / 6) of the result in norm, and 3 U for the rest."""
+    pop, n_in, n_out, r = shape
+    gen = torch.Generator().manual_seed(sum(shape))
+    _, a, b = layer(gen, pop, n_in, n_out, r, 1, dtype, device)
+    for n in (1, 16):
+        w = torch.zeros(pop)
+        at = torch.randperm(pop, generator=gen)[:n]
+        w[at] = randn(gen, n)
+        g, gb = lowrank_weighted_sum(w.to(device), a, b, scale=0.7)
+        w64, a64, b64 = w[at].double(), a.cpu()[at].double(), b.cpu()[at].double()
+        terms = 0.7 * w64[:, None, None, None] * a64[..., None] * b64[:, :r, None, :]
+        want, mag = terms.sum((0, 1)), terms.abs().sum((0, 1))
+        err = (g.cpu().double() - want).abs()
+        if n == 1:
+            assert bool((err <= (3 * r + 3) * U * mag).all()), float((err / mag).max() / U)
+        else:
+            assert float(err.norm()) <= U * (math.sqrt(4 * n) + 3) * float(want.norm()), float(err.norm() / want.norm() / U)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", PRECISION, ids=str)
+def test_long_sums_are_as_precise_as_the_tensor_form(cuda, dtype, shape):
+    """100 weights and all of them: off by half as much again as one float32 matrix product, and 4 U for the three parts."""
+    pop, n_in, n_out, r = shape
+    gen = torch.Generator().manual_seed(sum(shape) + 1)
+    _, a, b = layer(gen, pop, n_in, n_out, r, 0, dtype, cuda)
+    for n in (100, pop):
+        w = torch.zeros(pop)
+        at = torch.randperm(pop, generator=gen)[:n]
+        w[at] = randn(gen, n)
+        w = w.to(cuda)
+        aw = (a.double() * w.double()[:, None, None]).reshape(-1, n_in)
+        want = aw.T.contiguous() @ b.double().reshape(-1, n_out)
+        plain = (a.float() * w[:, None, None]).reshape(-1, n_in).T.contiguous() @ b.float().reshape(-1, n_out)
+        got, _ = lowrank_weighted_sum(w, a, b)
+        err, err_plain = (float((g.double() - want).norm() / want.norm()) for g in (got, plain))
+        assert err <= 1.5 * err_plain + 4 * U, (err, err_plain)

@@ -355,13 +355,14 @@ __global__ __launch_bounds__(WM* WN * 64) void linear_mfma_kernel(Linear q, Tile
 #pragma unroll
         for (int b = 0; b < TN; ++b) {
           const int n = n0 + wn0 + b * 16;
-          // (bf16: both halves of t meet the same rows of B_p)
+          // (bf16: both halves of t meet the same rows of B_p; the second one, which may be zero, no values that are not finite)
           if constexpr (BF) {
             s16x8 v;
 #pragma unroll
             for (int l = 0; l < 8; ++l) {
               const int j = ((lane >> 4) * 8 & 15) + l;
               v[l] = j < q.R && n + j16 < q.N ? (short)bp[(int64_t)j * q.N + n + j16] : (short)0;
+              if (lane >= 32 && (v[l] & 0x7f80) == 0x7f80) v[l] = 0;
             }
             fb[b] = __builtin_bit_cast(F, v);
           } else {

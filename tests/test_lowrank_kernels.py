@@ -166,3 +166,31 @@ def test_long_sums_are_as_precise_as_the_tensor_form(cuda, dtype, shape):
         got, _ = lowrank_weighted_sum(w, a, b)
         err, err_plain = (float((g.double() - want).norm() / want.norm()) for g in (got, plain))
         assert err <= 1.5 * err_plain + 4 * U, (err, err_plain)
+
+
+# ------------------------------------------------------------------ values at the ends of the range
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("per", [1, 16, 40])
+def test_infinite_factors(device, dtype, per):
+    """Infinite and NaN factors give what the formula gives, an infinity of the right sign among them."""
+    gen = torch.Generator().manual_seed(per)
+    pop, n_in, n_out, r = 64 // per + 30, 128, 136, 3
+    weight, a, b = layer(gen, pop, n_in, n_out, r, 1, dtype, device)
+    x = torch.randint(-3, 4, (pop, per, n_in), generator=gen).to(dtype).to(device)   # (t in few bits: nothing is left of it behind 8)
+    a.copy_(torch.randint(-2, 3, a.shape, generator=gen))
+    b[0, 0, 3], b[1, 2, 70], b[2, 1, 5], b[3, 3, 135] = math.inf, -math.inf, math.nan, math.inf
+    a[4, 1, 9], a[5, 0, 127] = math.inf, math.nan
+    x[6, 0, 0] = -math.inf
+    b[7, 0, :], b[7, 1, :] = math.inf, -math.inf
+    y = lowrank_linear(x, weight, a, b, scale=0.5).cpu().double()
+    # the own part entry by entry: t_j B_j, so that no product of a matrix library decides what 0 times infinity is
+    x64, w64, a64, b64 = x.cpu().double(), weight.cpu().double(), a.cpu().double(), b.cpu().double()
+    t = 0.5 * (x64[:, :, None, :] * a64[:, None]).sum(-1)
+    own = (t[..., None] * b64[:, None, :r]).sum(2) + 0.5 * b64[:, None, r]
+    want = (x64[..., None] * w64).sum(2) + own
+    for kind in (torch.isposinf, torch.isneginf, torch.isnan):
+        assert bool(kind(want).any())
+        wrong = int((kind(y) != kind(want)).sum())
+        assert wrong == 0, kind.__name__

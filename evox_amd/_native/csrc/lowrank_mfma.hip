@@ -30,6 +30,7 @@ using namespace evox::lr;
 
 namespace {
 
+constexpr float kMostBf16 = 0x1.fep127f;
 constexpr int SLOT = 1024;   // bytes of one individual's A_p in a stage: 16 rows of 64 bytes
 
 __device__ const uint4 kZero = {0, 0, 0, 0};
@@ -329,8 +330,11 @@ __global__ __launch_bounds__(WM* WN * 64) void linear_mfma_kernel(Linear q, Tile
           f32x4 rest;
 #pragma unroll
           for (int l = 0; l < 4; ++l) {
-            rest[l] = v[l] - bf2f(f2bf(v[l]));
-            if (rest[l] != rest[l]) rest[l] = 0.f;                    // (an infinite v leaves no rest)
+            // (a value that is not finite leaves no rest; a finite one does not become infinite by rounding)
+            const bool finite = fabsf(v[l]) < __builtin_inff();
+            const float first = finite ? fminf(fmaxf(bf2f(f2bf(v[l])), -kMostBf16), kMostBf16) : v[l];
+            rest[l] = finite ? v[l] - first : 0.f;
+            v[l] = first;
           }
           st4_lds(reinterpret_cast<uint16_t*>(o) + g4, v);
           st4_lds(reinterpret_cast<uint16_t*>(o) + 16 + g4, rest);

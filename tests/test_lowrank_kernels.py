@@ -194,3 +194,20 @@ def test_infinite_factors(device, dtype, per):
         assert bool(kind(want).any())
         wrong = int((kind(y) != kind(want)).sum())
         assert wrong == 0, kind.__name__
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("per", [1, 16])
+def test_intermediates_at_the_top_of_the_range(device, dtype, per):
+    """x A^T between bfloat16's and float32's largest value is finite, and so is its product with a small B."""
+    pop, n_in, n_out = 32, 64, 128
+    x = torch.zeros(pop, per, n_in, dtype=dtype, device=device)
+    x[..., :2] = 2.0 ** 64
+    a = torch.zeros(pop, 1, n_in, dtype=dtype, device=device)
+    a[..., 0], a[..., 1] = 1.9921875 * 2.0 ** 63, 1.5625 * 2.0 ** 55      # together 1.9982910 2^127: rounds to infinity in 8 bits
+    b = torch.full((pop, 1, n_out), 2.0 ** -120, dtype=dtype, device=device)
+    weight = torch.zeros(n_in, n_out, dtype=dtype, device=device)
+    want = 1.9921875 * 2.0 ** 7 + 1.5625 / 2
+    y = lowrank_linear(x, weight, a, b).double()
+    assert float((y - want).abs().max()) <= want * (torch.finfo(dtype).eps / 2 + 8 * U)

@@ -244,7 +244,8 @@ class MLP:
     def lowrank_apply(self, center: torch.Tensor, factors: torch.Tensor, obs: torch.Tensor, rank: int, scale: float = 1.0,
                       index=None) -> torch.Tensor:
         """The networks of a low-rank population on ``obs`` (P, E, in) or (P, in); with ``index`` (T,) on ``obs`` (T, in), row t
-        by individual ``index[t]`` (by the centre itself where that is negative).  Computes in the factors' type."""
+        by individual ``index[t]`` (by the centre itself where that is negative).  Computes in the factors' type; gelu and
+        callables are applied to a layer's rounded output, the other activations before it is rounded."""
         from ..ops.lowrank import lowrank_linear
 
         if center.dim() != 1 or center.shape[0] != self.n_params:
@@ -258,8 +259,11 @@ class MLP:
             if self.bias:
                 bias = center[off:off + o]
                 off += o
-            h = lowrank_linear(h, weight, a, b, index=index, bias=bias, scale=scale,
-                               activation=self.final_activation if li == last else self.activation)
+            act = self.final_activation if li == last else self.activation
+            fused = isinstance(act, str) and act in _ACT_CODE
+            h = lowrank_linear(h, weight, a, b, index=index, bias=bias, scale=scale, activation=act if fused else "identity")
+            if not fused:
+                h = (_ACT[act] if isinstance(act, str) else act)(h)
         return h
 
     def lowrank_gradient(self, w: torch.Tensor, factors: torch.Tensor, rank: int, scale: float = 1.0) -> torch.Tensor:

@@ -7,8 +7,10 @@ import torch
 
 from evox_amd import _native
 from evox_amd._native import build
+from evox_amd.core import random as rnd
+from evox_amd.models import MLP
 from evox_amd.ops.lowrank import lowrank_linear, lowrank_weighted_sum
-from test_lowrank import DEVICES, DTYPES, U, check_linear, check_sum, layer, randn
+from test_lowrank import ACT, DEVICES, DTYPES, U, check_linear, check_sum, layer, linear_oracle, randn
 
 needs_library = pytest.mark.skipif(not (build.HIP_LIB.exists() or build.have_hipcc()), reason="no kernel library")
 
@@ -211,3 +213,33 @@ def test_intermediates_at_the_top_of_the_range(device, dtype, per):
     want = 1.9921875 * 2.0 ** 7 + 1.5625 / 2
     y = lowrank_linear(x, weight, a, b).double()
     assert float((y - want).abs().max()) <= want * (torch.finfo(dtype).eps / 2 + 8 * U)
+
+
+# ------------------------------------------------------------------ networks
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("hidden,final", [("gelu", "tanh"), ("relu", "gelu"), (torch.sin, lambda v: 2 * v), (torch.nn.functional.silu, "sigmoid")])
+def test_networks_of_any_activation(device, dtype, hidden, final):
+    """MLP's other activations, by name and as callables: the layers' bound of test_linear, each layer on the one before as it came
+    out, then an activation whose slope is below 2 here and which rounds twice (to its type, and once inside)."""
+    gen = torch.Generator().manual_seed(37)
+    net = MLP([12, 40, 5], activation=hidden, final_activation=final)
+    center = net.init(rnd.PRNGKey(3)).to(device)
+    factors = randn(gen, 9, net.lowrank_size(2), dtype=dtype).to(device)
+    x = randn(gen, 9, 4, 12, dtype=dtype).to(device)
+    y = net.lowrank_apply(center, factors, x, 2, 0.1)
+    assert y.shape == (9, 4, 5) and y.dtype == dtype
+    names = {"gelu": torch.nn.functional.gelu, **ACT}
+    (a0, b0), (a1, b1) = net.lowrank_factors(factors, 2)
+    w0, c0, w1, c1 = (v.to(t) for v, t in zip(center.split([480, 40, 200, 5]), (dtype, torch.float32) * 2))
+    act, fin = (names.get(v, v) for v in (hidden, final))
+    eps = torch.finfo(dtype).eps / 2
+    h = lowrank_linear(x, w0.view(12, 40), a0, b0, bias=c0, scale=0.1, activation=hidden if hidden in ACT else "identity")
+    h = h if hidden in ACT else act(h)
+    z, off = linear_oracle(h, w1.view(40, 5), a1, b1, bias=c1, scale=0.1)
+    want = fin(z)
+    bound = 2 * off + (3 if final in ACT else 4) * eps * (want.abs() + 2 * off) + 16 * U
+    assert bool(((y.cpu().double() - want).abs() <= bound).all())
+    one = net.lowrank_apply(center, factors, x[:3, 0], 2, 0.1, index=torch.tensor([2, -1, 0], device=device))
+    assert one.shape == (3, 5) and one.dtype == dtype

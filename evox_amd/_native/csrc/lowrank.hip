@@ -16,6 +16,7 @@ int linear_mfma_side(const Linear& q, int elem);
 template <typename T>
 int linear_mfma(const Linear& q, bool grouped, hipStream_t s, int* tile = nullptr);
 void sum_mfma_plan(Sum& q, int elem);                            // lowrank_sum_mfma.hip
+int sum_mfma_side(const Sum& q, int elem);
 int sum_mfma(const Sum& q, int elem, hipStream_t s);
 }  // namespace lr
 }  // namespace evox
@@ -355,8 +356,9 @@ void launch_sum_join(const Sum& q, hipStream_t s) {
 
 enum class Path { kTile, kMfma, kGrouped, kFew };
 
-// Where the operands of a call lie in its workspace.
+// Where the operands of a call lie in its workspace, and the rows of its matrix-core tile.
 struct Layout {
+  int tile = 0;
   bool pack_x = false, pack_w = false, pack_a = false;
   int64_t t = 0, slab = 0, x = 0, w = 0, a = 0, floats = 0;
 };
@@ -526,8 +528,7 @@ static int linear_call(const void* x, const void* w, const void* a, const void* 
   at.a = copy(at.pack_a, q.pop * q.R, q.K);
   if (path == Path::kTile) return fits_launch(tile_workgroups(q), NT) ? 0 : (int)hipErrorInvalidValue;
   if (path == Path::kFew) return 0;
-  int tile;
-  return el == 2 ? linear_mfma<uint16_t>(q, path == Path::kGrouped, nullptr, &tile) : linear_mfma<float>(q, path == Path::kGrouped, nullptr, &tile);
+  return el == 2 ? linear_mfma<uint16_t>(q, path == Path::kGrouped, nullptr, &at.tile) : linear_mfma<float>(q, path == Path::kGrouped, nullptr, &at.tile);
 }
 
 // Floats of workspace that the same call of evox_hip_lowrank_linear takes (negative: the call is refused, y has more tiles than a
@@ -540,6 +541,17 @@ EVOX_API int64_t evox_hip_lowrank_linear_ws(const void* x, const void* w, const 
   Layout at;
   if (linear_call(x, w, a, b, bias, index, y, dims, ints, 1.f, q, path, at)) return -1;
   return at.floats;
+}
+
+// The kernel that the same call takes: the rows of its matrix-core tile, 1000 more where the individuals' parts are computed inside the
+// tiles; 1: up to four rows; 0: tiles of any size and alignment; negative: the call is refused.
+EVOX_API int evox_hip_lowrank_linear_kernel(const void* x, const void* w, const void* a, const void* b, const float* bias,
+                                            const void* index, void* y, const int64_t* dims, const int* ints) {
+  Linear q;
+  Path path;
+  Layout at;
+  if (linear_call(x, w, a, b, bias, index, y, dims, ints, 1.f, q, path, at)) return -1;
+  return path == Path::kGrouped ? 1000 + at.tile : path == Path::kMfma ? at.tile : path == Path::kFew ? 1 : 0;
 }
 
 EVOX_API int evox_hip_lowrank_linear(const void* x, const void* w, const void* a, const void* b, const float* bias,
@@ -627,6 +639,15 @@ EVOX_API int64_t evox_hip_lowrank_sum_ws(const float* w, const void* a, const vo
   SumLayout at;
   if (sum_call(w, a, b, g, gb, dims, ints, 1.f, q, at)) return -1;
   return at.floats;
+}
+
+// The kernel that the same call takes: the rows of its matrix-core tile; 0: tiles of any size and alignment; negative: refused.
+EVOX_API int evox_hip_lowrank_sum_kernel(const float* w, const void* a, const void* b, float* g, float* gb, const int64_t* dims,
+                                         const int* ints) {
+  Sum q;
+  SumLayout at;
+  if (sum_call(w, a, b, g, gb, dims, ints, 1.f, q, at)) return -1;
+  return at.mfma ? sum_mfma_side(q, ints[3] ? 2 : 4) : 0;
 }
 
 EVOX_API int evox_hip_lowrank_sum(const float* w, const void* a, const void* b, float* g, float* gb, const int64_t* dims,

@@ -313,19 +313,21 @@ int launch(const Sum& q, hipStream_t s) {
   return last_launch_status();
 }
 
-// Tiles of 256 x 256 for bf16 where there are at least 12 of them (1024 x 720: 73 us against 76 with 128 x 128); float32 products
-// last sixteen times as long as the reads that feed them and gain nothing from them.
-bool big_tiles(const Sum& q, int elem) { return elem == 2 && (int64_t)((q.M + 255) / 256) * ((q.N + 255) / 256) >= 12; }
-
 }  // namespace
 
 namespace evox {
 namespace lr {
 
+// Tiles of 256 x 256 for bf16 where there are at least 12 of them (1024 x 720: 73 us against 76 with 128 x 128); float32 products
+// last sixteen times as long as the reads that feed them and gain nothing from them.
+int sum_mfma_side(const Sum& q, int elem) {
+  return elem == 2 && (int64_t)((q.M + 255) / 256) * ((q.N + 255) / 256) >= 12 ? 256 : 128;
+}
+
 // K is split so that the chip is filled once (256 x 256: one workgroup a compute unit, else two); a split has 128 k at least, and
 // 2^30 at most: the kernel counts a split's k in 32 bits.
 void sum_mfma_plan(Sum& q, int elem) {
-  const bool big = big_tiles(q, elem);
+  const bool big = sum_mfma_side(q, elem) == 256;
   const int bk = 64 / elem;
   const int64_t side = big ? 256 : 128, tiles = ((q.M + side - 1) / side) * ((q.N + side - 1) / side);
   int64_t s = (big ? kNumCU : 2 * kNumCU) / tiles;
@@ -340,7 +342,7 @@ void sum_mfma_plan(Sum& q, int elem) {
 
 int sum_mfma(const Sum& q, int elem, hipStream_t s) {
   if (elem == 4) return launch<float, 128, 2, 2, 4>(q, s);
-  return big_tiles(q, elem) ? launch<uint16_t, 256, 4, 2, 4>(q, s) : launch<uint16_t, 128, 2, 2, 4>(q, s);
+  return sum_mfma_side(q, elem) == 256 ? launch<uint16_t, 256, 4, 2, 4>(q, s) : launch<uint16_t, 128, 2, 2, 4>(q, s);
 }
 
 }  // namespace lr

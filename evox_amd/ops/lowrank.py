@@ -21,8 +21,10 @@ from ._util import DTYPE_CODE, check, hip, launch_device, on_gpu, stream_of
 P, I, I64, F = _native.P, _native.I, _native.I64, _native.F
 _native.register_hip_api({
     "evox_hip_lowrank_linear_ws": (I64, [P, P, P, P, P, P, P, P, P]),
+    "evox_hip_lowrank_linear_kernel": (I, [P, P, P, P, P, P, P, P, P]),
     "evox_hip_lowrank_linear": (I, [P, P, P, P, P, P, P, P, P, P, I64, F, P]),
     "evox_hip_lowrank_sum_ws": (I64, [P, P, P, P, P, P, P]),
+    "evox_hip_lowrank_sum_kernel": (I, [P, P, P, P, P, P, P]),
     "evox_hip_lowrank_sum": (I, [P, P, P, P, P, P, P, P, I64, F, P]),
 })
 

@@ -243,3 +243,117 @@ def test_networks_of_any_activation(device, dtype, hidden, final):
     assert bool(((y.cpu().double() - want).abs() <= bound).all())
     one = net.lowrank_apply(center, factors, x[:3, 0], 2, 0.1, index=torch.tensor([2, -1, 0], device=device))
     assert one.shape == (3, 5) and one.dtype == dtype
+
+
+# ------------------------------------------------------------------ every variant that a size chooses
+
+ANY, FEW, GROUPED = 0, 1, 1000                     # any-size tiles, up to four rows, individuals' parts in the tiles
+BF, FP = torch.bfloat16, torch.float32
+VARIANTS = [  # type, individuals, rows each (None: rows that name their individual), in, out, rank, kernel: rows of its tile (+ GROUPED)
+    # bf16 tiles of 256: 2 to 5 steps of K and more, a last step in part, odd tile edges; 1 to 8 individuals in a tile
+    (BF, 256, 256, 64, 256, 16, GROUPED + 256),     # one individual a tile
+    (BF, 683, 48, 72, 264, 5, GROUPED + 256),       # three fragments each: up to seven individuals, which straddle tiles
+    (BF, 2048, 32, 96, 248, 16, GROUPED + 256),     # eight individuals a tile
+    (BF, 1500, 23, 128, 264, 3, GROUPED + 256),     # two fragments, the last one in part
+    (BF, 300, 230, 160, 132, 7, GROUPED + 256),     # fifteen fragments
+    (BF, 66, 1000, 200, 136, 16, GROUPED + 256),    # individuals longer than a tile
+    (BF, 3, 22000, 264, 136, 1, GROUPED + 256),
+    (BF, 683, 48, 73, 259, 5, GROUPED + 256),       # rows off 16 bytes: copied
+    (BF, 33000, 1, 64, 264, 3, 256),
+    (BF, 66000, 1, 104, 136, 1, 256),
+    (BF, 130, 256, 136, 264, 17, 256),              # rank above 16
+    (BF, 12, None, 264, 264, 4, 256),
+    (BF, 12, None, 1096, 1032, 4, 256),
+    (BF, 12, None, 265, 259, 4, 256),
+    # tiles of 128
+    (BF, 256, 128, 64, 128, 16, GROUPED + 128),
+    (BF, 2100, 16, 72, 120, 9, GROUPED + 128),      # eight individuals a tile
+    (BF, 2100, 16, 96, 264, 9, GROUPED + 128),      # sixteen would meet in a tile of 256
+    (BF, 700, 48, 104, 66, 2, GROUPED + 128),
+    (BF, 33000, 1, 200, 72, 3, 128),
+    (BF, 900, 20, 72, 200, 20, 128),
+    (FP, 256, 128, 32, 128, 16, GROUPED + 128),
+    (FP, 2100, 16, 36, 120, 9, GROUPED + 128),
+    (FP, 230, 48, 68, 264, 5, GROUPED + 128),
+    (FP, 40, 300, 100, 260, 12, GROUPED + 128),
+    (FP, 40, 300, 499, 261, 12, GROUPED + 128),
+    (FP, 11000, 1, 132, 264, 2, 128),
+    (FP, 5, None, 260, 264, 3, 128),
+    (FP, 100, 330, 64, 72, 24, 128),
+    # tiles of 64, K whole and divided, and of 16
+    (BF, 40, 48, 136, 72, 16, GROUPED + 64), (FP, 40, 48, 68, 72, 16, GROUPED + 64), (BF, 500, 23, 72, 40, 3, GROUPED + 64),
+    (BF, 20000, 1, 72, 64, 3, 64), (FP, 20000, 1, 72, 60, 3, 64),                        # t by the tiles' own workgroups
+    (BF, 300, 1, 1096, 200, 5, 64), (FP, 300, 1, 1096, 200, 5, 64),
+    (BF, 16, 1, 520, 264, 5, 16), (FP, 3, 5, 520, 264, 20, 16), (BF, 9, 1, 72, 1000, 5, 16),
+    # up to four rows, any size
+    (BF, 4, 1, 1001, 264, 5, FEW), (FP, 1, 1, 300, 1004, 5, FEW), (BF, 300, 7, 11, 32, 1, ANY), (FP, 300, 7, 11, 32, 1, ANY),
+]
+
+
+def kernel_of(dtype, pop, per, n_in, n_out, r):
+    rows = 33003 if per is None else pop * per
+    at, dims, ints = host_call((rows, pop, per or 1, (per or 1) * n_in, n_in, r * n_in, r * n_out),
+                               (n_in, n_out, r, 0, 0, int(dtype == torch.bfloat16), 2 * (per is None)))
+    return _native.hip().evox_hip_lowrank_linear_kernel(at, at, at, at, None, at, at, ctypes.addressof(dims), ctypes.addressof(ints))
+
+
+@needs_library
+@pytest.mark.parametrize("case", VARIANTS, ids=str)
+def test_kernel_of_each_shape(case):
+    """The shapes above take the kernels that they are there for."""
+    *shape, kernel = case
+    assert kernel_of(*shape) == kernel
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", VARIANTS, ids=str)
+def test_each_linear_kernel(cuda, case):
+    dtype, pop, per, n_in, n_out, r, _ = case
+    gen = torch.Generator().manual_seed(pop + n_in + n_out)
+    for own_bias, act in ((0, "identity"), (1, "tanh")):
+        weight, a, b = layer(gen, pop, n_in, n_out, r, own_bias, dtype, cuda, pitch=-(r * n_in + (r + own_bias) * n_out) % 8)
+        kw = dict(bias=randn(gen, n_out).to(cuda) if own_bias else None, scale=0.4, activation=act)
+        if per is None:
+            kw["index"] = torch.randint(-1, pop, (33003,), generator=gen).to(cuda)
+            x = randn(gen, 33003, n_in, dtype=dtype).to(cuda)
+        else:
+            x = randn(gen, pop, per, n_in, dtype=dtype).to(cuda)
+        y = lowrank_linear(x, weight, a, b, **kw)
+        check_linear(y, x, weight, a, b, **kw)
+        assert torch.equal(y, lowrank_linear(x, weight, a, b, **kw))
+
+
+SUM_VARIANTS = [  # type, individuals, in, out, rank, rows of the tile (0: any size)
+    (BF, 64, 1024, 720, 1, 256), (BF, 40, 1000, 1000, 2, 256), (BF, 33, 1032, 700, 5, 256), (BF, 700, 768, 1024, 3, 256),
+    (BF, 5000, 1024, 720, 1, 256), (BF, 4096, 1000, 700, 4, 256), (BF, 50, 1024, 768, 33, 256), (BF, 24, 1024, 720, 3, 256),
+    (BF, 64, 64, 64, 1, 128), (BF, 33, 136, 264, 3, 128), (BF, 9000, 130, 136, 2, 128), (BF, 20000, 128, 128, 1, 128),
+    (BF, 300, 300, 260, 16, 128), (BF, 300, 249, 250, 40, 128),
+    (FP, 64, 64, 64, 1, 128), (FP, 33, 136, 264, 3, 128), (FP, 9000, 130, 136, 2, 128), (FP, 300, 1024, 720, 7, 128), (FP, 300, 251, 249, 40, 128),
+    (BF, 300, 47, 400, 3, 0), (FP, 20000, 11, 32, 1, 0),
+]
+
+
+def sum_kernel_of(dtype, pop, n_in, n_out, r):
+    at, dims, ints = host_call((pop, r * n_in, r * n_out), (n_in, n_out, r, int(dtype == torch.bfloat16)))
+    return _native.hip().evox_hip_lowrank_sum_kernel(at, at, at, at, None, ctypes.addressof(dims), ctypes.addressof(ints))
+
+
+@needs_library
+@pytest.mark.parametrize("case", SUM_VARIANTS, ids=str)
+def test_kernel_of_each_sum(case):
+    *shape, kernel = case
+    assert sum_kernel_of(*shape) == kernel
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", SUM_VARIANTS, ids=str)
+def test_each_sum_kernel(cuda, case):
+    dtype, pop, n_in, n_out, r, _ = case
+    gen = torch.Generator().manual_seed(pop + n_in + n_out)
+    for own_bias in (0, 1):
+        _, a, b = layer(gen, pop, n_in, n_out, r, own_bias, dtype, cuda, pitch=-(r * n_in + (r + own_bias) * n_out) % 8)
+        w = randn(gen, pop).to(cuda)
+        got = lowrank_weighted_sum(w, a, b, scale=-0.3)
+        check_sum(got, w, a, b, -0.3)
+        again = lowrank_weighted_sum(w, a, b, scale=-0.3)
+        assert torch.equal(got[0], again[0]) and (not own_bias or torch.equal(got[1], again[1]))

@@ -117,8 +117,10 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], st
     bits = _check_state(state, device, total)
     hyper = (learning_rate, b1, b2, 1 - b1, 1 - b2, eps, weight_decay, math.log(b1) if b1 else -math.inf,
              math.log(b2) if b2 else -math.inf)
-    if where < 0 or total == 0:
+    if where < 0:
         return adamw_step_reference(params, grads, state, hyper, bits, decay, updates)
+    if total == 0:
+        return [torch.empty_like(p) for p in params], {**{k: v.clone() for k, v in state.items()}, "count": state["count"] + 1}
     return _step_hip(params, grads, sizes, flags, state, hyper, bits, decay, updates, total, device)
 
 

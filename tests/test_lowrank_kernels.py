@@ -357,3 +357,43 @@ def test_each_sum_kernel(cuda, case):
         check_sum(got, w, a, b, -0.3)
         again = lowrank_weighted_sum(w, a, b, scale=-0.3)
         assert torch.equal(got[0], again[0]) and (not own_bias or torch.equal(got[1], again[1]))
+
+
+@pytest.mark.gpu
+def test_recorded_large_calls(cuda):
+    """Large tiles recorded without a call before, replayed on new data with eager calls between the replays, on two graphs in turn."""
+    gen = torch.Generator().manual_seed(41)
+    sets = []
+    for k in range(2):
+        weight, a, b = layer(gen, 256, 128, 256, 16, 1, BF, cuda)
+        _, sa, sb = layer(gen, 2000, 1024, 720, 4, 1, BF, cuda)
+        sets.append((randn(gen, 256, 256, 128, dtype=BF).to(cuda), weight, a, b, randn(gen, 2000).to(cuda), sa, sb))
+
+    def calls(x, weight, a, b, w, sa, sb):
+        return (lowrank_linear(x, weight, a, b, activation="tanh"), *lowrank_weighted_sum(w, sa, sb))
+
+    graphs, outs = [], []
+    for s in sets:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            outs.append(calls(*s))
+    for _ in range(3):
+        for s, graph, out in zip(sets, graphs, outs):
+            s[0].copy_(randn(gen, 256, 256, 128, dtype=BF))
+            s[4].copy_(randn(gen, 2000))
+            want = calls(*s)
+            graph.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(p, q) for p, q in zip(out, want))
+    # and both at once, each on a stream of its own
+    want = [calls(*s) for s in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = []
+    for _ in range(4):
+        for s, stream in zip(sets, streams):
+            with torch.cuda.stream(stream):
+                got.append(calls(*s))
+    torch.cuda.synchronize()
+    for k, one in enumerate(got):
+        assert all(torch.equal(p, q) for p, q in zip(one, want[k % 2]))

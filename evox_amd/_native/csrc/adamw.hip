@@ -8,7 +8,8 @@
 // leaves live in one flat buffer in which every leaf starts at a multiple of 256 elements, so their accesses are always
 // aligned.  Results go to new buffers (the traffic is that of an update in place, and the old state stays valid).
 // Measured: 67 M bf16 parameters with fp32 gradients and moments 287 us (5.6 TB/s; a copy of 1 GiB reaches 5.1), 134 M fp32
-// parameters with 8-bit moments 420 us (5.2 TB/s), reading these moments back as bf16 156 us; six small leaves 5 us.
+// parameters with 8-bit moments 420 to 490 us from run to run (5.2 to 4.4 TB/s), reading these moments back as bf16 157 to 163 us;
+// six small leaves 5 us.
 //
 // 8-bit moments: 32 neighbouring elements share a power-of-two unit (one byte q, unit = 2^(q - 127)), the smallest whose
 // largest code holds the block's largest magnitude.  mu: sign, 4 exponent and 3 mantissa bits; nu: 5 exponent and 3

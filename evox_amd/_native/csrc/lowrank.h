@@ -66,8 +66,10 @@ __device__ __forceinline__ float activate(float v, int act) {
   }
 }
 
-// Activations whose result is rounded to bf16: the exponential of the hardware (2^x) is good to 2^-22, and tanh, which would lose
-// its small values in 1 - 2 / (e^2v + 1), is its series below 1/8 (next term 17/315 v^7: 2^-26 of v).
+// Activations whose result is rounded to bf16.  The exponential of the hardware (2^x) adds 2^-22 to what rounding its argument
+// leaves, 2^-24 of |v| log2(e), so a sigmoid is off by (|v| + 4) 2^-23 of itself: below 2^-16 wherever it is not zero (below
+// v = -87, where it is 1e-38, it is).  tanh, which would lose its small values in 1 - 2 / (e^2v + 1), is its series below 1/8 (next
+// term 17/315 v^7: 2^-22 of v).
 __device__ __forceinline__ float tanh_bf16(float v) {
   const float s = v * v, small = v * fmaf(s, fmaf(s, 2.f / 15.f, -1.f / 3.f), 1.f);
   const float big = 1.f - 2.f * __builtin_amdgcn_rcpf(__expf(2.f * v) + 1.f);

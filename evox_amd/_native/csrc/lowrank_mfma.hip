@@ -12,14 +12,16 @@
 // Tiles: 256 x 256 (bf16, eight wavefronts, the two of a SIMD half a step apart) where they fill the chip, else 128 x 128 or
 // 64 x 64 with K divided over workgroups; 16 x 128 for requests.  65536 x 2048 x 2048 bf16 with 256 individuals of rank 16: 612 us
 // (0.91 PFLOP/s; 530 without the tiles' ends, 377 without loads, 388 with nothing but loads); 16384 x 1024 x 1024 float32, rank 8:
-// 343 us (the matrix pipe is busy 75 % of the time); 4096 x 1024 x 720 bf16, single rows, rank 4: 25 us and 9 for t (its tiles of 64
-// move 200 MB from the second-level cache, 16 us; tiles of 128 half of that, with idle compute units: 33 to 43 us).
+// 343 us (the matrix pipe is busy 75 % of the time, a ninth of that with t, which each of the eight column tiles computes again);
+// 4096 x 1024 x 720 bf16, single rows, rank 4: 26 us and 9 for t (its tiles of 64 move 200 MB from the second-level cache, 16 us; tiles
+// of 128 half of that, with idle compute units: 33 to 43 us).
 //
 // The individuals' part:
 //   GROUPED (an individual has at least 16 rows, rank at most 16): the 16-row fragments of a tile each belong to one individual
 //     (its last one may be partly empty).  t = x A_p^T is one more matrix product of x's fragments, against A_p's rows in the stage
 //     (a slot for each individual that meets in the tile) - no second pass over x and no launch of its own.  At the end s t
-//     (bf16: in two halves, together 16 bits) times B_p is one product per fragment of outputs.
+//     (bf16: in two halves, together 16 bits, 2^-17 of a part of what is then rounded to 8) times B_p is one product per fragment
+//     of outputs.
 //   otherwise (single rows, requests): t comes from shrink_block - workgroups of their own in front, a launch before, or the
 //     workgroup itself where its rows are nobody else's - and every lane adds its row's R products to its columns.
 #include "lowrank.h"
@@ -30,7 +32,7 @@ using namespace evox::lr;
 
 namespace {
 
-constexpr float kMostBf16 = 0x1.fep127f;
+constexpr float kMostBf16 = 0x1.fep127f;   // the largest bfloat16
 constexpr int SLOT = 1024;   // bytes of one individual's A_p in a stage: 16 rows of 64 bytes
 
 __device__ const uint4 kZero = {0, 0, 0, 0};

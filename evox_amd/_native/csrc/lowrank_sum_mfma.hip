@@ -318,8 +318,9 @@ int launch(const Sum& q, hipStream_t s) {
 namespace evox {
 namespace lr {
 
-// Tiles of 256 x 256 for bf16 where there are at least 12 of them (1024 x 720: 73 us against 76 with 128 x 128); float32 products
-// last sixteen times as long as the reads that feed them and gain nothing from them.
+// Tiles of 256 x 256 for bf16 where there are at least 12 of them (K = 16384, 1024 x 720: 87 us against 104 with 128 x 128; K =
+// 65536, 768 x 1024: 261 against 348); float32 products last sixteen times as long as the reads that feed them and gain nothing
+// from them.
 int sum_mfma_side(const Sum& q, int elem) {
   return elem == 2 && (int64_t)((q.M + 255) / 256) * ((q.N + 255) / 256) >= 12 ? 256 : 128;
 }

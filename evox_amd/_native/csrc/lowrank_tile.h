@@ -1,4 +1,4 @@
-// Tiles in LDS for the bf16 matrix instructions: counted waits, transposed reads, permuted rows.
+// Tiles in LDS for the bf16 and float32 matrix instructions: counted waits, transposed reads, permuted rows.
 #pragma once
 #include "lowrank.h"
 #include <atomic>

@@ -3,7 +3,7 @@
 The moments of all leaves live in one flat buffer each: leaf after leaf in the order given, every leaf padded with zeros
 to a multiple of ``ALIGN`` elements.  A state is a dict of tensors:
 
-``count``                  float32 scalar, steps taken
+``count``                  float32 scalar, steps taken (stays at 2^24, and the dither of 8-bit moments stands still from there on)
 ``mu``, ``nu``             ``(total,)`` float32, or uint8 codes
 ``mu_scale``, ``nu_scale`` (8 bits only) ``(total / BLOCK,)`` uint8: ``BLOCK`` neighbours share the unit ``2^(scale - 127)``
 

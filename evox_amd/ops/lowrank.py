@@ -170,8 +170,9 @@ def lowrank_weighted_sum(w: torch.Tensor, a: torch.Tensor, b: torch.Tensor, scal
 
     w : (P,) float32;  a : (P, r, in), b : (P, r, out) or (P, r + 1, out) as in :func:`lowrank_linear`, float32 or bfloat16
     views of any stride between individuals.  Sums are float32 in an order that depends on sizes, strides and alignment alone
-    (repeated calls give the same bits).  A factor that is not finite (bfloat16: or a product w a of
-    more than 3.39e38) leaves its row or column of the sum not finite, and nothing else.  No autograd graph is built: inputs that ask for a gradient are refused."""
+    (repeated calls give the same bits).  A factor that is not finite leaves its row or column of the sum not finite, and nothing
+    else.  With bfloat16 factors a product w a is held to 24 bits from 2e-31 on (to 2^-126 below) and up to 3.39e38.  No autograd
+    graph is built: inputs that ask for a gradient are refused."""
     r, own_bias = _check_factors("lowrank_weighted_sum", a, b)
     pop = a.shape[0]
     if w.dtype != torch.float32:

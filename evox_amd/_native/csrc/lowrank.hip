@@ -420,13 +420,13 @@ int launch_linear(Linear q, Path path, const Layout& at, float* ws, hipStream_t 
   return last_launch_status();
 }
 
+// workgroups of the any-size tiles: the products', and all with the biases'
+int64_t sum_tiles(const Sum& q) { return (int64_t)((q.M + BM - 1) / BM) * ((q.N + BN - 1) / BN); }
+int64_t sum_workgroups(const Sum& q) { return (sum_tiles(q) + (q.gb != nullptr ? (q.N + 63) / 64 : 0)) * q.splits; }
+
 template <typename T>
 int launch_sum(const Sum& q, hipStream_t s) {
-  const int tiles_n = (q.N + BN - 1) / BN;
-  const int64_t tiles = (int64_t)((q.M + BM - 1) / BM) * tiles_n;
-  const int64_t wgs = (tiles + (q.gb != nullptr ? (q.N + 63) / 64 : 0)) * q.splits;
-  if (!fits_launch(wgs, NT)) return (int)hipErrorInvalidValue;
-  sum_kernel<T><<<(unsigned)wgs, NT, 0, s>>>(q, tiles_n, (int)tiles);
+  sum_kernel<T><<<(unsigned)sum_workgroups(q), NT, 0, s>>>(q, (q.N + BN - 1) / BN, (int)sum_tiles(q));
   if (q.splits > 1) launch_sum_join(q, s);
   return last_launch_status();
 }
@@ -603,6 +603,7 @@ static int sum_call(const float* w, const void* a, const void* b, float* g, floa
   }
   if (at.mfma) sum_mfma_plan(q, el);
   else plan_sum(q);
+  if (!at.mfma && !fits_launch(sum_workgroups(q), NT)) return (int)hipErrorInvalidValue;
   at.floats = q.splits > 1 ? ((int64_t)q.splits * (q.M + 1) * q.N + 3) / 4 * 4 : 0;
   at.a = at.floats;
   if (at.pack_a) at.floats += q.K * up16(q.M, el) * el / 4;
@@ -632,7 +633,8 @@ static int launch_sum_call(Sum q, const SumLayout& at, float* ws, hipStream_t s)
   return last_launch_status();
 }
 
-// Floats of workspace that the same call of evox_hip_lowrank_sum takes (negative: the call is refused).
+// Floats of workspace that the same call of evox_hip_lowrank_sum takes (negative: the call is refused, its result has more tiles than a
+// launch holds).
 EVOX_API int64_t evox_hip_lowrank_sum_ws(const float* w, const void* a, const void* b, float* g, float* gb, const int64_t* dims,
                                          const int* ints) {
   Sum q;

@@ -172,7 +172,7 @@ def lowrank_weighted_sum(w: torch.Tensor, a: torch.Tensor, b: torch.Tensor, scal
     views of any stride between individuals.  Sums are float32 in an order that depends on sizes, strides and alignment alone
     (repeated calls give the same bits).  A factor that is not finite leaves its row or column of the sum not finite, and nothing
     else.  With bfloat16 factors a product w a is held to 24 bits from 2e-31 on (to 2^-126 below) and up to 3.39e38.  No autograd
-    graph is built: inputs that ask for a gradient are refused."""
+    graph is built: inputs that ask for a gradient are refused, and so are results of 2^24 tiles of 64 x 64 or more."""
     r, own_bias = _check_factors("lowrank_weighted_sum", a, b)
     pop = a.shape[0]
     if w.dtype != torch.float32:
@@ -201,6 +201,8 @@ def lowrank_weighted_sum(w: torch.Tensor, a: torch.Tensor, b: torch.Tensor, scal
     call = (w.data_ptr(), a.data_ptr(), b.data_ptr(), g.data_ptr(), None if gb is None else gb.data_ptr(), ctypes.addressof(dims),
             ctypes.addressof(ints))
     floats = lib.evox_hip_lowrank_sum_ws(*call)
+    if floats < 0:
+        raise ValueError(f"lowrank_weighted_sum: {n_in} x {n_out} results are more tiles than one launch holds (2^24 of 64 x 64)")
     ws = w.new_empty(floats) if floats > 0 else None
     with launch_device(dev):
         check(lib.evox_hip_lowrank_sum(*call, None if ws is None else ws.data_ptr(), floats, float(scale), stream_of(g)), "lowrank_weighted_sum")

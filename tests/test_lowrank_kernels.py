@@ -113,6 +113,8 @@ def test_launches_of_many_rows(dtype):
         assert linear_workspace(2 ** 24, 264, 72, r, dtype, pop=2 ** 16, per=2 ** 8) >= 0
         assert linear_workspace(2 ** 28, 8, 8, r, dtype, pop=2 ** 28) >= 0
         assert linear_workspace(2 ** 30 + 64, 8, 8, r, dtype, pop=2 ** 30 + 64) < 0
+        assert sum_workspace(3, 2 ** 29, 5, r, dtype) >= 0
+        assert sum_workspace(3, 2 ** 30, 5, r, dtype) < 0 and sum_workspace(3, 5, 2 ** 30 + 1, r, dtype) < 0
 
 
 # ------------------------------------------------------------------ precision of the weighted sum

@@ -363,6 +363,12 @@ struct Layout {
   int64_t t = 0, slab = 0, x = 0, w = 0, a = 0, floats = 0;
 };
 
+// workgroups of linear_few_kernel: the ones that compute t, and the products'
+int64_t few_workgroups(const Linear& q, int elem) {
+  const int cols = 64 * 16 / elem;
+  return shrink_blocks(q, elem, FEW_NT) + (int64_t)((q.N + cols - 1) / cols) * ((q.K + FEW_K - 1) / FEW_K);
+}
+
 // workgroups of the any-size tiles
 int64_t tile_workgroups(const Linear& q) { return (q.rows + BM - 1) / BM * ((q.N + BN - 1) / BN) * q.splits; }
 
@@ -378,9 +384,8 @@ int launch_linear(Linear q, Path path, const Layout& at, float* ws, hipStream_t 
   };
   auto shrink = [&]() { shrink_kernel<T><<<(unsigned)shrink_blocks(q, sizeof(T), NT), NT, 0, s>>>(q); };
   if (path == Path::kFew) {
-    constexpr int COLS = 64 * 16 / (int)sizeof(T);
     const int first = (int)shrink_blocks(q, sizeof(T), FEW_NT);
-    const unsigned wgs = (unsigned)(first + (q.N + COLS - 1) / COLS * q.splits);
+    const unsigned wgs = (unsigned)few_workgroups(q, sizeof(T));
     if (q.rows == 1) linear_few_kernel<T, 1><<<wgs, FEW_NT, 0, s>>>(q, first);
     else linear_few_kernel<T, 4><<<wgs, FEW_NT, 0, s>>>(q, first);
     join();
@@ -482,8 +487,8 @@ static int linear_call(const void* x, const void* w, const void* a, const void* 
   at = Layout{};
   path = Path::kTile;
   const double flops = 2.0 * (double)q.rows * q.K * q.N;
-  if (q.rows <= 4 && w16 && flops >= 1 << 17) {
-    // up to four rows: W goes through registers once
+  if (q.rows <= 4 && w16 && flops >= 1 << 17 && fits_launch(few_workgroups(q, el), FEW_NT)) {
+    // up to four rows (and 2^30 inputs): W goes through registers once
     path = Path::kFew;
     q.splits = (q.K + FEW_K - 1) / FEW_K;
     q.k_per_split = FEW_K;

@@ -54,6 +54,16 @@ def test_long_sums_are_divided(dtype):
     assert sum_workspace(2 ** 30, 8192, 8192, 1, dtype) == 0
 
 
+@needs_library
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_few_rows_of_very_many_inputs(dtype):
+    """Up to four rows take a workgroup for each 128 inputs and 512 threads each: from 2^30 inputs on that is more than a launch counts,
+    and they take the tiles that divide the inputs into fewer parts."""
+    for n_out, few, many in ((8, 2 ** 29, 2 ** 30), (1024, 2 ** 26, 2 ** 29)):
+        assert kernel_of(dtype, 1, 4, few, n_out, 2) == FEW
+        assert kernel_of(dtype, 1, 4, many, n_out, 2) == 16
+
+
 def test_refuses_features_near_2_to_31():
     """Tiles are counted in 32 bits beyond a tensor's last feature."""
     n = 2 ** 31 - 2 ** 16
@@ -399,3 +409,16 @@ def test_recorded_large_calls(cuda):
     torch.cuda.synchronize()
     for k, one in enumerate(got):
         assert all(torch.equal(p, q) for p, q in zip(one, want[k % 2]))
+
+
+@pytest.mark.gpu
+def test_one_row_of_2_to_30_inputs(cuda):
+    """Zeros but for a few inputs, the last among them."""
+    n = 2 ** 30
+    at = torch.tensor([0, 1, 127, 128, 2 ** 29 + 3, n - 1], device=cuda)
+    gen = torch.Generator().manual_seed(43)
+    few = [randn(gen, 1, 6, dtype=BF).to(cuda), randn(gen, 6, 8, dtype=BF).to(cuda), randn(gen, 1, 2, 6, dtype=BF).to(cuda)]
+    x, weight, a = (torch.zeros(s, dtype=BF, device=cuda) for s in ((1, n), (n, 8), (1, 2, n)))
+    x[:, at], weight[at], a[:, :, at] = few
+    b = randn(gen, 1, 3, 8, dtype=BF).to(cuda)
+    check_linear(lowrank_linear(x, weight, a, b), few[0], few[1], few[2], b)

@@ -449,7 +449,7 @@ void plan_linear(Linear& q) {
   q.splits = (int)splits_for(tiles, q.K);
   const int64_t per = (q.K + q.splits - 1) / q.splits;
   q.k_per_split = per > 0 ? (int)((per + BK - 1) / BK * BK) : BK;
-  q.splits = (q.K + q.k_per_split - 1) / q.k_per_split;
+  q.splits = (int)(((int64_t)q.K + q.k_per_split - 1) / q.k_per_split);
   if (q.splits < 1) q.splits = 1;
 }
 

@@ -509,7 +509,7 @@ void linear_mfma_plan(Linear& q, int elem) {
   }
   if (s <= 1) return;
   q.k_per_split = (int)(((q.K + s - 1) / s + bk - 1) / bk * bk);
-  q.splits = (q.K + q.k_per_split - 1) / q.k_per_split;
+  q.splits = (int)(((int64_t)q.K + q.k_per_split - 1) / q.k_per_split);
 }
 
 template <typename T>

@@ -64,6 +64,16 @@ def test_few_rows_of_very_many_inputs(dtype):
         assert kernel_of(dtype, 1, 4, many, n_out, 2) == 16
 
 
+@needs_library
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_divided_inputs_near_2_to_31(dtype):
+    """The parts of K are counted without passing 2^31: tiles of 16 and 64 rows and those of any size have room for all their parts."""
+    n = 2 ** 31 - 2 ** 17
+    for rows, n_out, kernel, parts in ((4, 8, 16, 512), (100, 8, 64, 256), (5, 7, 0, 256)):
+        assert kernel_of(dtype, rows, 1, n, n_out, 1) == kernel
+        assert linear_workspace(rows, n, n_out, 1, dtype, pop=rows) >= parts * rows * n_out
+
+
 def test_refuses_features_near_2_to_31():
     """Tiles are counted in 32 bits beyond a tensor's last feature."""
     n = 2 ** 31 - 2 ** 16

@@ -24,6 +24,7 @@ from ._util import DTYPE_CODE, check, hip, launch_device, stream_of
 
 ALIGN = 256
 BLOCK = 32
+_MOST = (2 ** 32 - 1) // 256 * 1024               # elements of a leaf on a GPU: 1024 a workgroup, whose threads are counted in 32 bits
 _PHASE, _STEP_MU, _STEP_NU = 0x9E3779B9, 0x91E10DA5, 0xC13FA9A9
 
 P, I, I64 = _native.P, _native.I, _native.I64
@@ -89,7 +90,8 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], st
     ``params`` and ``grads`` are lists of float32 or bfloat16 tensors of pairwise equal shapes (any strides; types may differ
     from leaf to leaf and between a parameter and its gradient), ``decay`` says for each leaf whether ``weight_decay`` applies
     to it (default: to all).  Arithmetic is float32 whatever the types, results have the parameters' types and are contiguous.
-    Nothing is written in place, no autograd graph is built.  On a GPU all leaves take one launch per 72 of them."""
+    Nothing is written in place, no autograd graph is built.  On a GPU all leaves take one launch per 72 of them, and
+    a leaf holds fewer than 2^34 elements."""
     if len(params) != len(grads):
         raise ValueError(f"adamw: {len(params)} parameters but {len(grads)} gradients")
     if decay is not None and len(decay) != len(params):
@@ -113,6 +115,8 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], st
         _check_leaves(params, "params")
         _check_leaves(grads, "grads")
         raise
+    if total > _MOST and where >= 0 and max(sizes) > _MOST:
+        raise ValueError(f"adamw: a tensor of {max(sizes)} elements is more than one launch holds ({_MOST})")
     device = params[0].device
     bits = _check_state(state, device, total)
     hyper = (learning_rate, b1, b2, 1 - b1, 1 - b2, eps, weight_decay, math.log(b1) if b1 else -math.inf,
